@@ -1,0 +1,121 @@
+// paged.cuh — what the paged-cache kernels share: the cache's addressing, the visibility of keys, and the
+// argument checks of their entry points.
+#pragma once
+#include "common.cuh"
+
+namespace lthn {
+
+// lthn_paged_kv with its default strides filled in.
+struct PagedCache {
+    uint16_t* k;
+    uint16_t* v;
+    const int32_t* table;
+    int64_t page_stride, row_stride, head_stride;
+    int pages, page_size, table_stride, seqs, kv_heads;
+    int capacity;        // rows the table can name for a sequence
+    uint32_t* status;
+};
+
+// Score options with the defaults filled in. Scores are kept in units of log2, so that a weight is one ex2.
+struct AttnOpts {
+    float scale;         // softmax scale
+    float softcap;       // 0: none
+    const float* slopes;
+    int window;          // 0: none
+    const int32_t* prefix;
+};
+
+// Host: checks of the arguments every call has, and the fill-in. `name` is the entry point, for messages.
+int32_t paged_check_cache(const char* name, const lthn_paged_kv* c, PagedCache* out);
+int32_t paged_check_options(const char* name, const lthn_attn_options* o, int head_dim, AttnOpts* out);
+// the pointer is device memory of the current device (a host pointer or another GPU's would fault in the kernel)
+int32_t paged_check_device(const char* name, const char* what, const void* p);
+int paged_sm_count();
+
+#ifdef __CUDACC__
+// Element offset of kv head 0 of position pos of sequence seq, or -1 (and the status bit) for a page outside the pool.
+__device__ __forceinline__ int64_t paged_offset(const PagedCache& c, int page, int in_page) {
+    if ((unsigned)page >= (unsigned)c.pages) {
+        atomicOr(c.status, LTHN_STATUS_PAGED);
+        return -1;
+    }
+    return page * c.page_stride + in_page * c.row_stride;
+}
+
+// a sequence's length, cut at what the table can name
+__device__ __forceinline__ int paged_length(const PagedCache& c, int len) {
+    if (len > c.capacity) {
+        atomicOr(c.status, LTHN_STATUS_PAGED);
+        return c.capacity;
+    }
+    return max(len, 0);
+}
+
+// The key tiles (of TILE keys) that queries at positions [q0, q1] of a sequence may look at: tiles [0, na) hold the
+// prefix, tiles [b, b + n - na) the rest; piece i of n is tile i (i < na) or b + i - na.
+struct KeyTiles {
+    int na, b, n;
+    __device__ __forceinline__ int tile(int i) const { return i < na ? i : b + i - na; }
+};
+template <int TILE>
+__device__ __forceinline__ KeyTiles key_tiles(int q0, int q1, int len, int prefix, int window) {
+    KeyTiles t;
+    const int p = min(max(prefix, 0), len);
+    t.na = (p + TILE - 1) / TILE;
+    const int lo = window > 0 ? max(0, q0 - window + 1) : 0;   // first key the oldest query's window holds
+    const int hi = min(q1 + 1, len);                           // behind the last key the newest query sees
+    t.b = max(t.na, lo / TILE);
+    t.n = t.na + max(0, (hi + TILE - 1) / TILE - t.b);
+    return t;
+}
+
+// Inclusive scan over the block of one count per thread; returns the total. sh: one word per warp.
+template <int WARPS>
+__device__ __forceinline__ int paged_block_scan(int v, int& incl, int* sh) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
+    }
+    __syncthreads();
+    if (lane == 31) sh[warp] = incl;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) {
+        if (w < warp) incl += sh[w];
+        total += sh[w];
+    }
+    return total;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 16 bytes global -> shared; bytes = 0 writes zeros and reads nothing
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void paged_cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void paged_cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+#endif
+
+}  // namespace lthn

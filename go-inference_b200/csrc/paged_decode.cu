@@ -1,0 +1,577 @@
+// paged_decode.cu — attention of one new token per sequence over the paged KV cache, split over the length and joined.
+//
+//   out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),   s_j = cap(q.k_j scale) - slope |i - j|,   m = max_j s_j
+//
+// Every visible K and V row has to be read once: 4*D bytes per key and kv head against 4*D*G flops (G query heads share a
+// kv head), so HBM is the bound as long as the arithmetic of a group of query heads stays below it. With 8 or more query
+// heads per kv head it does not on the FMA pipe (G/2 multiply-adds per byte), so the products run on mma.sync with the query heads
+// as the M rows, where up to 16 heads cost what one costs.
+//
+// Work. The pieces (64 keys) of all (row, kv head, bundle of query heads) triples form one list, row by row; CTA c of C takes pieces
+// [U c / C, U (c+1) / C) of the U, so every CTA has the same work whatever the lengths are, and no host knowledge of
+// them is needed. A triple that lies within one CTA is finished there; otherwise each CTA that holds part of it leaves (max, sum,
+// unnormalised output) in its slot of the workspace - a CTA has at most two such parts, its first and its last - and
+// a second kernel joins them.
+//
+// A warp owns 16 keys of each piece and runs on its own: its own ring of shared-memory stages filled by its own cp.async (16 bytes,
+// rows padded by 16 bytes so that ldmatrix is free of bank conflicts), its own running maximum, sum and output; the
+// four warps meet at the end of a triple only. Rows outside the visible range are filled with zeros instead of
+// read: they may hold NaN, which a weight of zero would not silence.
+//
+// Types. K and V are exact in bf16. Bundles of up to 8 heads leave half of the 16 MMA rows free, and the free rows carry
+// what rounding to bf16 cuts off:
+//   bf16, <= 8 heads   rows 0-7 the weights rounded to bf16, rows 8-15 the remainders: the weights are good to 2^-17
+//   bf16, > 8 heads    16 heads, weights rounded to bf16 (2^-9 each, no more than the rounding of the output)
+//   f32                q and the weights as three bf16 parts (24 bits), two MMAs: rows 0-7 high, 8-15 middle; rows 0-7 low
+#include "paged.cuh"
+
+#include <algorithm>
+#include <mutex>
+
+namespace lthn {
+
+enum { DEC_BF16_16 = 0, DEC_BF16_8 = 1, DEC_F32_8 = 2 };
+
+struct DecodeArgs {
+    PagedCache c;
+    AttnOpts o;
+    const void* q;
+    void* out;
+    int64_t q_stride, out_stride;
+    const int32_t* lens;
+    float* lse;
+    int rows, Hq, G;      // G: query heads per kv head
+    int nb;               // bundles per kv head
+    int ctas;
+    float* part;          // [2*ctas][HB][D] unnormalised outputs
+    float2* ml;           // [2*ctas][HB] maximum (log2 units) and sum
+    int2* desc;           // [rows][kv_heads*nb] first and last CTA of a triple that several CTAs hold, (-1, .) otherwise
+};
+
+constexpr int DEC_WARPS = 4;
+constexpr int DEC_THREADS = DEC_WARPS * 32;
+constexpr int DEC_WK = 16;                       // keys of a warp's tile
+constexpr int DEC_TILE = DEC_WARPS * DEC_WK;
+
+template <int D, int MODE>
+struct DecCfg {
+    static constexpr int HB = MODE == DEC_BF16_16 ? 16 : 8;
+    static constexpr int NST = D == 64 ? 4 : 3;
+    static constexpr int PITCH = D * 2 + 16;                    // bytes of a shared-memory row
+    static constexpr int STAGE = 2 * DEC_WK * PITCH;            // K rows, then V rows
+    static constexpr int QROWS = MODE == DEC_F32_8 ? 24 : MODE == DEC_BF16_16 ? 16 : 8;
+    static constexpr int Q_BYTES = QROWS * PITCH;
+    static constexpr int RING = DEC_WARPS * NST * STAGE;
+    static constexpr size_t SMEM = (size_t)RING + Q_BYTES;
+    static constexpr int CTAS_PER_SM = D == 256 ? 1 : 2;
+    static_assert(HB * D * 4 <= NST * STAGE, "a warp's ring holds its output for the join");
+};
+
+__device__ __forceinline__ KeyTiles decode_tiles(const DecodeArgs& a, int row) {
+    const int len = paged_length(a.c, a.lens[row]);
+    return key_tiles<DEC_TILE>(len - 1, len - 1, len, a.o.prefix ? a.o.prefix[row] : 0, a.o.window);
+}
+
+// capped, biased score in log2 units. x: the raw product
+__device__ __forceinline__ float decode_score(const AttnOpts& o, float x, float slope, int gap) {
+    constexpr float LOG2E = 1.4426950408889634f;
+    x *= o.scale;
+    if (o.softcap > 0.f) x = o.softcap * tanhf(x / o.softcap);
+    if (o.slopes) x -= slope * (float)abs(gap);
+    return x * LOG2E;
+}
+
+template <int D, int MODE>
+__global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) paged_decode_kernel(const DecodeArgs a) {
+    using C = DecCfg<D, MODE>;
+    constexpr int HB = C::HB, NST = C::NST, PITCH = C::PITCH;
+    constexpr int KS = D / 16;                    // k-steps of q.k
+    constexpr int ND = D / 8;                     // output n-tiles
+    extern __shared__ __align__(128) unsigned char dec_smem[];
+    __shared__ float s_m[DEC_WARPS][16], s_l[DEC_WARPS][16];
+    __shared__ int s_scan[DEC_WARPS];
+    __shared__ int s_row, s_base;
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int g = lane >> 2, t = lane & 3;
+    unsigned char* q_sm = dec_smem + C::RING;
+    const uint32_t q_addr = smem_u32(q_sm);
+    const uint32_t ring = smem_u32(dec_smem) + warp * NST * C::STAGE;
+    const int triples = a.c.kv_heads * a.nb;      // per row
+
+    pdl_trigger();
+    // ---- this CTA's pieces -----------------------------------------------------------------------
+    int64_t U = 0;                                // in tiles of rows first, times the triples of a row
+    for (int r0 = 0; r0 < a.rows; r0 += DEC_THREADS) {
+        int incl;
+        const int r = r0 + tid;
+        U += paged_block_scan<DEC_WARPS>(r < a.rows ? decode_tiles(a, r).n : 0, incl, s_scan);
+    }
+    U *= triples;
+    const int ctas = (int)min((int64_t)a.ctas, U);   // none of them without a piece
+    if ((int)blockIdx.x >= ctas) return;
+    const int64_t u0 = U * blockIdx.x / ctas, u1 = U * (blockIdx.x + 1) / ctas;
+    // the row that holds piece u0
+    int64_t base = 0;
+    int row = 0;
+    for (int r0 = 0; r0 < a.rows; r0 += DEC_THREADS) {
+        const int r = r0 + tid;
+        const int n = r < a.rows ? decode_tiles(a, r).n : 0;
+        int incl;
+        const int total = paged_block_scan<DEC_WARPS>(n, incl, s_scan);
+        if ((base + total) * triples > u0) {
+            if (n > 0 && (base + incl) * triples > u0 && (base + incl - n) * triples <= u0) { s_row = r; s_base = incl - n; }
+            __syncthreads();
+            row = s_row;
+            base = (base + s_base) * triples;     // first piece of the row
+            break;
+        }
+        base += total;
+    }
+
+    int64_t u = u0;
+    while (u < u1 && row < a.rows) {
+        const KeyTiles kt = decode_tiles(a, row);
+        if (kt.n == 0) { row++; continue; }
+        const int v = (int)(u - base);            // piece within the row
+        const int triple = v / kt.n, i0 = v - triple * kt.n;
+        const int count = (int)min((int64_t)(kt.n - i0), u1 - u);
+        const int kvh = triple / a.nb, bundle = triple - kvh * a.nb;
+        const int len = paged_length(a.c, a.lens[row]);
+        const int pos = len - 1;
+        const int prefix = a.o.prefix ? min(max(a.o.prefix[row], 0), len) : 0;
+        const int lo = a.o.window > 0 ? max(0, len - a.o.window) : 0;
+        const int h0 = kvh * a.G + bundle * HB;   // first query head
+        const int nh = min(HB, a.G - bundle * HB);
+        const uint16_t* kbase = a.c.k + kvh * a.c.head_stride;
+        const uint16_t* vbase = a.c.v + kvh * a.c.head_stride;
+        const int32_t* trow = a.c.table + (int64_t)row * a.c.table_stride;
+
+        __syncthreads();                          // the ring and the query area are free
+        // ---- queries -----------------------------------------------------------------------------
+        for (int i = tid; i < HB * (D / 8); i += DEC_THREADS) {
+            const int h = i / (D / 8), c = i - h * (D / 8);
+            unsigned char* dst = q_sm + h * PITCH + c * 16;
+            if (MODE == DEC_F32_8) {
+                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (h < nh) {
+                    const float* src = (const float*)a.q + row * a.q_stride + (int64_t)(h0 + h) * D + c * 8;
+                    const float4 p = *(const float4*)src, r = *(const float4*)(src + 4);
+                    x[0] = p.x; x[1] = p.y; x[2] = p.z; x[3] = p.w; x[4] = r.x; x[5] = r.y; x[6] = r.z; x[7] = r.w;
+                }
+#pragma unroll
+                for (int part = 0; part < 3; part++) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        w[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
+                        x[2 * e] -= __uint_as_float(w[e] << 16);
+                        x[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
+                    }
+                    *(uint4*)(dst + part * 8 * PITCH) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            } else {
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (h < nh) x = *(const uint4*)((const uint16_t*)a.q + row * a.q_stride + (int64_t)(h0 + h) * D + c * 8);
+                *(uint4*)dst = x;
+            }
+        }
+        __syncthreads();
+        float slope[2] = {0.f, 0.f};
+        if (a.o.slopes) {
+            if (g < nh) slope[0] = a.o.slopes[h0 + g];
+            if (HB == 16 && g + 8 < nh) slope[1] = a.o.slopes[h0 + g + 8];
+        }
+
+        // ---- loads: piece i of the triple into stage i % NST ---------------------------------------
+        // lanes 0-15 keep the page of "their" key of the next piece to be loaded, fetched one piece ahead
+        auto my_key = [&](int i) {                // -1: not visible (its row is zeros)
+            const int key = kt.tile(i) * DEC_TILE + warp * DEC_WK + lane;
+            return lane < DEC_WK && key < len && (key < prefix || key >= lo) ? key : -1;
+        };
+        auto page_of = [&](int i) {
+            const int key = i < i0 + count ? my_key(i) : -1;
+            return key >= 0 ? trow[key / a.c.page_size] : 0;
+        };
+        auto issue = [&](int i, int page) {
+            if (i < i0 + count) {
+                const int key = my_key(i);
+                const int64_t off = key >= 0 ? paged_offset(a.c, page, key % a.c.page_size) : -1;
+                constexpr int CPR = D / 8;        // 16-byte chunks per row
+                constexpr int RPI = 32 / CPR > 0 ? 32 / CPR : 1;   // rows per instruction
+                const uint32_t st = ring + (i % NST) * C::STAGE;
+                const int c = lane % CPR;
+#pragma unroll
+                for (int r0 = 0; r0 < DEC_WK; r0 += RPI) {
+                    const int r = r0 + (RPI > 1 ? lane / CPR : 0);
+                    const int64_t o = __shfl_sync(0xffffffffu, off, r);
+                    const int64_t e = (o < 0 ? 0 : o) + c * 8;
+                    const int n = o < 0 ? 0 : 16;
+                    cp_async16_zfill(st + r * PITCH + c * 16, kbase + e, n);
+                    cp_async16_zfill(st + (DEC_WK + r) * PITCH + c * 16, vbase + e, n);
+                }
+            }
+            paged_cp_commit();
+        };
+        float acc[ND][4];
+#pragma unroll
+        for (int n = 0; n < ND; n++) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+        float mrun[2] = {-INFINITY, -INFINITY}, lrun[2] = {0.f, 0.f};
+        int page = page_of(i0);
+#pragma unroll
+        for (int s = 0; s < NST - 1; s++) {
+            const int next = page_of(i0 + s + 1);
+            issue(i0 + s, page);
+            page = next;
+        }
+
+        for (int i = i0; i < i0 + count; i++) {
+            const int next = page_of(i + NST);
+            paged_cp_wait<NST - 2>();
+            __syncwarp();                         // piece i has landed for every lane; nobody still reads the stage that is filled next
+            issue(i + NST - 1, page);
+            page = next;
+            const uint32_t kst = ring + (i % NST) * C::STAGE, vst = kst + DEC_WK * PITCH;
+            const int mi = lane >> 3;
+            // ---- scores: c[n][e], n-tile n = keys 8n.., e: row g (e < 2) or g + 8, key 2t + (e & 1) ----
+            float c[2][4] = {}, c2[2][4] = {};
+#pragma unroll
+            for (int kk = 0; kk < KS; kk++) {
+                uint32_t kb[4];
+                ldmatrix_x4(kb, kst + ((mi >> 1) * 8 + (lane & 7)) * PITCH + kk * 32 + (mi & 1) * 16);
+                uint32_t qa[4];
+                if (MODE == DEC_BF16_8) {
+                    // rows 0-7 only: the address lanes of the two upper matrices repeat the lower ones
+                    ldmatrix_x4(qa, q_addr + (lane & 7) * PITCH + kk * 32 + (lane >> 4) * 16);
+                    mma_bf16_16816(c[0], qa[0], 0u, qa[2], 0u, kb[0], kb[1]);
+                    mma_bf16_16816(c[1], qa[0], 0u, qa[2], 0u, kb[2], kb[3]);
+                } else {
+                    ldmatrix_x4(qa, q_addr + (lane & 15) * PITCH + kk * 32 + (lane >> 4) * 16);
+                    mma_bf16_16816(c[0], qa[0], qa[1], qa[2], qa[3], kb[0], kb[1]);
+                    mma_bf16_16816(c[1], qa[0], qa[1], qa[2], qa[3], kb[2], kb[3]);
+                }
+                if (MODE == DEC_F32_8) {
+                    ldmatrix_x4(qa, q_addr + (16 + (lane & 7)) * PITCH + kk * 32 + (lane >> 4) * 16);
+                    mma_bf16_16816(c2[0], qa[0], 0u, qa[2], 0u, kb[0], kb[1]);
+                    mma_bf16_16816(c2[1], qa[0], 0u, qa[2], 0u, kb[2], kb[3]);
+                }
+            }
+            const int key0 = kt.tile(i) * DEC_TILE + warp * DEC_WK;
+            constexpr int NR = MODE == DEC_BF16_16 ? 2 : 1;   // head rows of this thread
+            float p[NR][4];                                   // [row][n-tile*2 + key]
+            float mx[NR];
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                mx[r] = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int n = e >> 1, x = e & 1, key = key0 + n * 8 + 2 * t + x;
+                    float s = c[n][2 * r + x];
+                    if (MODE == DEC_F32_8) s += c[n][2 + x] + c2[n][x];
+                    s = decode_score(a.o, s, slope[r], pos - key);
+                    p[r][e] = key < len && (key < prefix || key >= lo) ? s : -INFINITY;
+                    mx[r] = fmaxf(mx[r], p[r][e]);
+                }
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+            }
+            bool grew = false;
+            float alpha[NR];
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                const float m = fmaxf(mrun[r], mx[r]);
+                const float ref = m == -INFINITY ? 0.f : m;   // no visible key yet: keep ex2 finite
+                alpha[r] = ex2(mrun[r] - ref);                // -inf -> 0
+                grew |= m != mrun[r];
+                mrun[r] = m;
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    p[r][e] = ex2(p[r][e] - ref);
+                    sum += p[r][e];
+                }
+                lrun[r] = lrun[r] * alpha[r] + sum;
+            }
+            if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+                for (int n = 0; n < ND; n++) {
+                    acc[n][0] *= alpha[0]; acc[n][1] *= alpha[0];
+                    acc[n][2] *= alpha[NR - 1]; acc[n][3] *= alpha[NR - 1];
+                }
+            }
+            // ---- weights as MMA rows ----------------------------------------------------------------------
+            uint32_t w0[2], w1[2], w2[2];                     // [n-tile]: rows 0-7, rows 8-15, the second MMA's rows 0-7
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                w0[n] = pack_bf16x2(p[0][2 * n], p[0][2 * n + 1]);
+                w2[n] = 0u;
+                if (MODE == DEC_BF16_16) {
+                    w1[n] = pack_bf16x2(p[NR - 1][2 * n], p[NR - 1][2 * n + 1]);
+                } else {
+                    const float r0 = p[0][2 * n] - __uint_as_float(w0[n] << 16), r1 = p[0][2 * n + 1] - __uint_as_float(w0[n] & 0xffff0000u);
+                    w1[n] = pack_bf16x2(r0, r1);
+                    if (MODE == DEC_F32_8) w2[n] = pack_bf16x2(r0 - __uint_as_float(w1[n] << 16), r1 - __uint_as_float(w1[n] & 0xffff0000u));
+                }
+            }
+#pragma unroll
+            for (int d2 = 0; d2 < D / 16; d2++) {
+                uint32_t vb[4];
+                ldmatrix_x4_trans(vb, vst + ((mi & 1) * 8 + (lane & 7)) * PITCH + d2 * 32 + (mi >> 1) * 16);
+                mma_bf16_16816(acc[2 * d2], w0[0], w1[0], w0[1], w1[1], vb[0], vb[1]);
+                mma_bf16_16816(acc[2 * d2 + 1], w0[0], w1[0], w0[1], w1[1], vb[2], vb[3]);
+                if (MODE == DEC_F32_8) {
+                    mma_bf16_16816(acc[2 * d2], w2[0], 0u, w2[1], 0u, vb[0], vb[1]);
+                    mma_bf16_16816(acc[2 * d2 + 1], w2[0], 0u, w2[1], 0u, vb[2], vb[3]);
+                }
+            }
+            __syncwarp();                                     // the stage may be refilled
+        }
+        paged_cp_wait<0>();
+
+        // ---- join the four warps --------------------------------------------------------------------------
+        __syncwarp();
+        float* red = (float*)(dec_smem + warp * NST * C::STAGE);   // this warp's ring, [HB][D]
+        constexpr int NR = MODE == DEC_BF16_16 ? 2 : 1;
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            float l = lrun[r];
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+            if (t == 0) { s_m[warp][g + 8 * r] = mrun[r]; s_l[warp][g + 8 * r] = l; }
+        }
+#pragma unroll
+        for (int n = 0; n < ND; n++) {
+            if (MODE == DEC_BF16_16) {
+                *(float2*)(red + g * D + n * 8 + 2 * t) = make_float2(acc[n][0], acc[n][1]);
+                *(float2*)(red + (g + 8) * D + n * 8 + 2 * t) = make_float2(acc[n][2], acc[n][3]);
+            } else {
+                *(float2*)(red + g * D + n * 8 + 2 * t) = make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]);
+            }
+        }
+        __syncthreads();
+        const bool whole = count == kt.n;
+        const int slot = 2 * blockIdx.x + (i0 > 0 ? 0 : 1);
+        for (int idx = tid; idx < nh * (D / 4); idx += DEC_THREADS) {
+            const int h = idx / (D / 4), d = (idx - h * (D / 4)) * 4;
+            float m = s_m[0][h];
+#pragma unroll
+            for (int w = 1; w < DEC_WARPS; w++) m = fmaxf(m, s_m[w][h]);
+            const float ref = m == -INFINITY ? 0.f : m;
+            float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < DEC_WARPS; w++) {
+                const float e = ex2(s_m[w][h] - ref);
+                const float4 y = *(const float4*)((const float*)(dec_smem + w * NST * C::STAGE) + h * D + d);
+                l = fmaf(s_l[w][h], e, l);
+                x[0] = fmaf(y.x, e, x[0]); x[1] = fmaf(y.y, e, x[1]); x[2] = fmaf(y.z, e, x[2]); x[3] = fmaf(y.w, e, x[3]);
+            }
+            if (whole) {
+                const float inv = l > 0.f ? 1.0f / l : 0.f;
+                const int64_t at = row * a.out_stride + (int64_t)(h0 + h) * D + d;
+                if (MODE == DEC_F32_8) *(float4*)((float*)a.out + at) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+                else *(uint2*)((uint16_t*)a.out + at) = make_uint2(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv));
+                if (a.lse && d == 0) a.lse[(int64_t)row * a.Hq + h0 + h] = (m + log2f(l)) * 0.6931471805599453f;
+            } else {
+                *(float4*)(a.part + ((int64_t)slot * HB + h) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+                if (d == 0) a.ml[slot * HB + h] = make_float2(m, l);
+            }
+        }
+        if (i0 == 0 && tid == 0) {
+            // the CTAs that hold the rest: the last piece u - i0 + n - 1 lies in CTA ceil((u + n) C / U) - 1
+            const int last = (int)(((u + kt.n) * ctas + U - 1) / U) - 1;
+            a.desc[(int64_t)row * triples + triple] = make_int2(whole ? -1 : (int)blockIdx.x, last);
+        }
+        u += count;
+        if (u - base >= (int64_t)kt.n * triples) { base += (int64_t)kt.n * triples; row++; }
+    }
+}
+
+// Joins the parts of triples that several CTAs hold, and writes the rows that see nothing. One CTA per (row, query head); warp w
+// takes parts w, w+4, ... with a running maximum, four loads in flight.
+template <int D>
+__global__ void __launch_bounds__(128) paged_decode_join_kernel(const DecodeArgs a, int HB, int out_f32) {
+    pdl_wait();
+    constexpr int DL = D / 32;
+    __shared__ float sm[4], sl[4];
+    __shared__ float so[4][D];
+    const int row = blockIdx.y, qh = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    float* of = (float*)a.out + row * a.out_stride + (int64_t)qh * D;
+    uint16_t* ob = (uint16_t*)a.out + row * a.out_stride + (int64_t)qh * D;
+    if (a.lens[row] <= 0 || a.c.capacity == 0) {
+        for (int d = tid; d < D; d += 128) {
+            if (out_f32) of[d] = 0.f;
+            else ob[d] = 0;
+        }
+        if (a.lse && tid == 0) a.lse[(int64_t)row * a.Hq + qh] = -INFINITY;
+        return;
+    }
+    const int kvh = qh / a.G, in = qh - kvh * a.G, bundle = in / HB, h = in - bundle * HB;
+    const int2 ds = a.desc[((int64_t)row * a.c.kv_heads + kvh) * a.nb + bundle];
+    if (ds.x < 0) return;
+    float m = -INFINITY, l = 0.f, acc[DL];
+#pragma unroll
+    for (int i = 0; i < DL; i++) acc[i] = 0.f;
+    constexpr int B = 4;
+    for (int c0 = ds.x + warp; c0 <= ds.y; c0 += 4 * B) {
+        float2 ml[B];
+        float2 x[B][DL / 2];
+#pragma unroll
+        for (int b = 0; b < B; b++) {
+            const int c = c0 + 4 * b;
+            const bool live = c <= ds.y;
+            const int64_t at = (int64_t)(2 * (live ? c : c0) + ((live ? c : c0) == ds.x ? 1 : 0)) * HB + h;
+            ml[b] = live ? a.ml[at] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int i = 0; i < DL / 2; i++) x[b][i] = ((const float2*)(a.part + at * D))[lane + 32 * i];
+        }
+        float nm = m;
+#pragma unroll
+        for (int b = 0; b < B; b++) nm = fmaxf(nm, ml[b].x);
+        if (nm == -INFINITY) continue;
+        const float e0 = ex2(m - nm);
+        l *= e0;
+#pragma unroll
+        for (int i = 0; i < DL; i++) acc[i] *= e0;
+#pragma unroll
+        for (int b = 0; b < B; b++) {
+            const float e = ex2(ml[b].x - nm);
+            l = fmaf(ml[b].y, e, l);
+#pragma unroll
+            for (int i = 0; i < DL / 2; i++) {
+                acc[2 * i] = fmaf(x[b][i].x, e, acc[2 * i]);
+                acc[2 * i + 1] = fmaf(x[b][i].y, e, acc[2 * i + 1]);
+            }
+        }
+        m = nm;
+    }
+    if (lane == 0) { sm[warp] = m; sl[warp] = l; }
+#pragma unroll
+    for (int i = 0; i < DL / 2; i++) *(float2*)&so[warp][2 * (lane + 32 * i)] = make_float2(acc[2 * i], acc[2 * i + 1]);
+    __syncthreads();
+    const float gm = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+    const float ref = gm == -INFINITY ? 0.f : gm;
+    float e[4], den = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) { e[w] = ex2(sm[w] - ref); den = fmaf(sl[w], e[w], den); }
+    const float inv = den > 0.f ? 1.0f / den : 0.f;
+    for (int d = tid; d < D; d += 128) {
+        const float o = (so[0][d] * e[0] + so[1][d] * e[1] + so[2][d] * e[2] + so[3][d] * e[3]) * inv;
+        if (out_f32) of[d] = o;
+        else ob[d] = f32_to_bf16_bits(o);
+    }
+    if (a.lse && tid == 0) a.lse[(int64_t)row * a.Hq + qh] = (gm + log2f(den)) * 0.6931471805599453f;
+}
+
+// Bundles of heads: f32 always 8 (three bf16 parts of q and of the weights fill the MMA rows), bf16 8 where that
+// holds the whole group and 16 otherwise (twice the heads per pass over the keys).
+static int decode_mode(int dtype, int G) { return dtype == LTHN_DTYPE_F32 ? DEC_F32_8 : G <= 8 ? DEC_BF16_8 : DEC_BF16_16; }
+static int decode_bundle(int mode) { return mode == DEC_BF16_16 ? 16 : 8; }
+
+struct DecodePlan { int mode, HB, nb, ctas; size_t part, ml, desc, total; };
+static DecodePlan decode_plan(int D, int kv_heads, int rows, int q_heads, int dtype) {
+    DecodePlan p;
+    const int G = q_heads / kv_heads;
+    p.mode = decode_mode(dtype, G);
+    p.HB = decode_bundle(p.mode);
+    p.nb = (G + p.HB - 1) / p.HB;
+    p.ctas = paged_sm_count() * (D == 256 ? 1 : 2);
+    auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    p.part = up((size_t)2 * p.ctas * p.HB * D * 4);
+    p.ml = up((size_t)2 * p.ctas * p.HB * 8);
+    p.desc = up((size_t)rows * kv_heads * p.nb * 8);
+    p.total = p.part + p.ml + p.desc;
+    return p;
+}
+
+template <int D, int MODE>
+static int32_t launch_decode_kernel(cudaStream_t s, const DecodeArgs& a) {
+    using C = DecCfg<D, MODE>;
+    static uint32_t attr_devs = 0;
+    static std::mutex mu;
+    int dev = 0;
+    LTHN_CUDA_TRY(cudaGetDevice(&dev));
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        if (!(attr_devs >> (dev & 31) & 1)) {
+            LTHN_CUDA_TRY(cudaFuncSetAttribute(paged_decode_kernel<D, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+            attr_devs |= 1u << (dev & 31);
+        }
+    }
+    paged_decode_kernel<D, MODE><<<a.ctas, DEC_THREADS, C::SMEM, s>>>(a);
+    LTHN_CUDA_TRY(cudaGetLastError());
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.Hq, a.rows); cfg.blockDim = dim3(128); cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    LTHN_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_decode_join_kernel<D>, a, C::HB, MODE == DEC_F32_8 ? 1 : 0));
+    return LTHN_OK;
+}
+template <int D>
+static int32_t launch_decode_mode(cudaStream_t s, const DecodeArgs& a, int mode) {
+    if (mode == DEC_BF16_16) return launch_decode_kernel<D, DEC_BF16_16>(s, a);
+    if (mode == DEC_BF16_8) return launch_decode_kernel<D, DEC_BF16_8>(s, a);
+    return launch_decode_kernel<D, DEC_F32_8>(s, a);
+}
+
+}  // namespace lthn
+
+using namespace lthn;
+
+static int32_t decode_check(const lthn_paged_kv* cache, int32_t rows, int32_t q_heads, int32_t dtype, PagedCache* c) {
+    int32_t rc;
+    if ((rc = paged_check_cache("paged_sdpa_decode", cache, c))) return rc;
+    LTHN_REQUIRE(dtype == LTHN_DTYPE_F32 || dtype == LTHN_DTYPE_BF16, "paged_sdpa_decode: dtype must be f32 or bf16");
+    LTHN_REQUIRE(rows >= 0 && rows <= 65535, "paged_sdpa_decode: rows must be in [0, 65535]");
+    LTHN_REQUIRE(rows <= cache->seqs, "paged_sdpa_decode: more rows than the page table has sequences");
+    LTHN_REQUIRE(q_heads > 0 && q_heads <= 65535 && q_heads % cache->kv_heads == 0, "paged_sdpa_decode: q_heads must be a positive multiple of kv_heads");
+    return LTHN_OK;
+}
+
+extern "C" {
+
+int32_t lthn_paged_sdpa_decode_workspace(const lthn_paged_kv* cache, int32_t rows, int32_t q_heads, int32_t dtype, size_t* bytes) {
+    clear_error();
+    LTHN_REQUIRE(bytes != nullptr, "paged_sdpa_decode_workspace: bytes is NULL");
+    PagedCache c;
+    int32_t rc;
+    if ((rc = decode_check(cache, rows, q_heads, dtype, &c))) return rc;
+    *bytes = decode_plan(cache->head_dim, cache->kv_heads, rows, q_heads, dtype).total;
+    return LTHN_OK;
+}
+
+int32_t lthn_paged_sdpa_decode(void* stream, const lthn_paged_kv* cache, const lthn_attn_options* options, const void* q, int32_t dtype,
+                               int64_t q_stride, const int32_t* kv_lens, int32_t rows, int32_t q_heads, void* out, int64_t out_stride,
+                               float* lse, void* workspace, size_t workspace_bytes) {
+    clear_error();
+    const char* me = "paged_sdpa_decode";
+    DecodeArgs a = {};
+    int32_t rc;
+    if ((rc = decode_check(cache, rows, q_heads, dtype, &a.c))) return rc;
+    const int D = cache->head_dim;
+    if ((rc = paged_check_options(me, options, D, &a.o))) return rc;
+    if (rows == 0) return LTHN_OK;
+    LTHN_REQUIRE(q && out && kv_lens && workspace, "paged_sdpa_decode: NULL pointer");
+    a.q_stride = q_stride ? q_stride : (int64_t)q_heads * D;
+    a.out_stride = out_stride ? out_stride : (int64_t)q_heads * D;
+    LTHN_REQUIRE(((a.q_stride | a.out_stride) & 7) == 0, "paged_sdpa_decode: strides must be multiples of 8 elements");
+    LTHN_REQUIRE(a.out_stride >= (int64_t)q_heads * D, "paged_sdpa_decode: rows of out would overlap");
+    LTHN_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15) == 0, "paged_sdpa_decode: q, out and workspace must be 16-byte aligned");
+    const DecodePlan p = decode_plan(D, cache->kv_heads, rows, q_heads, dtype);
+    LTHN_REQUIRE(workspace_bytes >= p.total, "paged_sdpa_decode: workspace too small");
+    if ((rc = paged_check_device(me, "the cache", cache->k))) return rc;
+    if ((rc = paged_check_device(me, "workspace", workspace))) return rc;
+    a.q = q; a.out = out; a.lens = kv_lens; a.lse = lse; a.rows = rows; a.Hq = q_heads; a.G = q_heads / cache->kv_heads;
+    a.nb = p.nb; a.ctas = p.ctas;
+    a.part = (float*)workspace;
+    a.ml = (float2*)((char*)workspace + p.part);
+    a.desc = (int2*)((char*)workspace + p.part + p.ml);
+    a.c.status = device_paged_status_word();
+    if (!a.c.status) return fail(LTHN_ERR_CUDA, "paged_sdpa_decode: no device status word");
+    if (D == 64) return launch_decode_mode<64>((cudaStream_t)stream, a, p.mode);
+    if (D == 128) return launch_decode_mode<128>((cudaStream_t)stream, a, p.mode);
+    return launch_decode_mode<256>((cudaStream_t)stream, a, p.mode);
+}
+
+}  // extern "C"

@@ -41,6 +41,13 @@ uint32_t* device_status_word() {
     return g_status[dev];
 }
 
+// The word next to it collects LTHN_STATUS_PAGED, so that a caller's bad page table is not taken for a
+// failed wait by the engine objects, which judge the first word after every forward.
+uint32_t* device_paged_status_word() {
+    uint32_t* w = device_status_word();
+    return w ? w + 1 : nullptr;
+}
+
 int32_t check_device_status(cudaStream_t s) {
     uint32_t* w = device_status_word();
     if (!w) return fail(LTHN_ERR_CUDA, "no device status word");
@@ -171,11 +178,11 @@ int32_t lthn_device_status(void* stream, uint32_t* bits) {
     int dev = 0;
     LTHN_CUDA_TRY(cudaGetDevice(&dev));
     LTHN_REQUIRE(dev >= 0 && dev < kMaxDev, "lthn_device_status: device index out of range");
-    uint32_t* words[5];
+    uint32_t* words[6];
     int n = 0;
     {
         std::lock_guard<std::mutex> lk(g_mu);
-        if (g_status[dev]) words[n++] = g_status[dev];
+        if (g_status[dev]) { words[n++] = g_status[dev]; words[n++] = g_status[dev] + 1; }
         for (uint32_t* w : g_extra_status[dev]) if (w) words[n++] = w;
     }
     LTHN_CUDA_TRY(cudaStreamSynchronize(s));
@@ -191,6 +198,8 @@ int32_t lthn_device_status(void* stream, uint32_t* bits) {
         all |= v;
     }
     if (bits) *bits = all;
+    if (all == LTHN_STATUS_PAGED)
+        return fail(LTHN_ERR_INVALID, "a paged-cache call met a page, sequence, position or length outside its table");
     if (all) return fail(LTHN_ERR_DEVICE_WAIT, "a device-side bounded wait ran out (status " + std::to_string(all) + ")");
     return LTHN_OK;
 }

@@ -97,6 +97,23 @@ class ModelConfig(C.Structure):
                 ("rope_local_base", C.c_float)]
 
 
+class PagedKVDesc(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_table", C.c_void_p), ("page_stride", C.c_int64), ("row_stride", C.c_int64),
+                ("head_stride", C.c_int64), ("pages", C.c_int32), ("page_size", C.c_int32), ("table_stride", C.c_int32),
+                ("seqs", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class RopeParams(C.Structure):
+    _fields_ = [("inv_freq", C.c_void_p), ("rotary_dim", C.c_int32), ("interleaved", C.c_int32), ("q_norm", C.c_void_p),
+                ("k_norm", C.c_void_p), ("eps", C.c_float)]
+
+
+class AttnOptions(C.Structure):
+    _fields_ = [("scale", C.c_float), ("softcap", C.c_float), ("slopes", C.c_void_p), ("window", C.c_int32), ("prefix_lens", C.c_void_p)]
+
+
+STATUS_PAGED = 0x40000000
+
 _lib = None
 
 
@@ -168,6 +185,11 @@ class _Sig:
     lthn_debug_rmsnorm_gather_local = (i32, [vp, vp, i32, vp, vp, vp, vp, vp, i32, i32, f32, i32, C.c_uint32])
     lthn_rmsnorm_rope = (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, f32, f32, i32])
     lthn_sdpa_decode = (i32, [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i64, f32, i32])
+    lthn_paged_kv_append = (i32, [vp, C.POINTER(PagedKVDesc), C.POINTER(RopeParams), vp, vp, vp, i32, i64, i64, i64, vp, vp, i32, i32, vp, i32, i64])
+    lthn_paged_sdpa_decode_workspace = (i32, [C.POINTER(PagedKVDesc), i32, i32, i32, C.POINTER(sz)])
+    lthn_paged_sdpa_decode = (i32, [vp, C.POINTER(PagedKVDesc), C.POINTER(AttnOptions), vp, i32, i64, vp, i32, i32, vp, i64, vp, vp, sz])
+    lthn_paged_prefill_attention_workspace = (i32, [C.POINTER(PagedKVDesc), i32, i32, i32, i32, C.POINTER(sz)])
+    lthn_paged_prefill_attention = (i32, [vp, C.POINTER(PagedKVDesc), C.POINTER(AttnOptions), vp, i64, vp, vp, i32, i32, i32, i32, vp, i64, vp, vp, sz])
     lthn_argmax = (i32, [vp, vp, i32, i32, vp])
     lthn_model_create = (i32, [C.POINTER(ModelConfig), pvp])
     lthn_model_load_dir = (i32, [C.c_char_p, C.POINTER(LoadOptions), pvp])
@@ -510,6 +532,81 @@ def qmv_host(x_bf16: np.ndarray, packed: np.ndarray, scales: np.ndarray, biases:
     check(lib().lthn_affine_qmv_host(xb.ctypes.data, xb.size, pb.ctypes.data, pb.size, sb.ctypes.data, sb.size,
                                      bb.ctypes.data, bb.size, out_dim, in_dim, gs, bits, y.ctypes.data, y.nbytes))
     return y
+
+
+# ----------------------------------------------------------- paged KV cache ----
+# Device memory is a Buf or anything with data_ptr() (a tensor of another library); a stream is a Stream or a raw
+# cudaStream_t as an int.
+
+def _p(x):
+    if x is None:
+        return None
+    return x.ptr if isinstance(x, Buf) else x.data_ptr()
+
+
+def _raw(stream):
+    return stream.h if isinstance(stream, Stream) else stream
+
+
+class PagedKV:
+    """A paged cache: pools k and v of bf16 pages and the table of each sequence's pages (lthn_paged_kv). Strides of 0
+    are those of [pages, page_size, kv_heads, head_dim]. Keeps what it is given alive."""
+
+    def __init__(self, k, v, page_table, *, pages, page_size, kv_heads, head_dim, seqs, table_stride, page_stride=0, row_stride=0,
+                 head_stride=0):
+        self.desc = PagedKVDesc(_p(k), _p(v), _p(page_table), page_stride, row_stride, head_stride, pages, page_size, table_stride, seqs,
+                                kv_heads, head_dim)
+        self._keep = (k, v, page_table)
+
+
+def rope_inv_freq(base: float, head_dim: int, rotary_dim: int = 0) -> np.ndarray:
+    """f64 frequencies base^(-2i/head_dim) of the first rotary_dim/2 pairs (lthn_rmsnorm_rope's), for the device copy of rope_params."""
+    return float(base) ** (-2.0 * np.arange((rotary_dim or head_dim) // 2, dtype=np.float64) / head_dim)
+
+
+def rope_params(inv_freq=None, rotary_dim=0, interleaved=False, q_norm=None, k_norm=None, eps=1e-6) -> RopeParams:
+    p = RopeParams(_p(inv_freq), rotary_dim, int(interleaved), _p(q_norm), _p(k_norm), eps)
+    p._keep = (inv_freq, q_norm, k_norm)
+    return p
+
+
+def attn_options(scale=0.0, softcap=0.0, slopes=None, window=0, prefix_lens=None) -> AttnOptions:
+    o = AttnOptions(scale, softcap, _p(slopes), window, _p(prefix_lens))
+    o._keep = (slopes, prefix_lens)
+    return o
+
+
+def paged_kv_append(cache: PagedKV, k, v, row_seq, row_pos, rows, dtype, *, rope: RopeParams = None, q=None, q_heads=0, q_out=None,
+                    out_dtype=None, q_stride=0, k_stride=0, v_stride=0, q_out_stride=0, stream=None):
+    """Rows of k and v (and q) through norm and rotation into the cache (and q_out)."""
+    check(lib().lthn_paged_kv_append(_raw(stream), cache.desc, rope, _p(q), _p(k), _p(v), dtype, q_stride, k_stride, v_stride, _p(row_seq),
+                                     _p(row_pos), rows, q_heads, _p(q_out), dtype if out_dtype is None else out_dtype, q_out_stride))
+
+
+def paged_sdpa_decode_workspace(cache: PagedKV, rows, q_heads, dtype) -> int:
+    n = C.c_size_t()
+    check(lib().lthn_paged_sdpa_decode_workspace(cache.desc, rows, q_heads, dtype, C.byref(n)))
+    return int(n.value)
+
+
+def paged_sdpa_decode(cache: PagedKV, q, dtype, kv_lens, rows, q_heads, out, workspace, *, options: AttnOptions = None, lse=None, q_stride=0,
+                      out_stride=0, stream=None):
+    """Attention of one new token per sequence; workspace: paged_sdpa_decode_workspace() bytes of device memory."""
+    check(lib().lthn_paged_sdpa_decode(_raw(stream), cache.desc, options, _p(q), dtype, q_stride, _p(kv_lens), rows, q_heads, _p(out),
+                                       out_stride, _p(lse), _p(workspace), workspace.nbytes))
+
+
+def paged_prefill_attention_workspace(cache: PagedKV, seqs, total_q, q_heads, max_ctx=0) -> int:
+    n = C.c_size_t()
+    check(lib().lthn_paged_prefill_attention_workspace(cache.desc, seqs, total_q, q_heads, max_ctx, C.byref(n)))
+    return int(n.value)
+
+
+def paged_prefill_attention(cache: PagedKV, q, q_start, kv_lens, seqs, total_q, q_heads, out, workspace, *, max_ctx=0,
+                            options: AttnOptions = None, lse=None, q_stride=0, out_stride=0, stream=None):
+    """Attention of packed prompt chunks; workspace: paged_prefill_attention_workspace() bytes of device memory."""
+    check(lib().lthn_paged_prefill_attention(_raw(stream), cache.desc, options, _p(q), q_stride, _p(q_start), _p(kv_lens), seqs, total_q,
+                                             q_heads, max_ctx, _p(out), out_stride, _p(lse), _p(workspace), workspace.nbytes))
 
 
 # ------------------------------------------------------------------ engine ----

@@ -63,6 +63,7 @@ int32_t lthn_cuda_mem_info(uint64_t* free_bytes, uint64_t* total_bytes); /* engi
  * entry points (lthn_affine_qmv, _geglu, _normed, _noalloc, lthn_affine_qmm, lthn_sdpa_decode)
  * call this to learn of it: synchronises `stream`, reads and clears the status words of the
  * current device into *bits (may be NULL) and returns LTHN_ERR_DEVICE_WAIT when any bit was set.
+ * LTHN_STATUS_PAGED alone (a paged-cache call met an index outside its table) returns LTHN_ERR_INVALID.
  * Copies four bytes per word to the host; allocates nothing. No counterpart in the reference
  * (its HIP shim reports launch failures through hipGetLastError, engine/hip/hip_driver_cgo.go). */
 int32_t lthn_device_status(void* stream, uint32_t* bits);
@@ -271,6 +272,119 @@ int32_t lthn_sdpa_decode(void* stream, const float* q, const uint16_t* kcache, c
  * (hip_transformer_reference.go:295-330). head_dim in {64,128,256}; scale<=0 means 1/sqrt(head_dim). */
 int32_t lthn_prefill_attention(void* stream, const float* q, const uint16_t* kcache, const uint16_t* vcache, uint16_t* out,
                                int32_t rows, int32_t pos0, int32_t q_heads, int32_t kv_heads, int32_t head_dim, float scale);
+/* ---- paged KV cache ------------------------------------------------------------------
+ * For servers whose conversations differ in length: the cache is a pool of pages of page_size token
+ * rows, and a page table names the pages of each sequence, so that a sequence holds the pages it has
+ * filled and no lane of max_len rows. Three operators work on it: append (per-head norm and rotation
+ * on the way), attention of one new token per sequence, attention of prompt chunks. They need no
+ * engine object; the reference keeps its paged forms inside its engines (engine/metal/kernels/
+ * attention/lthn_sdpa_paged*.metal) and has no public counterpart.
+ *
+ * The struct and the option structs are read by the host during the call; the pointers in them are
+ * device pointers of the current device. Row of position p of sequence s, kv head h:
+ *   page = page_table[s*table_stride + p / page_size],
+ *   first element at k + page*page_stride + (p % page_size)*row_stride + h*head_stride (v alike).
+ * So both [page][row][head][dim] (strides left 0) and [page][head][row][dim] (row_stride = head_dim,
+ * head_stride = page_size*head_dim) pools are served, as are pools that hold K and V side by side.
+ * k and v are 16-byte aligned and the strides multiples of 8 elements. Offsets are 64 bits wide.
+ * No call reads a row at or behind a sequence's length, nor a page it does not need: what lies there
+ * (NaN, stale rows, table entries of any value) does not matter.
+ *
+ * Errors the host cannot see: a page table entry outside [0, pages), a position or length beyond the
+ * table's table_stride*page_size rows, a sequence number >= seqs or a decreasing q_start sets bit
+ * LTHN_STATUS_PAGED of the sticky device status (lthn_device_status returns LTHN_ERR_INVALID for
+ * it alone). Nothing out of bounds is touched: such rows are not stored, such keys count as zero
+ * vectors, lengths are cut at the table; the outputs of the call are then not valid. */
+#define LTHN_STATUS_PAGED 0x40000000u
+typedef struct {
+    uint16_t* k;                /* bf16 */
+    uint16_t* v;
+    const int32_t* page_table;  /* [seqs][table_stride] */
+    int64_t page_stride;        /* elements between pages; 0 -> page_size * kv_heads * head_dim */
+    int64_t row_stride;         /* elements between token rows of a page; 0 -> kv_heads * head_dim */
+    int64_t head_stride;        /* elements between kv heads of a row; 0 -> head_dim */
+    int32_t pages;              /* pages of the pool */
+    int32_t page_size;          /* token rows per page, >= 1 */
+    int32_t table_stride;       /* page table entries per sequence */
+    int32_t seqs;               /* sequences of the page table */
+    int32_t kv_heads, head_dim; /* head_dim 64, 128 or 256 */
+} lthn_paged_kv;
+
+/* lthn_paged_kv_append: row r holds the projections of position row_pos[r] of sequence row_seq[r].
+ * Its k and v heads go to the cache as bf16; its q heads, when q is given, to q_out. q and k heads pass
+ * through, as the struct says (NULL: nothing),
+ *   the norm x / sqrt(mean(x^2) + eps) * w (q_norm / k_norm [head_dim] f32, each optional), then
+ *   the rotation of the first rotary_dim/2 pairs by pos * inv_freq[i] (f64 [rotary_dim/2]: with
+ *   base^(-2i/head_dim) the frequencies of lthn_rmsnorm_rope; scaled frequencies serve long contexts):
+ *   pairs (i, i + head_dim/2), or neighbours (2i, 2i+1) with interleaved = 1.
+ * Angles are formed in f64, everything else in f32, each result is rounded once. row_seq[r] < 0 marks a padding row: nothing of
+ * it is read or written. Rows must name different positions: which of two equal ones stays is not defined.
+ * dtype (LTHN_DTYPE_*) is the type of q, k and v, q_dtype that of q_out; strides are elements between
+ * rows (0 -> dense), multiples of 8, so that the three may be slices of one projection's output; all pointers
+ * 16-byte aligned. q_out may be q itself (same type and stride). rows == 0 is a successful no-op.
+ * Stands beside lthn_rmsnorm_rope and the append of the decode step (engine/metal/kernels/norms/
+ * lthn_qknorm_rope_bf16.metal, engine/hip/kernels/norms/rms_norm.hipinc:306-377). */
+typedef struct {
+    const double* inv_freq;     /* NULL: no rotation */
+    int32_t rotary_dim;         /* even, <= head_dim */
+    int32_t interleaved;
+    const float* q_norm;
+    const float* k_norm;
+    float eps;
+} lthn_rope_params;
+int32_t lthn_paged_kv_append(void* stream, const lthn_paged_kv* cache, const lthn_rope_params* rope, const void* q, const void* k,
+                             const void* v, int32_t dtype, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                             const int32_t* row_seq, const int32_t* row_pos, int32_t rows, int32_t q_heads, void* q_out,
+                             int32_t q_dtype, int64_t q_out_stride);
+
+/* What both attention calls do with the scores (NULL: softmax(q k^T / sqrt(head_dim)), causal). For the
+ * query at position i and the key at position j < the sequence's length:
+ *   s = softcap * tanh(q.k * scale / softcap)           (softcap 0: s = q.k * scale; the cap of
+ *                                                        engine/hip/hip_gemma4_q4_layer.go:3166-3177)
+ *   s = s - slopes[q head] * |i - j|                    (slopes given: a bias that grows with distance)
+ *   visible when j < prefix_lens[sequence], or j <= i and (window == 0 or j > i - window).
+ * prefix_lens gives a prefix that every query sees (a bidirectional prompt, or the first tokens kept in front
+ * of a sliding window). A query that sees nothing gets zeros and an lse of -infinity. lse (optional) is
+ * ln sum exp s per query and head, which joins results over different parts of a context. */
+typedef struct {
+    float scale;                 /* <= 0 -> 1/sqrt(head_dim) */
+    float softcap;               /* 0: none */
+    const float* slopes;         /* [q_heads], >= 0; NULL: none */
+    int32_t window;              /* 0: none */
+    const int32_t* prefix_lens;  /* [sequences of the call]; NULL: none */
+} lthn_attn_options;
+
+/* lthn_paged_sdpa_decode: one new token per sequence. Row r of q [rows, q_heads*head_dim] is the query at
+ * position kv_lens[r]-1 of sequence r of the page table and attends to its kv_lens[r] rows (its own
+ * included: append first); kv_lens[r] <= 0 is an empty row. q_heads is a multiple of kv_heads, head
+ * map as lthn_sdpa_decode. dtype is the type of q and out: f32 computes at f32 grade (the keys and values
+ * are exact in bf16 and the products of q and of the weights with them are not rounded), bf16 rounds the weights and the result.
+ * Lengths are read on the device, so a captured call replays with new ones. All work of the call is one list of
+ * 64-key pieces of all rows, dealt out evenly over the GPU: no bound on the lengths is needed and a long
+ * row does not wait for its own block. workspace: device memory of
+ * lthn_paged_sdpa_decode_workspace bytes, 16-byte aligned, uninitialised; nothing is kept in it between
+ * calls, but calls that can overlap (two streams, two captured graphs) need one each. Strides are
+ * elements between rows (0 -> dense), multiples of 8; q and out 16-byte aligned. */
+int32_t lthn_paged_sdpa_decode_workspace(const lthn_paged_kv* cache, int32_t rows, int32_t q_heads, int32_t dtype, size_t* bytes);
+int32_t lthn_paged_sdpa_decode(void* stream, const lthn_paged_kv* cache, const lthn_attn_options* options, const void* q, int32_t dtype,
+                               int64_t q_stride, const int32_t* kv_lens, int32_t rows, int32_t q_heads, void* out, int64_t out_stride,
+                               float* lse, void* workspace, size_t workspace_bytes);
+
+/* lthn_paged_prefill_attention: the rows of q (bf16 [total_q, q_heads*head_dim]) are the newest tokens of
+ * `seqs` sequences, packed behind one another: rows q_start[s] .. q_start[s+1]-1 (q_start [seqs+1], never
+ * decreasing, device memory) are the last of the kv_lens[s] positions of sequence s, which are all in the cache. Tokens of
+ * different sequences do not see each other. Rows that q_start leaves out are not touched, neither is their
+ * lse; a sequence with more query rows than positions has empty rows in front. Scores and sums are f32, the weights
+ * are rounded to bf16 for the second product, as in lthn_prefill_attention. max_ctx (0: the table's rows)
+ * bounds kv_lens for the choice of how the work is cut; longer sequences are still computed right. A NaN or
+ * infinity in a value row that some query of a tile sees may reach the other queries of that tile (256 rows of
+ * tokens times query heads of a kv head). Workspace and strides as above. */
+int32_t lthn_paged_prefill_attention_workspace(const lthn_paged_kv* cache, int32_t seqs, int32_t total_q, int32_t q_heads, int32_t max_ctx,
+                                               size_t* bytes);
+int32_t lthn_paged_prefill_attention(void* stream, const lthn_paged_kv* cache, const lthn_attn_options* options, const uint16_t* q,
+                                     int64_t q_stride, const int32_t* q_start, const int32_t* kv_lens, int32_t seqs, int32_t total_q,
+                                     int32_t q_heads, int32_t max_ctx, uint16_t* out, int64_t out_stride, float* lse, void* workspace,
+                                     size_t workspace_bytes);
 /* Greedy pick per row: strict '>', lowest index wins ties (model.Greedy, model/sample.go:
  * 29-50; hipReferenceGreedySample). logits [rows, vocab] f32. */
 int32_t lthn_argmax(void* stream, const float* logits, int32_t rows, int32_t vocab, int32_t* out_idx);
