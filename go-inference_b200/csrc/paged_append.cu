@@ -68,7 +68,7 @@ int32_t paged_check_options(const char* name, const lthn_attn_options* o, int he
         LTHN_REQUIRE(o->softcap >= 0.f && o->softcap < INFINITY, named(name, "softcap must be finite and not negative"));
         LTHN_REQUIRE(o->scale == o->scale && o->scale < INFINITY, named(name, "scale must be finite"));
         LTHN_REQUIRE(o->window >= 0, named(name, "window must not be negative"));
-        a.scale = o->scale; a.softcap = o->softcap; a.slopes = o->slopes; a.window = o->window; a.prefix = o->prefix_lens;
+        a.scale = o->scale; a.softcap = o->softcap; a.slopes = o->slopes; a.window = std::min(o->window, 1 << 30); a.prefix = o->prefix_lens;
     }
     if (a.scale <= 0.f) a.scale = 1.0f / sqrtf((float)head_dim);
     *out = a;

@@ -1,10 +1,35 @@
-// paged_prefill.cu — attention of packed prompt chunks over the paged KV cache.
+// paged_prefill.cu — attention of packed prompt chunks over the paged KV cache on the Blackwell tensor cores.
 //
 //   out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),   s_j = cap(q.k_j scale) - slope |i - j|,   m = max_j s_j
 //
-// The query rows of a tile are the (token, query head) pairs of one kv head, token by token, so the heads that share
-// K and V share their loads, and a chunk of a few tokens still fills a tile. One CTA = 64 rows, four warps of 16; K and V
-// tiles by cp.async, double buffered; both products on mma.sync with a running softmax.
+// 4*D flops per visible (query, key) pair against 4*D bytes of K and V per key and tile of query rows: bound by the tensor pipe
+// for prompts, by HBM for a few rows against a long context.
+//
+// Rows. The query rows of a tile are the (token, query head) pairs of one kv head, token by token, so the heads that share
+// K and V share their loads and a chunk of a few tokens still fills a tile. A CTA works on one or two tiles of 128 rows
+// (two: two accumulators of head_dim columns fit the tensor memory beside two score tiles for head_dim 64 and 128) and on
+// BN keys at a time.
+//
+//   softmax warps   one warpgroup per row tile, one thread per row: tcgen05.ld the row's BN scores, mask, maximum, ex2, sum - all
+//                   within the thread - and tcgen05.st the weights as bf16 over the scores they came from.
+//   issuer          one lane: S = Q K^T (both operands in shared memory), O += P V (P in tensor memory, V in shared
+//                   memory as an N-major operand, so it is stored as it comes). There are two score buffers. Unit u uses
+//                   buffer u & 1 and the issue order is S(0) S(1) | O(0) S(2) | O(1) S(3) | ..., so that the tensor pipe
+//                   works on one buffer while the other's softmax runs. With two row tiles the buffers belong to them,
+//                   with one they alternate over its key tiles.
+//   loaders         three warps, cp.async of 16 bytes into a ring of K and V tiles in the 128-byte swizzle. Page size and strides
+//                   are arbitrary, rows that nobody sees are zeros (they may hold NaN, which a weight of zero would not
+//                   silence), so rows are fetched one by one; the offsets of a tile are formed once by the lanes.
+//
+// The running maximum is only moved when a row's grew by more than 2^8: until then weights are up to 2^8, which neither
+// their bf16 rounding (relative) nor the f32 sums mind, and O in tensor memory needs no correction. A move multiplies
+// O by 2^(old - new) through registers; after the first tiles it is rare.
+//
+// Cutting. Where there are fewer tiles than SMs the keys of a tile are cut into chunks, one CTA each, that leave
+// (maximum, sum, unnormalised output) in the workspace for a second kernel to join.
+//
+// Every wait is bounded: on a time-out the roles record it in the device status word, drain what they have in flight, free
+// the tensor memory and return.
 #include "paged.cuh"
 
 #include <algorithm>
@@ -20,10 +45,17 @@ struct PrefillArgs {
     int64_t q_stride, out_stride;
     const int32_t *q_start, *lens;
     float* lse;
+    uint32_t* wait_status;
     int seqs, total_q, Hq, G;
+    int tiles;           // upper bound of the row tiles of all sequences
+    int chunks;          // CTAs per tile and kv head
+    int chunk_tiles;     // key tiles per chunk
+    float* part;         // [tiles*kv_heads*chunks][rows][D] unnormalised outputs
+    float2* ml;          // [tiles*kv_heads*chunks][rows] maximum (log2 units) and sum
+    int4* desc;          // [tiles] sequence, tile of the sequence, chunks in use
 };
 
-// The rows of sequence s, made safe: within [0, total_q), never overlapping the next one's.
+// The rows of sequence s, made safe: within [0, total_q).
 __device__ __forceinline__ int2 prefill_span(const PrefillArgs& a, int s) {
     const int b = a.q_start[s], e = a.q_start[s + 1];
     if (b < 0 || e < b || e > a.total_q) {
@@ -33,178 +65,571 @@ __device__ __forceinline__ int2 prefill_span(const PrefillArgs& a, int s) {
     return make_int2(b, e - b);
 }
 
-// Tile blockIdx.x counts through the tiles (of ROWS rows of token * G + head) of all sequences. Returns false past the last.
+// Tile `id` of the tiles (ROWS rows of token * G + head) of all sequences, counted from the last one: the later tiles of a prompt
+// see more keys, and the longest work goes first. Returns false past the first.
 template <int WARPS, int ROWS>
-__device__ __forceinline__ bool prefill_tile(const PrefillArgs& a, int* sh, int& seq, int& tile) {
-    int base = 0;
-    for (int s0 = 0; s0 < a.seqs; s0 += WARPS * 32) {
+__device__ __forceinline__ bool prefill_tile(const PrefillArgs& a, int* sh, int id, int& seq, int& tile) {
+    int all = 0, incl;
+    auto count = [&](int s0) {
         const int s = s0 + threadIdx.x;
-        const int n = s < a.seqs ? (prefill_span(a, s).y * a.G + ROWS - 1) / ROWS : 0;
-        int incl;
-        const int total = paged_block_scan<WARPS>(n, incl, sh);
-        const int want = (int)blockIdx.x - base;
+        return s < a.seqs ? (prefill_span(a, s).y * a.G + ROWS - 1) / ROWS : 0;
+    };
+    for (int s0 = 0; s0 < a.seqs; s0 += WARPS * 32) all += paged_block_scan<WARPS>(count(s0), incl, sh);
+    if (id >= all) return false;
+    int want = all - 1 - id;
+    for (int s0 = 0; s0 < a.seqs; s0 += WARPS * 32) {
+        const int n = count(s0), total = paged_block_scan<WARPS>(n, incl, sh);
         if (want < total) {
-            if (incl > want && incl - n <= want) { sh[WARPS] = s; sh[WARPS + 1] = want - (incl - n); }
+            if (incl > want && incl - n <= want) { sh[WARPS] = s0 + threadIdx.x; sh[WARPS + 1] = want - (incl - n); }
             __syncthreads();
             seq = sh[WARPS];
             tile = sh[WARPS + 1];
             return true;
         }
-        base += total;
+        want -= total;
     }
     return false;
 }
 
-constexpr int PP_BM = 64;
-constexpr int PP_WARPS = 4;
-constexpr int PP_THREADS = PP_WARPS * 32;
+// ---- tcgen05 wrappers (cta_group::1) ---------------------------------------------------------------
+__device__ __forceinline__ void pf_tmem_alloc(uint32_t* smem_dst, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_dst)), "r"(ncols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void pf_tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void pf_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pf_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pf_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void pf_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void pf_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void pf_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void pf_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void pf_ld32(uint32_t taddr, float* f) {
+    uint32_t* r = (uint32_t*)f;
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void pf_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pf_st32(uint32_t taddr, const float* f) {
+    const uint32_t* r = (const uint32_t*)f;
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+          "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+          "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+__device__ __forceinline__ void pf_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void pf_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-template <int D>
-struct PpCfg {
-    static constexpr int BN = D >= 256 ? 32 : 64;
-    static constexpr int PITCH = D * 2 + 16;
-    static constexpr size_t SMEM = (size_t)(PP_BM + 4 * BN) * PITCH;
-};
-
-template <int D>
-__global__ void __launch_bounds__(PP_THREADS) paged_prefill_kernel(const PrefillArgs a) {
-    using C = PpCfg<D>;
-    constexpr int BN = C::BN, PITCH = C::PITCH, NS = BN / 8, ND = D / 8, CPR = D / 8;
-    constexpr float LOG2E = 1.4426950408889634f;
-    extern __shared__ __align__(16) unsigned char pp_smem[];
-    __shared__ int sh[PP_WARPS + 2];
-    int seq, tile;
-    if (!prefill_tile<PP_WARPS, PP_BM>(a, sh, seq, tile)) return;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, mi = lane >> 3;
-    const int kvh = blockIdx.y;
-    const int2 span = prefill_span(a, seq);
-    const int len = paged_length(a.c, a.lens[seq]);
-    const int nrows = span.y * a.G, row0 = tile * PP_BM;
-    const int pos0 = len - span.y;                                   // position of the sequence's first query
-    const int prefix = a.o.prefix ? min(max(a.o.prefix[seq], 0), len) : 0;
-    const int qlo = pos0 + row0 / a.G, qhi = pos0 + (min(row0 + PP_BM, nrows) - 1) / a.G;
-    const KeyTiles kt = key_tiles<BN>(qlo, qhi, len, prefix, a.o.window);
-    const int lo = a.o.window > 0 ? max(0, qlo - a.o.window + 1) : 0;
-    const uint16_t* kbase = a.c.k + kvh * a.c.head_stride;
-    const uint16_t* vbase = a.c.v + kvh * a.c.head_stride;
-    const int32_t* trow = a.c.table + (int64_t)seq * a.c.table_stride;
-    const uint32_t qs = smem_u32(pp_smem), ks = qs + PP_BM * PITCH, vs = ks + 2 * BN * PITCH;
-
-    auto load_kv = [&](int i) {
-        const int k0 = kt.tile(i) * BN, buf = i & 1;
-        for (int x = tid; x < BN * CPR; x += PP_THREADS) {
-            const int r = x / CPR, c = x - r * CPR, key = k0 + r;
-            int64_t off = -1;
-            if (key < len && (key < prefix || key >= lo)) off = paged_offset(a.c, trow[key / a.c.page_size], key % a.c.page_size);
-            const int64_t e = (off < 0 ? 0 : off) + c * 8;
-            const int n = off < 0 ? 0 : 16;
-            cp_async16_zfill(ks + (buf * BN + r) * PITCH + c * 16, kbase + e, n);
-            cp_async16_zfill(vs + (buf * BN + r) * PITCH + c * 16, vbase + e, n);
+// Bounded wait on an mbarrier phase: try_wait parks the thread for a while each time; after 0.2 s of wall time it gives up.
+__device__ __forceinline__ bool pf_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t done = 0;
+    uint64_t t0 = 0;
+    for (uint32_t it = 0;; ++it) {
+        asm volatile("{\n\t.reg .pred p;\n\t"
+                     "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                     "selp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+        if (done) return true;
+        if ((it & 63) == 63) {
+            uint64_t now;
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+            if (t0 == 0) t0 = now;
+            else if (now - t0 > 200000000ull) return false;
         }
-        paged_cp_commit();
-    };
-    for (int x = tid; x < PP_BM * CPR; x += PP_THREADS) {
-        const int r = x / CPR, c = x - r * CPR, row = row0 + r;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row < nrows) v = *(const uint4*)(a.q + (span.x + row / a.G) * a.q_stride + (int64_t)(kvh * a.G + row % a.G) * D + c * 8);
-        *(uint4*)(pp_smem + r * PITCH + c * 16) = v;
-    }
-    if (kt.n > 0) load_kv(0);
-    float o[ND][4];
-#pragma unroll
-    for (int n = 0; n < ND; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-    float mrow[2] = {-INFINITY, -INFINITY}, lrow[2] = {0.f, 0.f}, slope[2] = {0.f, 0.f};
-    int qpos[2];
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const int row = row0 + warp * 16 + g + 8 * h;
-        qpos[h] = pos0 + row / a.G;
-        if (a.o.slopes && row < nrows) slope[h] = a.o.slopes[kvh * a.G + row % a.G];
-    }
-    for (int i = 0; i < kt.n; i++) {
-        const int buf = i & 1, k0 = kt.tile(i) * BN;
-        paged_cp_wait<0>();
-        __syncthreads();
-        if (i + 1 < kt.n) load_kv(i + 1);
-        float s[NS][4];
-#pragma unroll
-        for (int n = 0; n < NS; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; kk++) {
-            uint32_t qa[4];
-            ldmatrix_x4(qa, qs + (warp * 16 + (lane & 15)) * PITCH + kk * 32 + (lane >> 4) * 16);
-#pragma unroll
-            for (int n2 = 0; n2 < BN / 16; n2++) {
-                uint32_t kb[4];
-                ldmatrix_x4(kb, ks + (buf * BN + n2 * 16 + (mi >> 1) * 8 + (lane & 7)) * PITCH + kk * 32 + (mi & 1) * 16);
-                mma_bf16_16816(s[2 * n2], qa[0], qa[1], qa[2], qa[3], kb[0], kb[1]);
-                mma_bf16_16816(s[2 * n2 + 1], qa[0], qa[1], qa[2], qa[3], kb[2], kb[3]);
-            }
-        }
-        float mx[2] = {mrow[0], mrow[1]};
-#pragma unroll
-        for (int n = 0; n < NS; n++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int key = k0 + n * 8 + 2 * t + (e & 1), gap = qpos[e >> 1] - key;
-                float v = s[n][e] * a.o.scale;
-                if (a.o.softcap > 0.f) v = a.o.softcap * tanhf(v / a.o.softcap);
-                if (a.o.slopes) v -= slope[e >> 1] * (float)abs(gap);
-                const bool seen = key < len && (key < prefix || (gap >= 0 && (a.o.window == 0 || gap < a.o.window)));
-                s[n][e] = seen ? v * LOG2E : -INFINITY;
-                mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
-            }
-        float alpha[2];
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-            const float ref = mx[h] == -INFINITY ? 0.f : mx[h];
-            alpha[h] = ex2(mrow[h] - ref);
-            mrow[h] = mx[h];
-            mx[h] = ref;
-            lrow[h] *= alpha[h];
-        }
-        uint32_t p[NS][2];
-#pragma unroll
-        for (int n = 0; n < NS; n++) {
-            const float p0 = ex2(s[n][0] - mx[0]), p1 = ex2(s[n][1] - mx[0]), p2 = ex2(s[n][2] - mx[1]), p3 = ex2(s[n][3] - mx[1]);
-            lrow[0] += p0 + p1;
-            lrow[1] += p2 + p3;
-            p[n][0] = pack_bf16x2(p0, p1);
-            p[n][1] = pack_bf16x2(p2, p3);
-        }
-#pragma unroll
-        for (int n = 0; n < ND; n++) { o[n][0] *= alpha[0]; o[n][1] *= alpha[0]; o[n][2] *= alpha[1]; o[n][3] *= alpha[1]; }
-#pragma unroll
-        for (int k16 = 0; k16 < BN / 16; k16++)
-#pragma unroll
-            for (int d2 = 0; d2 < D / 16; d2++) {
-                uint32_t vb[4];
-                ldmatrix_x4_trans(vb, vs + (buf * BN + k16 * 16 + (mi & 1) * 8 + (lane & 7)) * PITCH + d2 * 32 + (mi >> 1) * 16);
-                mma_bf16_16816(o[2 * d2], p[2 * k16][0], p[2 * k16][1], p[2 * k16 + 1][0], p[2 * k16 + 1][1], vb[0], vb[1]);
-                mma_bf16_16816(o[2 * d2 + 1], p[2 * k16][0], p[2 * k16][1], p[2 * k16 + 1][0], p[2 * k16 + 1][1], vb[2], vb[3]);
-            }
-    }
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        float l = lrow[h];
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        const int row = row0 + warp * 16 + g + 8 * h;
-        if (row >= nrows) continue;
-        const float inv = l > 0.f ? 1.0f / l : 0.f;
-        const int64_t token = span.x + row / a.G;
-        const int head = kvh * a.G + row % a.G;
-        uint16_t* dst = a.out + token * a.out_stride + (int64_t)head * D + 2 * t;
-#pragma unroll
-        for (int n = 0; n < ND; n++) *(uint32_t*)(dst + n * 8) = pack_bf16x2(o[n][2 * h] * inv, o[n][2 * h + 1] * inv);
-        if (a.lse && t == 0) a.lse[token * a.Hq + head] = (mrow[h] + log2f(l)) * 0.6931471805599453f;
     }
 }
 
+// Shared-memory operands in the 128-byte swizzle: slabs of 64 elements, rows 128 bytes apart, 8-row groups 1024.
+// K-major (Q and K): a K = 16 step is 32 bytes further in the slab.
+__device__ __forceinline__ uint64_t pf_desc_k(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// N-major (V: rows are keys = the MMA's K, 64 head dimensions each): 8-key groups 1024 bytes apart (stride offset), the next 64
+// head dimensions one slab further (leading offset); a K = 16 step is 16 rows = 2048 bytes.
+__device__ __forceinline__ uint64_t pf_desc_n(uint32_t addr, uint32_t slab) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(slab >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+           ((uint64_t)2 << 61);
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// the n lowest bits of a word, n of any size and sign
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 template <int D>
+struct PfCfg {
+    static constexpr int NQ = D == 256 ? 1 : 2;              // row tiles per CTA
+    static constexpr int BN = D == 256 ? 64 : 128;           // keys per tile
+    static constexpr int ROWS = NQ * 128;
+    static constexpr int SM_WARPS = NQ * 4;                  // softmax warps
+    static constexpr int WARPS = SM_WARPS + 4;               // + issuer + three loaders
+    static constexpr int THREADS = WARPS * 32;
+    static constexpr int Q_BYTES = 128 * D * 2;              // one row tile
+    static constexpr int KV_BYTES = BN * D * 2;
+    static constexpr int SLAB = BN * 128;                    // bytes of 64 head dimensions of a K or V tile
+    static constexpr int ST = D == 64 ? 8 : 5;
+    static constexpr int RING = NQ * Q_BYTES;                // offsets in shared memory
+    static constexpr int OFFS = RING + ST * KV_BYTES;        // [2][BN] row offsets
+    static constexpr int BARS = OFFS + 2 * BN * 8;
+    static constexpr int TOTAL = BARS + 512;
+    static constexpr int S_COLS = BN;                        // tensor memory: two score buffers, then the outputs at column 256
+    static constexpr int LAG = 2;                            // ring slots in flight behind the one being filled
+    static_assert(LAG <= ST - 3, "a slot is handed over before the one that frees its successor is waited for");
+    static_assert(TOTAL <= 232448, "shared memory of a CTA");
+};
+
+// FEAT bit 0: tanh cap, bit 1: distance bias
+template <int D, int FEAT>
+__global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(const PrefillArgs a) {
+    using C = PfCfg<D>;
+    constexpr int BN = C::BN, ST = C::ST, ROWS = C::ROWS;
+    constexpr float LOG2E = 1.4426950408889634f;
+    extern __shared__ __align__(1024) unsigned char pf_smem[];
+    uint64_t* full = (uint64_t*)(pf_smem + C::BARS);         // [ST] loaders -> issuer
+    uint64_t* empty = full + ST;                             // [ST] issuer's commit -> loaders
+    uint64_t* s_full = empty + ST;                           // [2] scores are there
+    uint64_t* p_full = s_full + 2;                           // [2] weights are there, O is corrected
+    uint64_t* o_done = p_full + 2;                           // [2] per row tile: O(u) has been added, all but the last
+    uint64_t* o_last = o_done + 2;                           // [2] the last has (a barrier of its own: with one row tile the softmax
+                                                             //     may be two units ahead, which a parity cannot tell from none)
+    uint64_t* q_full = o_last + 2;
+    uint64_t* drain = q_full + 1;
+    uint32_t* tmem_slot = (uint32_t*)(drain + 1);
+    int* scan = (int*)(tmem_slot + 2);                       // WARPS + 2 words
+
+    pdl_trigger();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int kvh = blockIdx.x % a.c.kv_heads;
+    const int chunk = blockIdx.x / a.c.kv_heads % a.chunks;
+    const int id = blockIdx.x / a.c.kv_heads / a.chunks;
+    int seq, tile;
+    if (!prefill_tile<C::WARPS, ROWS>(a, scan, id, seq, tile)) {
+        if (a.chunks > 1 && chunk == 0 && kvh == 0 && tid == 0) a.desc[id] = make_int4(0, 0, 0, 0);
+        return;
+    }
+    const int2 span = prefill_span(a, seq);
+    const int len = paged_length(a.c, a.lens[seq]);
+    const int nrows = span.y * a.G, row0 = tile * ROWS;
+    const int pos0 = len - span.y;                           // position of the sequence's first query
+    const int prefix = a.o.prefix ? min(max(a.o.prefix[seq], 0), len) : 0;
+    const int qlo = pos0 + row0 / a.G, qhi = pos0 + (min(row0 + ROWS, nrows) - 1) / a.G;
+    const KeyTiles kt = key_tiles<BN>(qlo, qhi, len, prefix, a.o.window);
+    const int per = max(a.chunk_tiles, (kt.n + a.chunks - 1) / a.chunks);  // key tiles of a chunk, also where max_ctx was too small
+    const int used = a.chunks > 1 ? max(1, (kt.n + per - 1) / per) : 1;
+    if (a.chunks > 1 && chunk == 0 && kvh == 0 && tid == 0) a.desc[id] = make_int4(seq, tile, used, 0);
+    if (chunk >= used) return;
+    const int i0 = chunk * per;
+    const int n = a.chunks > 1 ? min(per, kt.n - i0) : kt.n;   // key tiles of this CTA (0 only where nothing is visible)
+    const bool two = C::NQ == 2 && nrows - row0 > 128;
+    const int units = two ? 2 * n : n;
+
+    if (tid == 0) {
+        for (int s = 0; s < ST; s++) { mbar_init(&full[s], 96); mbar_init(&empty[s], 1); }
+        for (int b = 0; b < 2; b++) { mbar_init(&s_full[b], 1); mbar_init(&p_full[b], 128); mbar_init(&o_done[b], 1); mbar_init(&o_last[b], 1); }
+        mbar_init(q_full, C::SM_WARPS * 32);
+        mbar_init(drain, 1);
+        mbar_fence_init();
+    }
+    if (warp == C::SM_WARPS) pf_tmem_alloc(tmem_slot, 512);
+    pf_fence_before();
+    __syncthreads();
+    pf_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t smem = smem_u32(pf_smem);
+    bool ok = true;
+
+    // ring slots of the K and V tile of key tile j, in the order of their last use
+    auto k_slot = [&](int j) { return two ? 2 * j : j < 2 ? j : 2 * j - 1; };
+    auto v_slot = [&](int j) { return two ? 2 * j + 1 : j == n - 1 ? 2 * n - 1 : 2 * j + 2; };
+
+    if (warp < C::SM_WARPS) {
+        // ================================ softmax ================================
+        if (C::NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int qt = C::NQ == 2 ? warp >> 2 : 0;
+        const int r = (warp & 3) * 32 + lane;                // row within the row tile = tensor memory lane
+        {   // queries into shared memory: a warp takes 32 rows, D/8 lanes a row
+            constexpr int CPR = D / 8;
+            unsigned char* qs = pf_smem + qt * C::Q_BYTES;
+#pragma unroll 4
+            for (int x = lane; x < 32 * CPR; x += 32) {
+                const int rr = (warp & 3) * 32 + x / CPR, c = x % CPR, row = row0 + qt * 128 + rr;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (row < nrows) v = *(const uint4*)(a.q + (span.x + row / a.G) * a.q_stride + (int64_t)(kvh * a.G + row % a.G) * D + c * 8);
+                *(uint4*)(qs + (c >> 3) * (128 * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
+            }
+            pf_fence_async();
+            pf_arrive(q_full);
+            __syncwarp();
+        }
+        if (qt == 0 || two) {
+            const int row = row0 + qt * 128 + r;
+            const bool live = row < nrows;
+            const int token = row / a.G, head = kvh * a.G + row - token * a.G;
+            const int qpos = pos0 + token;
+            // visible: key < pre, or klo <= key < khi
+            const int pre = prefix, khi = min(qpos + 1, len), klo = a.o.window > 0 ? qpos - a.o.window + 1 : 0;
+            // plain scores stay as the product left them, the others are brought to log2 units first
+            const float c1 = FEAT ? 1.0f : a.o.scale * LOG2E;
+            const float cap2 = a.o.softcap * LOG2E, cin = FEAT & 1 ? 2.0f * LOG2E * a.o.scale / a.o.softcap : a.o.scale * LOG2E;
+            const float slope = (FEAT & 2) && live ? a.o.slopes[head] * LOG2E : 0.f;
+            const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+            const uint32_t o_addr = lanes + 256 + qt * D;
+            float m = -INFINITY, l = 0.f;                    // reference maximum (units of the scores), sum
+
+            for (int j = 0; j < n; j++) {
+                const int u = two ? 2 * j + qt : j, buf = u & 1;
+                ok = __all_sync(0xffffffffu, pf_wait(&s_full[buf], (u >> 1) & 1));
+                if (!ok) break;
+                pf_fence_after();
+                const uint32_t s_addr = lanes + buf * C::S_COLS;
+                float s[BN];
+#pragma unroll
+                for (int x = 0; x < BN; x += 32) pf_ld32(s_addr + x, s + x);
+                pf_ld_wait();
+                const int k0 = kt.tile(i0 + j) * BN;
+                if (FEAT & 1) {
+                    // cap tanh(x scale / cap) = cap (1 - 2 / (1 + e^(2 x scale / cap)))
+#pragma unroll
+                    for (int x = 0; x < BN; x++) s[x] = fmaf(-2.0f * cap2, rcp_approx(1.0f + ex2(s[x] * cin)), cap2);
+                }
+                if (FEAT & 2) {
+                    const float gap = (float)(qpos - k0);
+#pragma unroll
+                    for (int x = 0; x < BN; x++) s[x] = fmaf(-slope, fabsf(gap - (float)x), FEAT & 1 ? s[x] : s[x] * cin);
+                }
+                const bool all = !live || k0 + BN <= pre || (k0 >= klo && k0 + BN <= khi);
+                if (!__all_sync(0xffffffffu, all)) {
+                    const int p = pre - k0, lo = klo - k0, hi = khi - k0;
+#pragma unroll
+                    for (int x0 = 0; x0 < BN; x0 += 32) {
+                        const uint32_t seen = low_bits(p - x0) | (low_bits(hi - x0) & ~low_bits(lo - x0));
+#pragma unroll
+                        for (int x = 0; x < 32; x++) s[x0 + x] = seen >> x & 1 ? s[x0 + x] : -INFINITY;
+                    }
+                }
+                float mx = max3(s[0], s[1], s[2]);
+#pragma unroll
+                for (int x = 3; x + 1 < BN; x += 2) mx = max3(mx, s[x], s[x + 1]);
+                mx = fmaxf(mx, s[BN - 1]);
+                const float mnew = fmaxf(m, mx);
+                if (__any_sync(0xffffffffu, (mnew - m) * c1 > 8.0f)) {
+                    const float alpha = m == -INFINITY ? 0.f : ex2((m - mnew) * c1);
+                    m = mnew;
+                    l *= alpha;
+                    if (j > 0) {
+                        ok = __all_sync(0xffffffffu, pf_wait(&o_done[qt], (j - 1) & 1));
+                        if (!ok) break;
+                        pf_fence_after();
+#pragma unroll
+                        for (int x = 0; x < D; x += 32) {
+                            float o[32];
+                            pf_ld32(o_addr + x, o);
+                            pf_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 32; e++) o[e] *= alpha;
+                            pf_st32(o_addr + x, o);
+                        }
+                    }
+                }
+                const float neg = m == -INFINITY ? 0.f : -m * c1;
+                float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+                for (int x = 0; x < BN; x += 32) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float p0 = ex2(fmaf(s[x + e], c1, neg)), p1 = ex2(fmaf(s[x + e + 1], c1, neg));
+                        l0 += p0;
+                        l1 += p1;
+                        w[e / 2] = pack_bf16x2(p0, p1);
+                    }
+                    pf_st16(s_addr + x / 2, w);
+                }
+                l += l0 + l1;
+                pf_st_wait();
+                pf_fence_before();
+                pf_arrive(&p_full[buf]);
+            }
+            if (ok && n > 0) ok = __all_sync(0xffffffffu, pf_wait(&o_last[qt], 0));
+            if (!ok && lane == 0) atomicOr(a.wait_status, 1u << 26);
+            if (ok) {
+                pf_fence_after();
+                const int64_t tok = span.x + token;
+                const float m2 = m * c1;                     // log2 units (c1 > 0)
+                if (used == 1) {
+                    const float inv = l > 0.f ? 1.0f / l : 0.f;
+                    uint16_t* dst = a.out + tok * a.out_stride + (int64_t)head * D;
+#pragma unroll 1
+                    for (int x = 0; x < D; x += 32) {
+                        float o[32];
+                        __syncwarp();                        // the stores below are not made by all lanes, the loads have to be
+                        if (n > 0) {
+                            pf_ld32(o_addr + x, o);
+                            pf_ld_wait();
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; e++) o[e] = 0.f;
+                        }
+                        if (live) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 8)
+                                *(uint4*)(dst + x + e) = make_uint4(pack_bf16x2(o[e] * inv, o[e + 1] * inv), pack_bf16x2(o[e + 2] * inv, o[e + 3] * inv),
+                                                                    pack_bf16x2(o[e + 4] * inv, o[e + 5] * inv), pack_bf16x2(o[e + 6] * inv, o[e + 7] * inv));
+                        }
+                    }
+                    if (live && a.lse) a.lse[tok * a.Hq + head] = (m2 + log2f(l)) * 0.6931471805599453f;
+                } else {
+                    const int64_t at = (((int64_t)id * a.c.kv_heads + kvh) * a.chunks + chunk) * ROWS + qt * 128 + r;
+#pragma unroll 1
+                    for (int x = 0; x < D; x += 32) {
+                        float o[32];
+                        __syncwarp();
+                        pf_ld32(o_addr + x, o);
+                        pf_ld_wait();
+                        if (live) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) *(float4*)(a.part + at * D + x + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        }
+                    }
+                    if (live) a.ml[at] = make_float2(m2, l);
+                }
+            }
+        }
+    } else if (warp == C::SM_WARPS) {
+        // ================================ issuer ================================
+        if (C::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (lane == 0 && n > 0) {
+            // f32 accumulators, bf16 operands, M = 128; S: N = BN, both K-major; O: N = D, B is N-major
+            const uint32_t base = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);
+            const uint32_t idesc_s = base | ((uint32_t)(BN >> 3) << 17), idesc_o = base | (1u << 16) | ((uint32_t)(D >> 3) << 17);
+            ok = pf_wait(q_full, 0);
+            auto scores = [&](int u) {
+                const int j = two ? u >> 1 : u, qt = two ? u & 1 : 0, slot = k_slot(j), st = slot % ST;
+                ok = pf_wait(&full[st], (slot / ST) & 1);
+                if (!ok) return;
+                pf_fence_after();
+                const uint32_t qa = smem + qt * C::Q_BYTES, kb = smem + C::RING + st * C::KV_BYTES, d = tmem + (u & 1) * C::S_COLS;
+#pragma unroll
+                for (int x = 0; x < D / 16; x++)
+                    pf_mma_ss(d, pf_desc_k(qa + (x >> 2) * (128 * 128) + (x & 3) * 32), pf_desc_k(kb + (x >> 2) * C::SLAB + (x & 3) * 32), idesc_s, x > 0);
+                pf_commit(&s_full[u & 1]);
+                if (!two || qt == 1) pf_commit(&empty[st]);
+            };
+            if (ok) scores(0);
+            if (ok && units > 1) scores(1);
+            for (int u = 0; u < units && ok; u++) {
+                const int j = two ? u >> 1 : u, qt = two ? u & 1 : 0, slot = v_slot(j), st = slot % ST;
+                ok = pf_wait(&full[st], (slot / ST) & 1) && pf_wait(&p_full[u & 1], (u >> 1) & 1);
+                if (!ok) break;
+                pf_fence_after();
+                const uint32_t vb = smem + C::RING + st * C::KV_BYTES, pa = tmem + (u & 1) * C::S_COLS, d = tmem + 256 + qt * D;
+#pragma unroll
+                for (int x = 0; x < BN / 16; x++) pf_mma_ts(d, pa + x * 8, pf_desc_n(vb + x * 2048, C::SLAB), idesc_o, j > 0 || x > 0);
+                if (!two || qt == 1) pf_commit(&empty[st]);
+                pf_commit(j == n - 1 ? &o_last[qt] : &o_done[qt]);   // the last commit of all is one that is waited for
+                if (u + 2 < units) scores(u + 2);
+            }
+            if (!ok) {
+                atomicOr(a.wait_status, 1u << 25);
+                pf_commit(drain);                            // nothing of this CTA may still run when its memory is given back
+                pf_wait(drain, 0);
+            }
+        }
+        __syncwarp();
+    } else {
+        // ================================ loaders ================================
+        if (C::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        const int lw = warp - C::SM_WARPS - 1;
+        constexpr int NX = (BN / 4 + 2) / 3 * 4;             // rows of a warp: every third group of four
+        constexpr int PER = (NX + 31) / 32;
+        int64_t* offs = (int64_t*)(pf_smem + C::OFFS);
+        const int32_t* trow = a.c.table + (int64_t)seq * a.c.table_stride;
+        const uint16_t* kbase = a.c.k + kvh * a.c.head_stride;
+        const uint16_t* vbase = a.c.v + kvh * a.c.head_stride;
+        const int lo = a.o.window > 0 ? max(0, qlo - a.o.window + 1) : 0;
+        auto row_of = [&](int x) { return (x >> 2) * 12 + lw * 4 + (x & 3); };
+        auto key_of = [&](int j, int x) {                    // -1: a row nobody sees
+            const int rr = row_of(x), key = kt.tile(i0 + j) * BN + rr;
+            return x < NX && rr < BN && key < len && (key < prefix || (key >= lo && key <= qhi)) ? key : -1;
+        };
+        int page[PER];
+        auto fetch_pages = [&](int j) {
+#pragma unroll
+            for (int e = 0; e < PER; e++) {
+                const int key = j < n ? key_of(j, lane + 32 * e) : -1;
+                page[e] = key >= 0 ? trow[key / a.c.page_size] : 0;
+            }
+        };
+        auto fill = [&](int slot, const uint16_t* src, const int64_t* off) {
+            const int st = slot % ST;
+            ok = __all_sync(0xffffffffu, pf_wait(&empty[st], ((slot / ST) & 1) ^ 1));
+            if (!ok) return;
+            const uint32_t dst = smem + C::RING + st * C::KV_BYTES;
+            constexpr int CPR = D / 8, RPI = 32 / CPR;       // 16-byte chunks per row, rows per instruction
+            const int c = lane % CPR;
+#pragma unroll 4
+            for (int x0 = 0; x0 < NX; x0 += RPI) {
+                const int rr = row_of(x0 + lane / CPR);
+                if ((x0 >> 2) * 12 + lw * 4 >= BN) break;
+                const int64_t o = off[rr];
+                cp_async16_zfill(dst + (c >> 3) * C::SLAB + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), src + (o < 0 ? 0 : o) + c * 8, o < 0 ? 0 : 16);
+            }
+            paged_cp_commit();
+            if (slot >= C::LAG) {
+                paged_cp_wait<C::LAG>();
+                pf_fence_async();
+                pf_arrive(&full[(slot - C::LAG) % ST]);
+            }
+        };
+        auto fill_k = [&](int j) {
+            int64_t* off = offs + (j & 1) * BN;
+#pragma unroll
+            for (int e = 0; e < PER; e++) {
+                const int x = lane + 32 * e, key = key_of(j, x);
+                if (x < NX && row_of(x) < BN) off[row_of(x)] = key >= 0 ? paged_offset(a.c, page[e], key % a.c.page_size) : -1;
+            }
+            __syncwarp();
+            fetch_pages(j + 1);
+            fill(k_slot(j), kbase, off);
+        };
+        auto fill_v = [&](int j) {
+            fill(v_slot(j), vbase, offs + (j & 1) * BN);
+            __syncwarp();                                    // the offsets may be replaced
+        };
+        fetch_pages(0);
+        if (two || n == 1) {
+            for (int j = 0; j < n && ok; j++) {
+                fill_k(j);
+                if (ok) fill_v(j);
+            }
+        } else if (n > 1) {
+            fill_k(0);
+            if (ok) fill_k(1);
+            for (int j = 0; j < n && ok; j++) {
+                fill_v(j);
+                if (ok && j + 2 < n) fill_k(j + 2);
+            }
+        }
+        // hand over the last slots
+        paged_cp_wait<0>();
+        if (ok) {
+            pf_fence_async();
+            const int slots = 2 * n;
+            for (int s = max(0, slots - C::LAG); s < slots; s++) pf_arrive(&full[s % ST]);
+        } else if (lane == 0) {
+            atomicOr(a.wait_status, 1u << 24);
+        }
+        __syncwarp();
+    }
+    pf_fence_before();
+    __syncthreads();
+    if (warp == C::SM_WARPS) pf_tmem_dealloc(tmem, 512);
+}
+
+// Joins the chunks of a tile: one warp per row.
+template <int D>
+__global__ void __launch_bounds__(256) paged_prefill_join_kernel(const PrefillArgs a) {
+    pdl_wait();
+    constexpr int ROWS = PfCfg<D>::ROWS, DL = D / 64;
+    const int lane = threadIdx.x & 31, r = blockIdx.z * 8 + (threadIdx.x >> 5), kvh = blockIdx.y, id = blockIdx.x;
+    const int4 ds = a.desc[id];
+    if (ds.z <= 1) return;
+    const int2 span = prefill_span(a, ds.x);
+    const int row = ds.y * ROWS + r;
+    if (row >= span.y * a.G) return;
+    const int64_t at = ((int64_t)id * a.c.kv_heads + kvh) * a.chunks * ROWS + r;
+    float m = -INFINITY;
+    for (int z = lane; z < ds.z; z += 32) m = fmaxf(m, a.ml[at + (int64_t)z * ROWS].x);
+    m = warp_max(m);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float2 acc[DL];
+#pragma unroll
+    for (int i = 0; i < DL; i++) acc[i] = make_float2(0.f, 0.f);
+#pragma unroll 4
+    for (int z = 0; z < ds.z; z++) {
+        const float2 ml = a.ml[at + (int64_t)z * ROWS];
+        const float e = ex2(ml.x - ref);
+        l = fmaf(ml.y, e, l);
+        const float2* src = (const float2*)(a.part + (at + (int64_t)z * ROWS) * D);
+#pragma unroll
+        for (int i = 0; i < DL; i++) {
+            const float2 v = src[lane + 32 * i];
+            acc[i].x = fmaf(v.x, e, acc[i].x);
+            acc[i].y = fmaf(v.y, e, acc[i].y);
+        }
+    }
+    const float inv = l > 0.f ? 1.0f / l : 0.f;
+    const int64_t tok = span.x + row / a.G;
+    const int head = kvh * a.G + row % a.G;
+    uint32_t* dst = (uint32_t*)(a.out + tok * a.out_stride + (int64_t)head * D);
+#pragma unroll
+    for (int i = 0; i < DL; i++) dst[lane + 32 * i] = pack_bf16x2(acc[i].x * inv, acc[i].y * inv);
+    if (a.lse && lane == 0) a.lse[tok * a.Hq + head] = (m + log2f(l)) * 0.6931471805599453f;
+}
+
+struct PrefillPlan { int tiles, chunks, chunk_tiles; size_t part, ml, desc, total; };
+// Tiles of one CTA each: with fewer of them than SMs their keys are cut so that one wave of CTAs covers the GPU
+// (at least four key tiles a chunk: below that a CTA's start and the join cost more than they save).
+static PrefillPlan prefill_plan(int D, int kv_heads, int seqs, int total_q, int q_heads, int max_ctx) {
+    PrefillPlan p;
+    const int rows = D == 256 ? 128 : 256, bn = D == 256 ? 64 : 128, G = q_heads / kv_heads, sms = paged_sm_count();
+    // each sequence may end in a tile of its own; none has fewer than one row
+    p.tiles = (int)std::min<int64_t>((int64_t)total_q * G / rows + std::min(seqs, total_q), (int64_t)total_q * ((G + rows - 1) / rows));
+    const int64_t ctas = (int64_t)p.tiles * kv_heads;
+    const int keys = (int)(((int64_t)max_ctx + bn - 1) / bn);
+    p.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(sms / std::max<int64_t>(ctas, 1), keys / 4));
+    p.chunk_tiles = std::max(1, (keys + p.chunks - 1) / p.chunks);
+    auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    const size_t parts = p.chunks > 1 ? (size_t)ctas * p.chunks * rows : 0;
+    p.part = up(parts * D * 4);
+    p.ml = up(parts * 8);
+    p.desc = p.chunks > 1 ? up((size_t)p.tiles * 16) : 0;
+    p.total = std::max<size_t>(16, p.part + p.ml + p.desc);
+    return p;
+}
+
+template <int D, int FEAT>
 static int32_t launch_prefill(cudaStream_t s, const PrefillArgs& a) {
+    using C = PfCfg<D>;
     static uint32_t attr_devs = 0;
     static std::mutex mu;
     int dev = 0;
@@ -212,28 +637,43 @@ static int32_t launch_prefill(cudaStream_t s, const PrefillArgs& a) {
     {
         std::lock_guard<std::mutex> lk(mu);
         if (!(attr_devs >> (dev & 31) & 1)) {
-            LTHN_CUDA_TRY(cudaFuncSetAttribute(paged_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PpCfg<D>::SMEM));
+            LTHN_CUDA_TRY(cudaFuncSetAttribute(paged_prefill_kernel<D, FEAT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::TOTAL));
             attr_devs |= 1u << (dev & 31);
         }
     }
-    // at most this many tiles: each sequence may end in a tile of its own
-    const int64_t tiles = (int64_t)a.total_q * a.G / PP_BM + a.seqs;
-    paged_prefill_kernel<D><<<dim3((unsigned)tiles, a.c.kv_heads), PP_THREADS, PpCfg<D>::SMEM, s>>>(a);
+    const int64_t ctas = (int64_t)a.tiles * a.c.kv_heads * a.chunks;
+    paged_prefill_kernel<D, FEAT><<<(unsigned)ctas, C::THREADS, C::TOTAL, s>>>(a);
     LTHN_CUDA_TRY(cudaGetLastError());
+    if (a.chunks > 1) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(a.tiles, a.c.kv_heads, C::ROWS / 8); cfg.blockDim = dim3(256); cfg.stream = s;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = at; cfg.numAttrs = 1;
+        LTHN_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_prefill_join_kernel<D>, a));
+    }
     return LTHN_OK;
+}
+template <int D>
+static int32_t launch_prefill_feat(cudaStream_t s, const PrefillArgs& a) {
+    const int f = (a.o.softcap > 0.f ? 1 : 0) | (a.o.slopes ? 2 : 0);
+    return f == 0 ? launch_prefill<D, 0>(s, a) : f == 1 ? launch_prefill<D, 1>(s, a) : f == 2 ? launch_prefill<D, 2>(s, a) : launch_prefill<D, 3>(s, a);
 }
 
 }  // namespace lthn
 
 using namespace lthn;
 
-static int32_t prefill_check(const lthn_paged_kv* cache, int32_t seqs, int32_t total_q, int32_t q_heads, int32_t max_ctx, PagedCache* c) {
+static int32_t prefill_check(const lthn_paged_kv* cache, int32_t seqs, int32_t total_q, int32_t q_heads, int32_t max_ctx, PagedCache* c, PrefillPlan* p) {
     int32_t rc;
     if ((rc = paged_check_cache("paged_prefill_attention", cache, c))) return rc;
     LTHN_REQUIRE(seqs >= 0 && total_q >= 0 && max_ctx >= 0, "paged_prefill_attention: negative size");
     LTHN_REQUIRE(seqs <= cache->seqs, "paged_prefill_attention: more sequences than the page table has");
     LTHN_REQUIRE(q_heads > 0 && q_heads <= 65535 && q_heads % cache->kv_heads == 0, "paged_prefill_attention: q_heads must be a positive multiple of kv_heads");
-    LTHN_REQUIRE((int64_t)total_q * (q_heads / cache->kv_heads) + (int64_t)seqs * 256 < (int64_t)1 << 31, "paged_prefill_attention: too many query rows");
+    LTHN_REQUIRE((int64_t)total_q * (q_heads / cache->kv_heads) < ((int64_t)1 << 31) - 512, "paged_prefill_attention: too many query rows");
+    *p = prefill_plan(cache->head_dim, cache->kv_heads, seqs, total_q, q_heads, max_ctx ? std::min(max_ctx, c->capacity) : c->capacity);
+    LTHN_REQUIRE((int64_t)p->tiles * cache->kv_heads * p->chunks < (int64_t)1 << 31, "paged_prefill_attention: too many query rows");
     return LTHN_OK;
 }
 
@@ -244,9 +684,10 @@ int32_t lthn_paged_prefill_attention_workspace(const lthn_paged_kv* cache, int32
     clear_error();
     LTHN_REQUIRE(bytes != nullptr, "paged_prefill_attention_workspace: bytes is NULL");
     PagedCache c;
+    PrefillPlan p;
     int32_t rc;
-    if ((rc = prefill_check(cache, seqs, total_q, q_heads, max_ctx, &c))) return rc;
-    *bytes = 16;
+    if ((rc = prefill_check(cache, seqs, total_q, q_heads, max_ctx, &c, &p))) return rc;
+    *bytes = p.total;
     return LTHN_OK;
 }
 
@@ -257,8 +698,9 @@ int32_t lthn_paged_prefill_attention(void* stream, const lthn_paged_kv* cache, c
     clear_error();
     const char* me = "paged_prefill_attention";
     PrefillArgs a = {};
+    PrefillPlan p;
     int32_t rc;
-    if ((rc = prefill_check(cache, seqs, total_q, q_heads, max_ctx, &a.c))) return rc;
+    if ((rc = prefill_check(cache, seqs, total_q, q_heads, max_ctx, &a.c, &p))) return rc;
     const int D = cache->head_dim;
     if ((rc = paged_check_options(me, options, D, &a.o))) return rc;
     if (seqs == 0 || total_q == 0) return LTHN_OK;
@@ -268,16 +710,21 @@ int32_t lthn_paged_prefill_attention(void* stream, const lthn_paged_kv* cache, c
     LTHN_REQUIRE(((a.q_stride | a.out_stride) & 7) == 0, "paged_prefill_attention: strides must be multiples of 8 elements");
     LTHN_REQUIRE(a.out_stride >= (int64_t)q_heads * D, "paged_prefill_attention: rows of out would overlap");
     LTHN_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15) == 0, "paged_prefill_attention: q, out and workspace must be 16-byte aligned");
-    LTHN_REQUIRE(workspace_bytes >= 16, "paged_prefill_attention: workspace too small");
+    LTHN_REQUIRE(workspace_bytes >= p.total, "paged_prefill_attention: workspace too small");
     if ((rc = paged_check_device(me, "the cache", cache->k))) return rc;
     if ((rc = paged_check_device(me, "q", q))) return rc;
     a.q = q; a.out = out; a.q_start = q_start; a.lens = kv_lens; a.lse = lse;
     a.seqs = seqs; a.total_q = total_q; a.Hq = q_heads; a.G = q_heads / cache->kv_heads;
+    a.tiles = p.tiles; a.chunks = p.chunks; a.chunk_tiles = p.chunk_tiles;
+    a.part = (float*)workspace;
+    a.ml = (float2*)((char*)workspace + p.part);
+    a.desc = (int4*)((char*)workspace + p.part + p.ml);
+    a.wait_status = device_status_word();
     a.c.status = device_paged_status_word();
     if (!a.c.status) return fail(LTHN_ERR_CUDA, "paged_prefill_attention: no device status word");
-    if (D == 64) return launch_prefill<64>((cudaStream_t)stream, a);
-    if (D == 128) return launch_prefill<128>((cudaStream_t)stream, a);
-    return launch_prefill<256>((cudaStream_t)stream, a);
+    if (D == 64) return launch_prefill_feat<64>((cudaStream_t)stream, a);
+    if (D == 128) return launch_prefill_feat<128>((cudaStream_t)stream, a);
+    return launch_prefill_feat<256>((cudaStream_t)stream, a);
 }
 
 }  // extern "C"
