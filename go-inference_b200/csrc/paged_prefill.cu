@@ -12,14 +12,17 @@
 //
 //   softmax warps   one warpgroup per row tile, one thread per row: tcgen05.ld the row's BN scores, mask, maximum, ex2, sum - all
 //                   within the thread - and tcgen05.st the weights as bf16 over the scores they came from.
-//   issuer          one lane: S = Q K^T (both operands in shared memory), O += P V (P in tensor memory, V in shared
+//   issuer          one warp: S = Q K^T (both operands in shared memory), O += P V (P in tensor memory, V in shared
 //                   memory as an N-major operand, so it is stored as it comes). There are two score buffers. Unit u uses
 //                   buffer u & 1 and the issue order is S(0) S(1) | O(0) S(2) | O(1) S(3) | ..., so that the tensor pipe
 //                   works on one buffer while the other's softmax runs. With two row tiles the buffers belong to them,
 //                   with one they alternate over its key tiles.
-//   loaders         three warps, cp.async of 16 bytes into a ring of K and V tiles in the 128-byte swizzle. Page size and strides
-//                   are arbitrary, rows that nobody sees are zeros (they may hold NaN, which a weight of zero would not
-//                   silence), so rows are fetched one by one; the offsets of a tile are formed once by the lanes.
+//   loaders         three warps fill a ring of K and V tiles in the 128-byte swizzle. Where the page size is a multiple of 8 (the
+//                   swizzle's row group) by tiled TMA, one box per page, 64 head dimensions and gcd(page size, BN) rows. V rows
+//                   that nobody sees must be zeros (they may hold NaN, which a weight of zero would not silence), so a V
+//                   tile with such rows - the last of a sequence, the first of a window - and pools of other page
+//                   sizes come row by row with cp.async of 16 bytes, zero-filled; unseen K rows may hold anything, their
+//                   scores are replaced. 8192 tokens of 32 heads: 1007 us with cp.async throughout, 541 us with TMA.
 //
 // The running maximum is only moved when a row's grew by more than 2^8: until then weights are up to 2^8, which neither
 // their bf16 rounding (relative) nor the f32 sums mind, and O in tensor memory needs no correction. A move multiplies
@@ -32,13 +35,18 @@
 // the tensor memory and return.
 #include "paged.cuh"
 
+#include <cuda.h>
+
 #include <algorithm>
 #include <mutex>
+#include <numeric>
 
 namespace lthn {
 
 struct PrefillArgs {
     PagedCache c;
+    int box;             // rows of a TMA box, 0: rows are copied one by one
+    int rows_first;      // the tensor maps' dimensions are (dim, row, head, page), else (dim, head, row, page)
     AttnOpts o;
     const uint16_t* q;
     uint16_t* out;
@@ -102,18 +110,25 @@ __device__ __forceinline__ void pf_tmem_dealloc(uint32_t taddr, uint32_t ncols) 
 __device__ __forceinline__ void pf_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void pf_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void pf_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Issued by one lane, but from code that the whole warp runs: the operands are then known to be the same for all lanes and live in
+// uniform registers, where the instruction wants them (from a one-lane branch each issue costs several register moves).
 __device__ __forceinline__ void pf_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+    asm volatile("{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void pf_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+    asm volatile("{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void pf_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void pf_tma_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ void pf_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -218,7 +233,7 @@ struct PfCfg {
 
 // FEAT bit 0: tanh cap, bit 1: distance bias
 template <int D, int FEAT>
-__global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(const PrefillArgs a) {
+__global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const PrefillArgs a) {
     using C = PfCfg<D>;
     constexpr int BN = C::BN, ST = C::ST, ROWS = C::ROWS;
     constexpr float LOG2E = 1.4426950408889634f;
@@ -236,7 +251,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
     int* scan = (int*)(tmem_slot + 2);                       // WARPS + 2 words
 
     pdl_trigger();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int kvh = blockIdx.x % a.c.kv_heads;
     const int chunk = blockIdx.x / a.c.kv_heads % a.chunks;
     const int id = blockIdx.x / a.c.kv_heads / a.chunks;
@@ -436,14 +451,14 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
     } else if (warp == C::SM_WARPS) {
         // ================================ issuer ================================
         if (C::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        if (lane == 0 && n > 0) {
+        if (n > 0) {
             // f32 accumulators, bf16 operands, M = 128; S: N = BN, both K-major; O: N = D, B is N-major
             const uint32_t base = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);
             const uint32_t idesc_s = base | ((uint32_t)(BN >> 3) << 17), idesc_o = base | (1u << 16) | ((uint32_t)(D >> 3) << 17);
-            ok = pf_wait(q_full, 0);
+            ok = __all_sync(0xffffffffu, pf_wait(q_full, 0));
             auto scores = [&](int u) {
                 const int j = two ? u >> 1 : u, qt = two ? u & 1 : 0, slot = k_slot(j), st = slot % ST;
-                ok = pf_wait(&full[st], (slot / ST) & 1);
+                ok = __all_sync(0xffffffffu, pf_wait(&full[st], (slot / ST) & 1));
                 if (!ok) return;
                 pf_fence_after();
                 const uint32_t qa = smem + qt * C::Q_BYTES, kb = smem + C::RING + st * C::KV_BYTES, d = tmem + (u & 1) * C::S_COLS;
@@ -457,7 +472,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             if (ok && units > 1) scores(1);
             for (int u = 0; u < units && ok; u++) {
                 const int j = two ? u >> 1 : u, qt = two ? u & 1 : 0, slot = v_slot(j), st = slot % ST;
-                ok = pf_wait(&full[st], (slot / ST) & 1) && pf_wait(&p_full[u & 1], (u >> 1) & 1);
+                ok = __all_sync(0xffffffffu, pf_wait(&full[st], (slot / ST) & 1) && pf_wait(&p_full[u & 1], (u >> 1) & 1));
                 if (!ok) break;
                 pf_fence_after();
                 const uint32_t vb = smem + C::RING + st * C::KV_BYTES, pa = tmem + (u & 1) * C::S_COLS, d = tmem + 256 + qt * D;
@@ -468,7 +483,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                 if (u + 2 < units) scores(u + 2);
             }
             if (!ok) {
-                atomicOr(a.wait_status, 1u << 25);
+                if (lane == 0) atomicOr(a.wait_status, 1u << 25);
                 pf_commit(drain);                            // nothing of this CTA may still run when its memory is given back
                 pf_wait(drain, 0);
             }
@@ -490,7 +505,12 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             const int rr = row_of(x), key = kt.tile(i0 + j) * BN + rr;
             return x < NX && rr < BN && key < len && (key < prefix || (key >= lo && key <= qhi)) ? key : -1;
         };
-        int page[PER];
+        auto free_slot = [&](int slot) {
+            ok = __all_sync(0xffffffffu, pf_wait(&empty[slot % ST], ((slot / ST) & 1) ^ 1));
+            return ok;
+        };
+        // ---- row by row ----
+        int page[PER];                                       // of this lane's rows of the next tile
         auto fetch_pages = [&](int j) {
 #pragma unroll
             for (int e = 0; e < PER; e++) {
@@ -498,43 +518,120 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                 page[e] = key >= 0 ? trow[key / a.c.page_size] : 0;
             }
         };
-        auto fill = [&](int slot, const uint16_t* src, const int64_t* off) {
-            const int st = slot % ST;
-            ok = __all_sync(0xffffffffu, pf_wait(&empty[st], ((slot / ST) & 1) ^ 1));
-            if (!ok) return;
-            const uint32_t dst = smem + C::RING + st * C::KV_BYTES;
-            constexpr int CPR = D / 8, RPI = 32 / CPR;       // 16-byte chunks per row, rows per instruction
+        auto set_offsets = [&](int j) {
+#pragma unroll
+            for (int e = 0; e < PER; e++) {
+                const int x = lane + 32 * e, key = key_of(j, x);
+                if (x < NX && row_of(x) < BN) offs[(j & 1) * BN + row_of(x)] = key >= 0 ? paged_offset(a.c, page[e], key % a.c.page_size) : -1;
+            }
+            __syncwarp();
+        };
+        auto copy_rows = [&](int slot, const uint16_t* src, int j) {
+            const int64_t* off = offs + (j & 1) * BN;
+            const uint32_t dst = smem + C::RING + slot % ST * C::KV_BYTES;
+            constexpr int CPR = D / 8, RPI = 32 / CPR, B = 4;    // 16-byte chunks per row, rows per instruction, instructions at once
             const int c = lane % CPR;
-#pragma unroll 4
-            for (int x0 = 0; x0 < NX; x0 += RPI) {
-                const int rr = row_of(x0 + lane / CPR);
-                if ((x0 >> 2) * 12 + lw * 4 >= BN) break;
-                const int64_t o = off[rr];
-                cp_async16_zfill(dst + (c >> 3) * C::SLAB + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), src + (o < 0 ? 0 : o) + c * 8, o < 0 ? 0 : 16);
+            src += c * 8;
+#pragma unroll 1
+            for (int x0 = 0; x0 < NX; x0 += RPI * B) {
+                int64_t o[B];
+#pragma unroll
+                for (int b = 0; b < B; b++) {
+                    const int x = x0 + b * RPI + lane / CPR;
+                    o[b] = x < NX && row_of(x) < BN ? off[row_of(x)] : -2;
+                }
+#pragma unroll
+                for (int b = 0; b < B; b++) {
+                    const int rr = row_of(x0 + b * RPI + lane / CPR);
+                    if (o[b] > -2)
+                        cp_async16_zfill(dst + (c >> 3) * C::SLAB + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), src + max(o[b], (int64_t)0), o[b] < 0 ? 0 : 16);
+                }
             }
             paged_cp_commit();
-            if (slot >= C::LAG) {
+        };
+        // ---- by pages: lane i looks after box i of a tile ----
+        const int boxes = a.box ? BN / a.box : 0;
+        int box_page = 0;
+        auto box_key = [&](int j) {                          // -1: nobody sees a row of the box
+            const int key = kt.tile(i0 + j) * BN + lane * a.box;
+            return j < n && lane < boxes && key < len && (key < prefix || (key + a.box > lo && key <= qhi)) ? key : -1;
+        };
+        auto fetch_box_page = [&](int j) {
+            const int key = box_key(j);
+            return key >= 0 ? trow[key / a.c.page_size] : 0;
+        };
+        auto copy_boxes = [&](int slot, const CUtensorMap* map, int j, int pages_of_tile) {
+            const int key = box_key(j);
+            const int in_page = key >= 0 ? key % a.c.page_size : -1;
+            const int st = slot % ST, total = boxes * (D / 64), t = lane * 3 + lw;
+            const int bx = min(t / (D / 64), 31), slab = t % (D / 64);
+            const int pg = __shfl_sync(0xffffffffu, pages_of_tile, bx), row = __shfl_sync(0xffffffffu, in_page, bx);
+            if (t < total && row >= 0) {
+                mbar_expect_tx(&full[st], a.box * 128);
+                pf_tma_4d(smem + C::RING + st * C::KV_BYTES + slab * C::SLAB + bx * a.box * 128, map, slab * 64, a.rows_first ? row : kvh,
+                          a.rows_first ? kvh : row, pg, &full[st]);
+            } else {
+                pf_arrive(&full[st]);
+            }
+            __syncwarp();
+        };
+        // rows copied one by one are handed over when they have landed: LAG slots later where every slot is copied so
+        auto hand_over = [&](int slot) {
+            if (a.box) {
+                paged_cp_wait<0>();
+                pf_fence_async();
+                pf_arrive(&full[slot % ST]);
+            } else if (slot >= C::LAG) {
                 paged_cp_wait<C::LAG>();
                 pf_fence_async();
                 pf_arrive(&full[(slot - C::LAG) % ST]);
             }
         };
+        static_assert(16 * (D / 64) <= 96, "a lane issues one box");
+        int v_page = 0, v_page2 = 0;                         // box pages of the K tiles whose V tile is still to come
         auto fill_k = [&](int j) {
-            int64_t* off = offs + (j & 1) * BN;
-#pragma unroll
-            for (int e = 0; e < PER; e++) {
-                const int x = lane + 32 * e, key = key_of(j, x);
-                if (x < NX && row_of(x) < BN) off[row_of(x)] = key >= 0 ? paged_offset(a.c, page[e], key % a.c.page_size) : -1;
+            const int slot = k_slot(j);
+            if (!a.box) {
+                set_offsets(j);
+                fetch_pages(j + 1);
+                if (!free_slot(slot)) return;
+                copy_rows(slot, kbase, j);
+            } else {
+                const int pages_of_tile = box_page;
+                box_page = fetch_box_page(j + 1);
+                v_page2 = v_page;
+                v_page = pages_of_tile;
+                if (!free_slot(slot)) return;
+                if (__all_sync(0xffffffffu, box_key(j) < 0 || (unsigned)pages_of_tile < (unsigned)a.c.pages)) {
+                    copy_boxes(slot, &k_map, j, pages_of_tile);
+                    return;
+                }
+                fetch_pages(j);                              // a bad page: reported, and zeros
+                set_offsets(j);
+                copy_rows(slot, kbase, j);
             }
-            __syncwarp();
-            fetch_pages(j + 1);
-            fill(k_slot(j), kbase, off);
+            hand_over(slot);
         };
         auto fill_v = [&](int j) {
-            fill(v_slot(j), vbase, offs + (j & 1) * BN);
+            const int slot = v_slot(j);
+            if (!free_slot(slot)) return;
+            if (a.box) {
+                const int pages_of_tile = two || n == 1 || j == n - 1 ? v_page : v_page2;
+                const int k0 = kt.tile(i0 + j) * BN;
+                const bool whole = k0 + BN <= len && (k0 + BN <= prefix || (k0 >= lo && k0 + BN - 1 <= qhi));
+                if (whole && __all_sync(0xffffffffu, box_key(j) < 0 || (unsigned)pages_of_tile < (unsigned)a.c.pages)) {
+                    copy_boxes(slot, &v_map, j, pages_of_tile);
+                    return;
+                }
+                fetch_pages(j);
+                set_offsets(j);
+            }
+            copy_rows(slot, vbase, j);
+            hand_over(slot);
             __syncwarp();                                    // the offsets may be replaced
         };
-        fetch_pages(0);
+        if (a.box) box_page = fetch_box_page(0);
+        else fetch_pages(0);
         if (two || n == 1) {
             for (int j = 0; j < n && ok; j++) {
                 fill_k(j);
@@ -550,11 +647,11 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         }
         // hand over the last slots
         paged_cp_wait<0>();
-        if (ok) {
+        if (ok && !a.box) {
             pf_fence_async();
             const int slots = 2 * n;
             for (int s = max(0, slots - C::LAG); s < slots; s++) pf_arrive(&full[s % ST]);
-        } else if (lane == 0) {
+        } else if (!ok && lane == 0) {
             atomicOr(a.wait_status, 1u << 24);
         }
         __syncwarp();
@@ -627,8 +724,38 @@ static PrefillPlan prefill_plan(int D, int kv_heads, int seqs, int total_q, int 
     return p;
 }
 
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiled encode_tiled() {
+    static EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess
+                   ? (EncodeTiled)p : nullptr;
+    }();
+    return fn;
+}
+// Tensor maps of the pools with boxes of 64 head dimensions by gcd(page size, bn) rows. False where the pool has no such form (page
+// sizes that are not multiples of 8 rows, strides that do not nest): its rows are copied one by one.
+static bool prefill_maps(const PagedCache& c, int D, int bn, CUtensorMap* km, CUtensorMap* vm, int* box, int* rows_first) {
+    if (c.page_size % 8 || !encode_tiled()) return false;
+    *box = std::gcd(c.page_size, bn);
+    *rows_first = c.row_stride < c.head_stride;
+    const int64_t s1 = *rows_first ? c.row_stride : c.head_stride, s2 = *rows_first ? c.head_stride : c.row_stride, s3 = c.page_stride;
+    const int64_t n1 = *rows_first ? c.page_size : c.kv_heads, n2 = *rows_first ? c.kv_heads : c.page_size;
+    if (s1 < D || s2 % s1 || s3 % s2 || s2 < s1 * n1 || s3 < s2 * n2 || s3 >= (int64_t)1 << 39) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)n1, (cuuint64_t)n2, (cuuint64_t)std::max(1, c.pages)};
+    const cuuint64_t strides[3] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2, (cuuint64_t)s3 * 2};
+    const cuuint32_t boxes[4] = {64, *rows_first ? (cuuint32_t)*box : 1, *rows_first ? 1 : (cuuint32_t)*box, 1}, es[4] = {1, 1, 1, 1};
+    for (int i = 0; i < 2; i++)
+        if (encode_tiled()(i ? vm : km, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, i ? c.v : c.k, dims, strides, boxes, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return false;
+    return true;
+}
+
 template <int D, int FEAT>
-static int32_t launch_prefill(cudaStream_t s, const PrefillArgs& a) {
+static int32_t launch_prefill(cudaStream_t s, PrefillArgs a) {
     using C = PfCfg<D>;
     static uint32_t attr_devs = 0;
     static std::mutex mu;
@@ -642,7 +769,9 @@ static int32_t launch_prefill(cudaStream_t s, const PrefillArgs& a) {
         }
     }
     const int64_t ctas = (int64_t)a.tiles * a.c.kv_heads * a.chunks;
-    paged_prefill_kernel<D, FEAT><<<(unsigned)ctas, C::THREADS, C::TOTAL, s>>>(a);
+    CUtensorMap km = {}, vm = {};
+    if (!prefill_maps(a.c, D, C::BN, &km, &vm, &a.box, &a.rows_first)) a.box = 0;
+    paged_prefill_kernel<D, FEAT><<<(unsigned)ctas, C::THREADS, C::TOTAL, s>>>(km, vm, a);
     LTHN_CUDA_TRY(cudaGetLastError());
     if (a.chunks > 1) {
         cudaLaunchConfig_t cfg = {};

@@ -381,6 +381,27 @@ def test_prefill_masks(lthn, mask, D, kv, G):
     check_prefill(lthn, c, rng.standard_normal((sum(new), kv * G, D)), new, o, kws)
 
 
+@pytest.mark.parametrize("D,kv,G", [(128, 1, 2), (64, 2, 1), (256, 1, 1)])
+@pytest.mark.parametrize("page", [16, 5])
+@pytest.mark.parametrize("new", [[400], [30, 90]])
+def test_prefill_growing_scores(lthn, D, kv, G, page, new):
+    """Keys that grow along the sequence: the running maximum moves again and again, and what was summed before is scaled down."""
+    rng = np.random.default_rng(25)
+    past = [500, 333][:len(new)]
+    lens = [a + b for a, b in zip(new, past)]
+    c = HostCache(rng, lens, page, kv, D)
+    for s, n in enumerate(lens):
+        k, v = c.get(s, n)
+        c.put(s, np.arange(n), k * (0.2 + np.arange(n)[:, None, None] / 150.0), v)
+    q = rng.standard_normal((sum(new), kv * G, D))
+    x, got, lse, start = run_prefill(lthn, c, q, new)
+    for s, n in enumerate(lens):
+        rows = slice(start[s], start[s + 1])
+        want, wl, mag = attention(c, s, x[rows], n - new[s], n)
+        close(got[rows], want, 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 8 * W) * mag)      # |k| is up to 6 times larger, and so are the errors of s
+        assert np.all(np.abs(lse[rows] - wl) <= 8 * W + 2.0 ** -22 * np.abs(wl))
+
+
 def test_prefill_many_sequences(lthn):
     rng = np.random.default_rng(21)
     new = [int(n) for n in rng.integers(0, 7, 300)]
