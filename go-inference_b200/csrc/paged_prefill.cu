@@ -10,13 +10,14 @@
 // (two: two accumulators of head_dim columns fit the tensor memory beside two score tiles for head_dim 64 and 128) and on
 // BN keys at a time.
 //
-//   softmax warps   one warpgroup per row tile, one thread per row: tcgen05.ld the row's BN scores, mask, maximum, ex2, sum - all
-//                   within the thread - and tcgen05.st the weights as bf16 over the scores they came from.
+//   softmax warps   two warpgroups, one per score buffer, one thread per row: tcgen05.ld the row's BN scores, mask, maximum, ex2,
+//                   sum - all within the thread - and tcgen05.st the weights as bf16 over the scores they came from.
 //   issuer          one warp: S = Q K^T (both operands in shared memory), O += P V (P in tensor memory, V in shared
 //                   memory as an N-major operand, so it is stored as it comes). There are two score buffers. Unit u uses
 //                   buffer u & 1 and the issue order is S(0) S(1) | O(0) S(2) | O(1) S(3) | ..., so that the tensor pipe
-//                   works on one buffer while the other's softmax runs. With two row tiles the buffers belong to them,
-//                   with one they alternate over its key tiles.
+//                   works on one buffer while the other's softmax runs. With two row tiles the buffers belong to them;
+//                   with one they alternate over its key tiles, and the warpgroups pass the running maximum of a row to one
+//                   another (the sums stay apart until the end), which leaves only load and maximum in sequence.
 //   loaders         three warps fill a ring of K and V tiles in the 128-byte swizzle. Where the page size is a multiple of 8 (the
 //                   swizzle's row group) by tiled TMA, one box per page, 64 head dimensions and gcd(page size, BN) rows. V rows
 //                   that nobody sees must be zeros (they may hold NaN, which a weight of zero would not silence), so a V
@@ -203,6 +204,23 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 // the n lowest bits of a word, n of any size and sign
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+// two f32 operations in one instruction
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ float rcp_approx(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -214,7 +232,7 @@ struct PfCfg {
     static constexpr int NQ = D == 256 ? 1 : 2;              // row tiles per CTA
     static constexpr int BN = D == 256 ? 64 : 128;           // keys per tile
     static constexpr int ROWS = NQ * 128;
-    static constexpr int SM_WARPS = NQ * 4;                  // softmax warps
+    static constexpr int SM_WARPS = 8;                       // softmax warps
     static constexpr int WARPS = SM_WARPS + 4;               // + issuer + three loaders
     static constexpr int THREADS = WARPS * 32;
     static constexpr int Q_BYTES = 128 * D * 2;              // one row tile
@@ -224,7 +242,9 @@ struct PfCfg {
     static constexpr int RING = NQ * Q_BYTES;                // offsets in shared memory
     static constexpr int OFFS = RING + ST * KV_BYTES;        // [2][BN] row offsets
     static constexpr int BARS = OFFS + 2 * BN * 8;
-    static constexpr int TOTAL = BARS + 512;
+    // one row tile: the rows' running maximum, in the place of the second row tile where there is room for one
+    static constexpr int ROW_MAX = NQ == 2 ? Q_BYTES : BARS + 512;
+    static constexpr int TOTAL = BARS + 512 + (NQ == 2 ? 0 : 512);
     static constexpr int S_COLS = BN;                        // tensor memory: two score buffers, then the outputs at column 256
     static constexpr int LAG = 2;                            // ring slots in flight behind the one being filled
     static_assert(LAG <= ST - 3, "a slot is handed over before the one that frees its successor is waited for");
@@ -245,7 +265,8 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
     uint64_t* o_done = p_full + 2;                           // [2] per row tile: O(u) has been added, all but the last
     uint64_t* o_last = o_done + 2;                           // [2] the last has (a barrier of its own: with one row tile the softmax
                                                              //     may be two units ahead, which a parity cannot tell from none)
-    uint64_t* q_full = o_last + 2;
+    uint64_t* turn = o_last + 2;                             // [4] one row tile: the maximum of key tile j is out, per 32 rows
+    uint64_t* q_full = turn + 4;
     uint64_t* drain = q_full + 1;
     uint32_t* tmem_slot = (uint32_t*)(drain + 1);
     int* scan = (int*)(tmem_slot + 2);                       // WARPS + 2 words
@@ -279,6 +300,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
     if (tid == 0) {
         for (int s = 0; s < ST; s++) { mbar_init(&full[s], 96); mbar_init(&empty[s], 1); }
         for (int b = 0; b < 2; b++) { mbar_init(&s_full[b], 1); mbar_init(&p_full[b], 128); mbar_init(&o_done[b], 1); mbar_init(&o_last[b], 1); }
+        for (int w = 0; w < 4; w++) mbar_init(&turn[w], 1);
         mbar_init(q_full, C::SM_WARPS * 32);
         mbar_init(drain, 1);
         mbar_fence_init();
@@ -297,15 +319,15 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
 
     if (warp < C::SM_WARPS) {
         // ================================ softmax ================================
-        if (C::NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        const int qt = C::NQ == 2 ? warp >> 2 : 0;
-        const int r = (warp & 3) * 32 + lane;                // row within the row tile = tensor memory lane
-        {   // queries into shared memory: a warp takes 32 rows, D/8 lanes a row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int wg = warp >> 2, qt = two ? wg : 0;         // score buffer = warpgroup; row tile
+        const int wr = (warp & 3) * 32, r = wr + lane;       // row within the row tile = tensor memory lane
+        {   // queries into shared memory: the warps of a row tile take 32 rows each, D/8 lanes a row
             constexpr int CPR = D / 8;
             unsigned char* qs = pf_smem + qt * C::Q_BYTES;
 #pragma unroll 4
-            for (int x = lane; x < 32 * CPR; x += 32) {
-                const int rr = (warp & 3) * 32 + x / CPR, c = x % CPR, row = row0 + qt * 128 + rr;
+            for (int x = two ? lane : lane + 32 * wg; x < 32 * CPR; x += two ? 32 : 64) {
+                const int rr = wr + x / CPR, c = x % CPR, row = row0 + qt * 128 + rr;
                 uint4 v = make_uint4(0, 0, 0, 0);
                 if (row < nrows) v = *(const uint4*)(a.q + (span.x + row / a.G) * a.q_stride + (int64_t)(kvh * a.G + row % a.G) * D + c * 8);
                 *(uint4*)(qs + (c >> 3) * (128 * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
@@ -314,143 +336,175 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             pf_arrive(q_full);
             __syncwarp();
         }
-        if (qt == 0 || two) {
-            const int row = row0 + qt * 128 + r;
-            const bool live = row < nrows;
-            const int token = row / a.G, head = kvh * a.G + row - token * a.G;
-            const int qpos = pos0 + token;
-            // visible: key < pre, or klo <= key < khi
-            const int pre = prefix, khi = min(qpos + 1, len), klo = a.o.window > 0 ? qpos - a.o.window + 1 : 0;
-            // plain scores stay as the product left them, the others are brought to log2 units first
-            const float c1 = FEAT ? 1.0f : a.o.scale * LOG2E;
-            const float cap2 = a.o.softcap * LOG2E, cin = FEAT & 1 ? 2.0f * LOG2E * a.o.scale / a.o.softcap : a.o.scale * LOG2E;
-            const float slope = (FEAT & 2) && live ? a.o.slopes[head] * LOG2E : 0.f;
-            const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-            const uint32_t o_addr = lanes + 256 + qt * D;
-            float m = -INFINITY, l = 0.f;                    // reference maximum (units of the scores), sum
+        const int row = row0 + qt * 128 + r;
+        const bool live = row < nrows;
+        const int token = row / a.G, head = kvh * a.G + row - token * a.G;
+        const int qpos = pos0 + token;
+        // visible: key < pre, or klo <= key < khi
+        const int pre = prefix, khi = min(qpos + 1, len), klo = a.o.window > 0 ? qpos - a.o.window + 1 : 0;
+        // plain scores stay as the product left them, the others are brought to log2 units first
+        const float c1 = FEAT ? 1.0f : a.o.scale * LOG2E;
+        const float cap2 = a.o.softcap * LOG2E, cin = FEAT & 1 ? 2.0f * LOG2E * a.o.scale / a.o.softcap : a.o.scale * LOG2E;
+        const float slope = (FEAT & 2) && live ? a.o.slopes[head] * LOG2E : 0.f;
+        const uint32_t lanes = tmem + ((uint32_t)wr << 16);
+        const uint32_t s_addr = lanes + wg * C::S_COLS, o_addr = lanes + 256 + qt * D;
+        float* row_max = (float*)(pf_smem + C::ROW_MAX);     // one row tile only
+        float m = -INFINITY, l = 0.f;                        // reference maximum (units of the scores), sum relative to it
 
-            for (int j = 0; j < n; j++) {
-                const int u = two ? 2 * j + qt : j, buf = u & 1;
-                ok = __all_sync(0xffffffffu, pf_wait(&s_full[buf], (u >> 1) & 1));
+        for (int j = two ? 0 : wg; j < n; j += two ? 1 : 2) {
+            const int use = two ? j : j >> 1;                // of this warpgroup's buffer
+            ok = __all_sync(0xffffffffu, pf_wait(&s_full[wg], use & 1));
+            if (!ok) break;
+            pf_fence_after();
+            float s[BN];
+#pragma unroll
+            for (int x = 0; x < BN; x += 32) pf_ld32(s_addr + x, s + x);
+            pf_ld_wait();
+            const int k0 = kt.tile(i0 + j) * BN;
+            if (FEAT & 1) {
+                // cap tanh(x scale / cap) = cap (1 - 2 / (1 + e^(2 x scale / cap)))
+#pragma unroll
+                for (int x = 0; x < BN; x++) s[x] = fmaf(-2.0f * cap2, rcp_approx(1.0f + ex2(s[x] * cin)), cap2);
+            }
+            if (FEAT & 2) {
+                const float gap = (float)(qpos - k0);
+#pragma unroll
+                for (int x = 0; x < BN; x++) s[x] = fmaf(-slope, fabsf(gap - (float)x), FEAT & 1 ? s[x] : s[x] * cin);
+            }
+            const bool all = !live || k0 + BN <= pre || (k0 >= klo && k0 + BN <= khi);
+            if (!__all_sync(0xffffffffu, all)) {
+                const int p = pre - k0, lo = klo - k0, hi = khi - k0;
+#pragma unroll
+                for (int x0 = 0; x0 < BN; x0 += 32) {
+                    const uint32_t seen = low_bits(p - x0) | (low_bits(hi - x0) & ~low_bits(lo - x0));
+#pragma unroll
+                    for (int x = 0; x < 32; x++) s[x0 + x] = seen >> x & 1 ? s[x0 + x] : -INFINITY;
+                }
+            }
+            float mx[4];                                     // four chains
+#pragma unroll
+            for (int x = 0; x < 4; x++) mx[x] = max3(s[x], s[x + 4], s[x + 8]);
+#pragma unroll
+            for (int x = 12; x + 8 <= BN; x += 8)
+#pragma unroll
+                for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], s[x + e], s[x + 4 + e]);
+            static_assert((BN - 12) % 8 == 4, "the last four scores");
+            mx[0] = max3(mx[0], s[BN - 4], s[BN - 3]);
+            mx[1] = max3(mx[1], s[BN - 2], s[BN - 1]);
+            if (!two && j > 0) {                             // the row's maximum so far, from the other warpgroup
+                ok = __all_sync(0xffffffffu, pf_wait(&turn[warp & 3], (j - 1) & 1));
+                if (!ok) break;
+                const float mo = row_max[r];
+                if (mo != m) {                               // it has moved: this warpgroup's sum follows
+                    l = m == -INFINITY ? 0.f : l * ex2((m - mo) * c1);
+                    m = mo;
+                }
+                __syncwarp();
+            }
+            const float mnew = max3(fmaxf(m, mx[0]), mx[1], fmaxf(mx[2], mx[3]));
+            const bool move = __any_sync(0xffffffffu, (mnew - m) * c1 > 8.0f);
+            const float mold = m;
+            if (move) {
+                l = m == -INFINITY ? 0.f : l * ex2((m - mnew) * c1);
+                m = mnew;
+            }
+            if (!two) {
+                row_max[r] = m;
+                __syncwarp();
+                if (lane == 0) pf_arrive(&turn[warp & 3]);
+                __syncwarp();
+            }
+            if (move && j > 0) {
+                const float alpha = mold == -INFINITY ? 0.f : ex2((mold - mnew) * c1);
+                ok = __all_sync(0xffffffffu, pf_wait(&o_done[qt], (j - 1) & 1));
                 if (!ok) break;
                 pf_fence_after();
-                const uint32_t s_addr = lanes + buf * C::S_COLS;
-                float s[BN];
 #pragma unroll
-                for (int x = 0; x < BN; x += 32) pf_ld32(s_addr + x, s + x);
-                pf_ld_wait();
-                const int k0 = kt.tile(i0 + j) * BN;
-                if (FEAT & 1) {
-                    // cap tanh(x scale / cap) = cap (1 - 2 / (1 + e^(2 x scale / cap)))
+                for (int x = 0; x < D; x += 32) {
+                    float o[32];
+                    pf_ld32(o_addr + x, o);
+                    pf_ld_wait();
 #pragma unroll
-                    for (int x = 0; x < BN; x++) s[x] = fmaf(-2.0f * cap2, rcp_approx(1.0f + ex2(s[x] * cin)), cap2);
+                    for (int e = 0; e < 32; e++) o[e] *= alpha;
+                    pf_st32(o_addr + x, o);
                 }
-                if (FEAT & 2) {
-                    const float gap = (float)(qpos - k0);
-#pragma unroll
-                    for (int x = 0; x < BN; x++) s[x] = fmaf(-slope, fabsf(gap - (float)x), FEAT & 1 ? s[x] : s[x] * cin);
-                }
-                const bool all = !live || k0 + BN <= pre || (k0 >= klo && k0 + BN <= khi);
-                if (!__all_sync(0xffffffffu, all)) {
-                    const int p = pre - k0, lo = klo - k0, hi = khi - k0;
-#pragma unroll
-                    for (int x0 = 0; x0 < BN; x0 += 32) {
-                        const uint32_t seen = low_bits(p - x0) | (low_bits(hi - x0) & ~low_bits(lo - x0));
-#pragma unroll
-                        for (int x = 0; x < 32; x++) s[x0 + x] = seen >> x & 1 ? s[x0 + x] : -INFINITY;
-                    }
-                }
-                float mx = max3(s[0], s[1], s[2]);
-#pragma unroll
-                for (int x = 3; x + 1 < BN; x += 2) mx = max3(mx, s[x], s[x + 1]);
-                mx = fmaxf(mx, s[BN - 1]);
-                const float mnew = fmaxf(m, mx);
-                if (__any_sync(0xffffffffu, (mnew - m) * c1 > 8.0f)) {
-                    const float alpha = m == -INFINITY ? 0.f : ex2((m - mnew) * c1);
-                    m = mnew;
-                    l *= alpha;
-                    if (j > 0) {
-                        ok = __all_sync(0xffffffffu, pf_wait(&o_done[qt], (j - 1) & 1));
-                        if (!ok) break;
-                        pf_fence_after();
-#pragma unroll
-                        for (int x = 0; x < D; x += 32) {
-                            float o[32];
-                            pf_ld32(o_addr + x, o);
-                            pf_ld_wait();
-#pragma unroll
-                            for (int e = 0; e < 32; e++) o[e] *= alpha;
-                            pf_st32(o_addr + x, o);
-                        }
-                    }
-                }
-                const float neg = m == -INFINITY ? 0.f : -m * c1;
-                float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-                for (int x = 0; x < BN; x += 32) {
-                    uint32_t w[16];
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const float p0 = ex2(fmaf(s[x + e], c1, neg)), p1 = ex2(fmaf(s[x + e + 1], c1, neg));
-                        l0 += p0;
-                        l1 += p1;
-                        w[e / 2] = pack_bf16x2(p0, p1);
-                    }
-                    pf_st16(s_addr + x / 2, w);
-                }
-                l += l0 + l1;
-                pf_st_wait();
-                pf_fence_before();
-                pf_arrive(&p_full[buf]);
             }
-            if (ok && n > 0) ok = __all_sync(0xffffffffu, pf_wait(&o_last[qt], 0));
-            if (!ok && lane == 0) atomicOr(a.wait_status, 1u << 26);
-            if (ok) {
-                pf_fence_after();
-                const int64_t tok = span.x + token;
-                const float m2 = m * c1;                     // log2 units (c1 > 0)
-                if (used == 1) {
-                    const float inv = l > 0.f ? 1.0f / l : 0.f;
-                    uint16_t* dst = a.out + tok * a.out_stride + (int64_t)head * D;
-#pragma unroll 1
-                    for (int x = 0; x < D; x += 32) {
-                        float o[32];
-                        __syncwarp();                        // the stores below are not made by all lanes, the loads have to be
-                        if (n > 0) {
-                            pf_ld32(o_addr + x, o);
-                            pf_ld_wait();
-                        } else {
+            const float neg = m == -INFINITY ? 0.f : -m * c1;
+            const uint64_t c2 = pack2(c1, c1), n2 = pack2(neg, neg);
+            uint64_t sum[2] = {0, 0};
 #pragma unroll
-                            for (int e = 0; e < 32; e++) o[e] = 0.f;
-                        }
-                        if (live) {
+            for (int x = 0; x < BN; x += 32) {
+                uint32_t w[16];
 #pragma unroll
-                            for (int e = 0; e < 32; e += 8)
-                                *(uint4*)(dst + x + e) = make_uint4(pack_bf16x2(o[e] * inv, o[e + 1] * inv), pack_bf16x2(o[e + 2] * inv, o[e + 3] * inv),
-                                                                    pack_bf16x2(o[e + 4] * inv, o[e + 5] * inv), pack_bf16x2(o[e + 6] * inv, o[e + 7] * inv));
-                        }
-                    }
-                    if (live && a.lse) a.lse[tok * a.Hq + head] = (m2 + log2f(l)) * 0.6931471805599453f;
-                } else {
-                    const int64_t at = (((int64_t)id * a.c.kv_heads + kvh) * a.chunks + chunk) * ROWS + qt * 128 + r;
-#pragma unroll 1
-                    for (int x = 0; x < D; x += 32) {
-                        float o[32];
-                        __syncwarp();
-                        pf_ld32(o_addr + x, o);
-                        pf_ld_wait();
-                        if (live) {
-#pragma unroll
-                            for (int e = 0; e < 32; e += 4) *(float4*)(a.part + at * D + x + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                        }
-                    }
-                    if (live) a.ml[at] = make_float2(m2, l);
+                for (int e = 0; e < 32; e += 2) {
+                    float p0, p1;
+                    unpack2(fma2(pack2(s[x + e], s[x + e + 1]), c2, n2), p0, p1);
+                    p0 = ex2(p0);
+                    p1 = ex2(p1);
+                    sum[e / 2 & 1] = add2(sum[e / 2 & 1], pack2(p0, p1));
+                    w[e / 2] = pack_bf16x2(p0, p1);
                 }
+                pf_st16(s_addr + x / 2, w);
+            }
+            pf_st_wait();
+            pf_fence_before();
+            pf_arrive(&p_full[wg]);
+            float l0, l1;
+            unpack2(add2(sum[0], sum[1]), l0, l1);
+            l += l0 + l1;
+        }
+        if (ok && n > 0) ok = __all_sync(0xffffffffu, pf_wait(&o_last[qt], 0));
+        if (!ok && lane == 0) atomicOr(a.wait_status, 1u << 26);
+        int x0 = 0, x1 = D;                                  // output columns of this warpgroup
+        if (!two) {
+            // the two sums of a row meet, over the ring that nothing uses any more; each warpgroup stores half of the columns
+            float2* sums = (float2*)(pf_smem + C::RING);
+            sums[wg * 128 + r] = make_float2(m, l);
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const float2 other = sums[(wg ^ 1) * 128 + r];
+            const float mm = fmaxf(m, other.x);              // the later of the two is the maximum O is relative to
+            l = (m == -INFINITY ? 0.f : l * ex2((m - mm) * c1)) + (other.x == -INFINITY ? 0.f : other.y * ex2((other.x - mm) * c1));
+            m = mm;
+            x0 = wg * (D / 2);
+            x1 = x0 + D / 2;
+        }
+        if (ok) {
+            pf_fence_after();
+            const int64_t tok = span.x + token;
+            const float m2 = m * c1;                         // log2 units (c1 > 0)
+            const float inv = l > 0.f ? 1.0f / l : 0.f;
+            uint16_t* dst = a.out + tok * a.out_stride + (int64_t)head * D;
+            const int64_t at = (((int64_t)id * a.c.kv_heads + kvh) * a.chunks + chunk) * ROWS + qt * 128 + r;
+#pragma unroll 1
+            for (int x = x0; x < x1; x += 32) {
+                float o[32];
+                __syncwarp();                                // the stores below are not made by all lanes, the loads have to be
+                if (n > 0) {
+                    pf_ld32(o_addr + x, o);
+                    pf_ld_wait();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = 0.f;
+                }
+                if (!live) continue;
+                if (used == 1) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8)
+                        *(uint4*)(dst + x + e) = make_uint4(pack_bf16x2(o[e] * inv, o[e + 1] * inv), pack_bf16x2(o[e + 2] * inv, o[e + 3] * inv),
+                                                            pack_bf16x2(o[e + 4] * inv, o[e + 5] * inv), pack_bf16x2(o[e + 6] * inv, o[e + 7] * inv));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) *(float4*)(a.part + at * D + x + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                }
+            }
+            if (live && x0 == 0) {
+                if (used > 1) a.ml[at] = make_float2(m2, l);
+                else if (a.lse) a.lse[tok * a.Hq + head] = (m2 + log2f(l)) * 0.6931471805599453f;
             }
         }
     } else if (warp == C::SM_WARPS) {
         // ================================ issuer ================================
-        if (C::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (n > 0) {
             // f32 accumulators, bf16 operands, M = 128; S: N = BN, both K-major; O: N = D, B is N-major
             const uint32_t base = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);
@@ -491,7 +545,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         __syncwarp();
     } else {
         // ================================ loaders ================================
-        if (C::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         const int lw = warp - C::SM_WARPS - 1;
         constexpr int NX = (BN / 4 + 2) / 3 * 4;             // rows of a warp: every third group of four
         constexpr int PER = (NX + 31) / 32;
@@ -704,17 +758,27 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const PrefillAr
 }
 
 struct PrefillPlan { int tiles, chunks, chunk_tiles; size_t part, ml, desc, total; };
-// Tiles of one CTA each: with fewer of them than SMs their keys are cut so that one wave of CTAs covers the GPU
-// (at least four key tiles a chunk: below that a CTA's start and the join cost more than they save).
-static PrefillPlan prefill_plan(int D, int kv_heads, int seqs, int total_q, int q_heads, int max_ctx) {
+// Cutting the keys of a tile. A CTA holds an SM, so with `work` key tiles in all an SM has work / SMs of them to do: a tile whose keys are
+// a good deal more than half of that is cut, so that its longest piece does not decide the time (prompts: the last rows see
+// twice the average; chunks behind contexts of different lengths). Not below four key tiles: a CTA's start, its partial
+// output and the join then cost more than they save.
+static PrefillPlan prefill_plan(int D, int kv_heads, int seqs, int total_q, int q_heads, int max_ctx, int window, int has_prefix) {
     PrefillPlan p;
     const int rows = D == 256 ? 128 : 256, bn = D == 256 ? 64 : 128, G = q_heads / kv_heads, sms = paged_sm_count();
     // each sequence may end in a tile of its own; none has fewer than one row
     p.tiles = (int)std::min<int64_t>((int64_t)total_q * G / rows + std::min(seqs, total_q), (int64_t)total_q * ((G + rows - 1) / rows));
     const int64_t ctas = (int64_t)p.tiles * kv_heads;
-    const int keys = (int)(((int64_t)max_ctx + bn - 1) / bn);
-    p.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(sms / std::max<int64_t>(ctas, 1), keys / 4));
-    p.chunk_tiles = std::max(1, (keys + p.chunks - 1) / p.chunks);
+    // key tiles of the longest row tile, and of an average one: the mean over a sequence's new rows is half of them less
+    double keys = max_ctx, mean = std::max(0.5 * max_ctx, max_ctx - 0.5 * total_q / std::max(1, seqs));
+    if (window > 0 && !has_prefix) {
+        const double seen = (double)window + rows / G + bn;
+        keys = std::min(keys, seen);
+        mean = std::min(mean, seen);
+    }
+    const double longest = keys / bn, work = std::max(1.0, mean / bn) * ctas;
+    const double piece = std::max(4.0, work / (2.0 * sms));
+    p.chunks = (int)std::max(1.0, std::min(longest / piece, 1024.0));
+    p.chunk_tiles = std::max(1, (int)((longest + p.chunks - 1) / p.chunks));
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
     const size_t parts = p.chunks > 1 ? (size_t)ctas * p.chunks * rows : 0;
     p.part = up(parts * D * 4);
@@ -794,14 +858,19 @@ static int32_t launch_prefill_feat(cudaStream_t s, const PrefillArgs& a) {
 
 using namespace lthn;
 
-static int32_t prefill_check(const lthn_paged_kv* cache, int32_t seqs, int32_t total_q, int32_t q_heads, int32_t max_ctx, PagedCache* c, PrefillPlan* p) {
+static int32_t prefill_check(const lthn_paged_kv* cache, int32_t seqs, int32_t total_q, int32_t q_heads, int32_t max_ctx, PagedCache* c) {
     int32_t rc;
     if ((rc = paged_check_cache("paged_prefill_attention", cache, c))) return rc;
     LTHN_REQUIRE(seqs >= 0 && total_q >= 0 && max_ctx >= 0, "paged_prefill_attention: negative size");
     LTHN_REQUIRE(seqs <= cache->seqs, "paged_prefill_attention: more sequences than the page table has");
     LTHN_REQUIRE(q_heads > 0 && q_heads <= 65535 && q_heads % cache->kv_heads == 0, "paged_prefill_attention: q_heads must be a positive multiple of kv_heads");
     LTHN_REQUIRE((int64_t)total_q * (q_heads / cache->kv_heads) < ((int64_t)1 << 31) - 512, "paged_prefill_attention: too many query rows");
-    *p = prefill_plan(cache->head_dim, cache->kv_heads, seqs, total_q, q_heads, max_ctx ? std::min(max_ctx, c->capacity) : c->capacity);
+    return LTHN_OK;
+}
+static int32_t prefill_plan_for(const lthn_paged_kv* cache, const PagedCache& c, const lthn_attn_options* o, int32_t seqs, int32_t total_q, int32_t q_heads,
+                                int32_t max_ctx, PrefillPlan* p) {
+    *p = prefill_plan(cache->head_dim, cache->kv_heads, seqs, total_q, q_heads, max_ctx ? std::min(max_ctx, c.capacity) : c.capacity, o ? o->window : 0,
+                      o && o->prefix_lens);
     LTHN_REQUIRE((int64_t)p->tiles * cache->kv_heads * p->chunks < (int64_t)1 << 31, "paged_prefill_attention: too many query rows");
     return LTHN_OK;
 }
@@ -815,7 +884,9 @@ int32_t lthn_paged_prefill_attention_workspace(const lthn_paged_kv* cache, int32
     PagedCache c;
     PrefillPlan p;
     int32_t rc;
-    if ((rc = prefill_check(cache, seqs, total_q, q_heads, max_ctx, &c, &p))) return rc;
+    if ((rc = prefill_check(cache, seqs, total_q, q_heads, max_ctx, &c))) return rc;
+    // without options: a window only makes the longest and the average tile shorter and more alike, so fewer pieces
+    if ((rc = prefill_plan_for(cache, c, nullptr, seqs, total_q, q_heads, max_ctx, &p))) return rc;
     *bytes = p.total;
     return LTHN_OK;
 }
@@ -829,7 +900,7 @@ int32_t lthn_paged_prefill_attention(void* stream, const lthn_paged_kv* cache, c
     PrefillArgs a = {};
     PrefillPlan p;
     int32_t rc;
-    if ((rc = prefill_check(cache, seqs, total_q, q_heads, max_ctx, &a.c, &p))) return rc;
+    if ((rc = prefill_check(cache, seqs, total_q, q_heads, max_ctx, &a.c))) return rc;
     const int D = cache->head_dim;
     if ((rc = paged_check_options(me, options, D, &a.o))) return rc;
     if (seqs == 0 || total_q == 0) return LTHN_OK;
@@ -839,6 +910,7 @@ int32_t lthn_paged_prefill_attention(void* stream, const lthn_paged_kv* cache, c
     LTHN_REQUIRE(((a.q_stride | a.out_stride) & 7) == 0, "paged_prefill_attention: strides must be multiples of 8 elements");
     LTHN_REQUIRE(a.out_stride >= (int64_t)q_heads * D, "paged_prefill_attention: rows of out would overlap");
     LTHN_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15) == 0, "paged_prefill_attention: q, out and workspace must be 16-byte aligned");
+    if ((rc = prefill_plan_for(cache, a.c, options, seqs, total_q, q_heads, max_ctx, &p))) return rc;
     LTHN_REQUIRE(workspace_bytes >= p.total, "paged_prefill_attention: workspace too small");
     if ((rc = paged_check_device(me, "the cache", cache->k))) return rc;
     if ((rc = paged_check_device(me, "q", q))) return rc;
