@@ -59,7 +59,7 @@ struct PrefillArgs {
     int tiles;           // upper bound of the row tiles of all sequences
     int chunks;          // CTAs per tile and kv head
     int chunk_tiles;     // key tiles per chunk
-    float* part;         // [tiles*kv_heads*chunks][rows][D] unnormalised outputs
+    float4* part;        // [tiles*kv_heads*chunks][D/4][rows] unnormalised outputs, four columns each
     float2* ml;          // [tiles*kv_heads*chunks][rows] maximum (log2 units) and sum
     int4* desc;          // [tiles] sequence, tile of the sequence, chunks in use
 };
@@ -78,16 +78,19 @@ __device__ __forceinline__ int2 prefill_span(const PrefillArgs& a, int s) {
 // see more keys, and the longest work goes first. Returns false past the first.
 template <int WARPS, int ROWS>
 __device__ __forceinline__ bool prefill_tile(const PrefillArgs& a, int* sh, int id, int& seq, int& tile) {
-    int all = 0, incl;
     auto count = [&](int s0) {
         const int s = s0 + threadIdx.x;
         return s < a.seqs ? (prefill_span(a, s).y * a.G + ROWS - 1) / ROWS : 0;
     };
-    for (int s0 = 0; s0 < a.seqs; s0 += WARPS * 32) all += paged_block_scan<WARPS>(count(s0), incl, sh);
+    int incl, n = count(0);
+    int total = paged_block_scan<WARPS>(n, incl, sh), all = total;
+    for (int s0 = WARPS * 32; s0 < a.seqs; s0 += WARPS * 32) {
+        int x;
+        all += paged_block_scan<WARPS>(count(s0), x, sh);
+    }
     if (id >= all) return false;
     int want = all - 1 - id;
-    for (int s0 = 0; s0 < a.seqs; s0 += WARPS * 32) {
-        const int n = count(s0), total = paged_block_scan<WARPS>(n, incl, sh);
+    for (int s0 = 0;;) {
         if (want < total) {
             if (incl > want && incl - n <= want) { sh[WARPS] = s0 + threadIdx.x; sh[WARPS + 1] = want - (incl - n); }
             __syncthreads();
@@ -96,8 +99,10 @@ __device__ __forceinline__ bool prefill_tile(const PrefillArgs& a, int* sh, int 
             return true;
         }
         want -= total;
+        s0 += WARPS * 32;
+        n = count(s0);
+        total = paged_block_scan<WARPS>(n, incl, sh);
     }
-    return false;
 }
 
 // ---- tcgen05 wrappers (cta_group::1) ---------------------------------------------------------------
@@ -322,16 +327,20 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int wg = warp >> 2, qt = two ? wg : 0;         // score buffer = warpgroup; row tile
         const int wr = (warp & 3) * 32, r = wr + lane;       // row within the row tile = tensor memory lane
-        {   // queries into shared memory: the warps of a row tile take 32 rows each, D/8 lanes a row
-            constexpr int CPR = D / 8;
-            unsigned char* qs = pf_smem + qt * C::Q_BYTES;
-#pragma unroll 4
-            for (int x = two ? lane : lane + 32 * wg; x < 32 * CPR; x += two ? 32 : 64) {
-                const int rr = wr + x / CPR, c = x % CPR, row = row0 + qt * 128 + rr;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (row < nrows) v = *(const uint4*)(a.q + (span.x + row / a.G) * a.q_stride + (int64_t)(kvh * a.G + row % a.G) * D + c * 8);
-                *(uint4*)(qs + (c >> 3) * (128 * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
+        {   // queries into shared memory: each warp of a row tile takes 32 rows, lane i knows where row i lies
+            constexpr int CPR = D / 8, RPI = 32 / CPR;       // 16-byte chunks per row, rows per instruction
+            const int mine = row0 + qt * 128 + r, tk = mine / a.G;
+            const int64_t at = mine < nrows ? (span.x + tk) * a.q_stride + (int64_t)(kvh * a.G + mine - tk * a.G) * D : -1;
+            const uint32_t qs = smem + qt * C::Q_BYTES;
+            const int c = lane % CPR, half = two ? 0 : wg * 16, count = two ? 32 : 16;   // one row tile: the warpgroups share its rows
+#pragma unroll 8
+            for (int i = 0; i < count; i += RPI) {
+                const int x = half + i + lane / CPR, rr = wr + x;
+                const int64_t o = __shfl_sync(0xffffffffu, at, x);
+                cp_async16_zfill(qs + (c >> 3) * (128 * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), a.q + (o < 0 ? 0 : o) + c * 8, o < 0 ? 0 : 16);
             }
+            paged_cp_commit();
+            paged_cp_wait<0>();
             pf_fence_async();
             pf_arrive(q_full);
             __syncwarp();
@@ -474,7 +483,8 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             const float m2 = m * c1;                         // log2 units (c1 > 0)
             const float inv = l > 0.f ? 1.0f / l : 0.f;
             uint16_t* dst = a.out + tok * a.out_stride + (int64_t)head * D;
-            const int64_t at = (((int64_t)id * a.c.kv_heads + kvh) * a.chunks + chunk) * ROWS + qt * 128 + r;
+            const int64_t cta = ((int64_t)id * a.c.kv_heads + kvh) * a.chunks + chunk;
+            float4* part = a.part + cta * (D / 4) * ROWS + qt * 128 + r;
 #pragma unroll 1
             for (int x = x0; x < x1; x += 32) {
                 float o[32];
@@ -494,11 +504,11 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                                                             pack_bf16x2(o[e + 4] * inv, o[e + 5] * inv), pack_bf16x2(o[e + 6] * inv, o[e + 7] * inv));
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) *(float4*)(a.part + at * D + x + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    for (int e = 0; e < 32; e += 4) part[(x + e) / 4 * ROWS] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                 }
             }
             if (live && x0 == 0) {
-                if (used > 1) a.ml[at] = make_float2(m2, l);
+                if (used > 1) a.ml[cta * ROWS + qt * 128 + r] = make_float2(m2, l);
                 else if (a.lse) a.lse[tok * a.Hq + head] = (m2 + log2f(l)) * 0.6931471805599453f;
             }
         }
@@ -715,46 +725,37 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
     if (warp == C::SM_WARPS) pf_tmem_dealloc(tmem, 512);
 }
 
-// Joins the chunks of a tile: one warp per row.
+// Joins the chunks of a tile: a lane is a row, a thread 8 columns of it.
 template <int D>
 __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const PrefillArgs a) {
     pdl_wait();
-    constexpr int ROWS = PfCfg<D>::ROWS, DL = D / 64;
-    const int lane = threadIdx.x & 31, r = blockIdx.z * 8 + (threadIdx.x >> 5), kvh = blockIdx.y, id = blockIdx.x;
+    constexpr int ROWS = PfCfg<D>::ROWS, GROUPS = D / 8;
+    const int item = blockIdx.z * 256 + threadIdx.x, r = item % ROWS, col = item / ROWS, kvh = blockIdx.y, id = blockIdx.x;
     const int4 ds = a.desc[id];
     if (ds.z <= 1) return;
     const int2 span = prefill_span(a, ds.x);
     const int row = ds.y * ROWS + r;
-    if (row >= span.y * a.G) return;
-    const int64_t at = ((int64_t)id * a.c.kv_heads + kvh) * a.chunks * ROWS + r;
-    float m = -INFINITY;
-    for (int z = lane; z < ds.z; z += 32) m = fmaxf(m, a.ml[at + (int64_t)z * ROWS].x);
-    m = warp_max(m);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    float2 acc[DL];
-#pragma unroll
-    for (int i = 0; i < DL; i++) acc[i] = make_float2(0.f, 0.f);
+    if (row >= span.y * a.G || col >= GROUPS) return;
+    const int64_t cta = ((int64_t)id * a.c.kv_heads + kvh) * a.chunks;
+    float m = -INFINITY, l = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int z = 0; z < ds.z; z++) {
-        const float2 ml = a.ml[at + (int64_t)z * ROWS];
-        const float e = ex2(ml.x - ref);
-        l = fmaf(ml.y, e, l);
-        const float2* src = (const float2*)(a.part + (at + (int64_t)z * ROWS) * D);
-#pragma unroll
-        for (int i = 0; i < DL; i++) {
-            const float2 v = src[lane + 32 * i];
-            acc[i].x = fmaf(v.x, e, acc[i].x);
-            acc[i].y = fmaf(v.y, e, acc[i].y);
-        }
+        const float2 ml = a.ml[(cta + z) * ROWS + r];
+        const float4* src = a.part + ((cta + z) * (D / 4) + 2 * col) * ROWS + r;
+        const float4 p = src[0], q = src[ROWS];
+        const float nm = fmaxf(m, ml.x), ref = nm == -INFINITY ? 0.f : nm;
+        const float e0 = ex2(m - ref), e1 = ex2(ml.x - ref);     // -inf -> 0
+        m = nm;
+        l = l * e0 + ml.y * e1;
+        x[0] = x[0] * e0 + p.x * e1; x[1] = x[1] * e0 + p.y * e1; x[2] = x[2] * e0 + p.z * e1; x[3] = x[3] * e0 + p.w * e1;
+        x[4] = x[4] * e0 + q.x * e1; x[5] = x[5] * e0 + q.y * e1; x[6] = x[6] * e0 + q.z * e1; x[7] = x[7] * e0 + q.w * e1;
     }
     const float inv = l > 0.f ? 1.0f / l : 0.f;
     const int64_t tok = span.x + row / a.G;
     const int head = kvh * a.G + row % a.G;
-    uint32_t* dst = (uint32_t*)(a.out + tok * a.out_stride + (int64_t)head * D);
-#pragma unroll
-    for (int i = 0; i < DL; i++) dst[lane + 32 * i] = pack_bf16x2(acc[i].x * inv, acc[i].y * inv);
-    if (a.lse && lane == 0) a.lse[tok * a.Hq + head] = (m + log2f(l)) * 0.6931471805599453f;
+    *(uint4*)(a.out + tok * a.out_stride + (int64_t)head * D + col * 8) =
+        make_uint4(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv), pack_bf16x2(x[4] * inv, x[5] * inv), pack_bf16x2(x[6] * inv, x[7] * inv));
+    if (a.lse && col == 0) a.lse[tok * a.Hq + head] = (m + log2f(l)) * 0.6931471805599453f;
 }
 
 struct PrefillPlan { int tiles, chunks, chunk_tiles; size_t part, ml, desc, total; };
@@ -839,7 +840,7 @@ static int32_t launch_prefill(cudaStream_t s, PrefillArgs a) {
     LTHN_CUDA_TRY(cudaGetLastError());
     if (a.chunks > 1) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(a.tiles, a.c.kv_heads, C::ROWS / 8); cfg.blockDim = dim3(256); cfg.stream = s;
+        cfg.gridDim = dim3(a.tiles, a.c.kv_heads, C::ROWS * (D / 8) / 256); cfg.blockDim = dim3(256); cfg.stream = s;
         cudaLaunchAttribute at[1];
         at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -917,7 +918,7 @@ int32_t lthn_paged_prefill_attention(void* stream, const lthn_paged_kv* cache, c
     a.q = q; a.out = out; a.q_start = q_start; a.lens = kv_lens; a.lse = lse;
     a.seqs = seqs; a.total_q = total_q; a.Hq = q_heads; a.G = q_heads / cache->kv_heads;
     a.tiles = p.tiles; a.chunks = p.chunks; a.chunk_tiles = p.chunk_tiles;
-    a.part = (float*)workspace;
+    a.part = (float4*)workspace;
     a.ml = (float2*)((char*)workspace + p.part);
     a.desc = (int4*)((char*)workspace + p.part + p.ml);
     a.wait_status = device_status_word();
