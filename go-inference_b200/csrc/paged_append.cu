@@ -56,7 +56,7 @@ int32_t paged_check_cache(const char* name, const lthn_paged_kv* c, PagedCache* 
     LTHN_REQUIRE(((o.row_stride | o.head_stride | o.page_stride) & 7) == 0, named(name, "cache strides must be multiples of 8 elements"));
     LTHN_REQUIRE((((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0, named(name, "k and v must be 16-byte aligned"));
     o.pages = c->pages; o.page_size = c->page_size; o.table_stride = c->table_stride; o.seqs = c->seqs; o.kv_heads = c->kv_heads;
-    o.capacity = (int)std::min<int64_t>((int64_t)c->table_stride * c->page_size, 0x7fffff00);
+    o.capacity = (int)std::min<int64_t>((int64_t)c->table_stride * c->page_size, 1 << 26);
     o.status = nullptr;
     *out = o;
     return LTHN_OK;

@@ -5,9 +5,9 @@
 // 4*D flops per visible (query, key) pair against 4*D bytes of K and V per key and tile of query rows: bound by the tensor pipe
 // for prompts, by HBM for a few rows against a long context.
 //
-// Rows. The query rows of a tile are the (token, query head) pairs of one kv head, token by token, so the heads that share
-// K and V share their loads and a chunk of a few tokens still fills a tile. A CTA works on one or two tiles of 128 rows
-// (two: two accumulators of head_dim columns fit the tensor memory beside two score tiles for head_dim 64 and 128) and on
+// Rows. The query rows of a tile are the (token, query head) pairs of one kv head, token by token, as many whole tokens as 128
+// rows hold, so the heads that share K and V share their loads, a chunk of a few tokens still fills a tile, and the
+// queries of a tile are one TMA box per 64 head dimensions. A CTA works on one or two tiles of 128 rows (two: two accumulators of head_dim columns fit the tensor memory beside two score tiles for head_dim 64 and 128) and on
 // BN keys at a time.
 //
 //   softmax warps   two warpgroups, one per score buffer, one thread per row: tcgen05.ld the row's BN scores, mask, maximum, ex2,
@@ -18,7 +18,7 @@
 //                   works on one buffer while the other's softmax runs. With two row tiles the buffers belong to them;
 //                   with one they alternate over its key tiles, and the warpgroups pass the running maximum of a row to one
 //                   another (the sums stay apart until the end), which leaves only load and maximum in sequence.
-//   loaders         three warps fill a ring of K and V tiles in the 128-byte swizzle. Where the page size is a multiple of 8 (the
+//   loaders         three warps fetch the queries of a segment and fill a ring of K and V tiles in the 128-byte swizzle. Where the page size is a multiple of 8 (the
 //                   swizzle's row group) by tiled TMA, one box per page, 64 head dimensions and gcd(page size, BN) rows. V rows
 //                   that nobody sees must be zeros (they may hold NaN, which a weight of zero would not silence), so a V
 //                   tile with such rows - the last of a sequence, the first of a window - and pools of other page
@@ -29,8 +29,13 @@
 // their bf16 rounding (relative) nor the f32 sums mind, and O in tensor memory needs no correction. A move multiplies
 // O by 2^(old - new) through registers; after the first tiles it is rare.
 //
-// Cutting. Where there are fewer tiles than SMs the keys of a tile are cut into chunks, one CTA each, that leave
-// (maximum, sum, unnormalised output) in the workspace for a second kernel to join.
+// Work. The key tiles of all (row tile, kv head) pairs form one list, weighted by what they cost; CTA c of C (one per SM) takes the
+// c-th C-th of it, whatever the lengths are, and walks through its segments without stopping: the loaders are at the next
+// segment's queries and keys while the softmax warps finish the last one. A pair that lies within one CTA is finished there; otherwise each
+// CTA that holds part of it leaves (maximum, sum, unnormalised output) in its slot of the workspace - at most two such
+// parts, its first and its last segment - and a second kernel joins them. (One CTA per tile, longest first, spent 7 us of
+// each CTA on its start and end; cut into equal chunks, the few rows of drafts against long contexts of different lengths took
+// two waves where the work was one.)
 //
 // Every wait is bounded: on a time-out the roles record it in the device status word, drain what they have in flight, free
 // the tensor memory and return.
@@ -56,12 +61,11 @@ struct PrefillArgs {
     float* lse;
     uint32_t* wait_status;
     int seqs, total_q, Hq, G;
-    int tiles;           // upper bound of the row tiles of all sequences
-    int chunks;          // CTAs per tile and kv head
-    int chunk_tiles;     // key tiles per chunk
-    float4* part;        // [tiles*kv_heads*chunks][D/4][rows] unnormalised outputs, four columns each
-    float2* ml;          // [tiles*kv_heads*chunks][rows] maximum (log2 units) and sum
-    int4* desc;          // [tiles] sequence, tile of the sequence, chunks in use
+    int tokens;          // of a row tile: 128 / G
+    int q_box;           // queries by TMA (their row stride is a multiple of head_dim), else copied row by row
+    float4* part;        // [2*CTAs][D/4][rows] unnormalised outputs, four columns each
+    float2* ml;          // [2*CTAs][rows] maximum (log2 units) and sum
+    int4* desc;          // [CTAs] the pair that begins in the CTA and ends in another: sequence, tile, head, last CTA (-1: none)
 };
 
 // The rows of sequence s, made safe: within [0, total_q).
@@ -74,36 +78,80 @@ __device__ __forceinline__ int2 prefill_span(const PrefillArgs& a, int s) {
     return make_int2(b, e - b);
 }
 
-// Tile `id` of the tiles (ROWS rows of token * G + head) of all sequences, counted from the last one: the later tiles of a prompt
-// see more keys, and the longest work goes first. Returns false past the first.
-template <int WARPS, int ROWS>
-__device__ __forceinline__ bool prefill_tile(const PrefillArgs& a, int* sh, int id, int& seq, int& tile) {
-    auto count = [&](int s0) {
-        const int s = s0 + threadIdx.x;
-        return s < a.seqs ? (prefill_span(a, s).y * a.G + ROWS - 1) / ROWS : 0;
-    };
-    int incl, n = count(0);
-    int total = paged_block_scan<WARPS>(n, incl, sh), all = total;
-    for (int s0 = WARPS * 32; s0 < a.seqs; s0 += WARPS * 32) {
-        int x;
-        all += paged_block_scan<WARPS>(count(s0), x, sh);
-    }
-    if (id >= all) return false;
-    int want = all - 1 - id;
-    for (int s0 = 0;;) {
-        if (want < total) {
-            if (incl > want && incl - n <= want) { sh[WARPS] = s0 + threadIdx.x; sh[WARPS + 1] = want - (incl - n); }
-            __syncthreads();
-            seq = sh[WARPS];
-            tile = sh[WARPS + 1];
-            return true;
-        }
-        want -= total;
-        s0 += WARPS * 32;
-        n = count(s0);
-        total = paged_block_scan<WARPS>(n, incl, sh);
-    }
+// The tokens of one or two row tiles of a sequence.
+struct PfTile {
+    int2 span;           // the sequence's rows of q: first, count
+    int len, pos0;       // keys; position of the first query
+    int prefix;
+    int tok0;            // first token of the tile
+    int qlo, qhi;        // positions of its first and last token
+    KeyTiles kt;
+    bool two;            // both row tiles have tokens
+};
+template <int NQ, int BN>
+__device__ __forceinline__ PfTile prefill_tile(const PrefillArgs& a, int seq, int tile) {
+    PfTile t;
+    t.span = prefill_span(a, seq);
+    t.len = paged_length(a.c, a.lens[seq]);
+    t.pos0 = t.len - t.span.y;
+    t.prefix = a.o.prefix ? min(max(a.o.prefix[seq], 0), t.len) : 0;
+    t.tok0 = tile * NQ * a.tokens;
+    t.qlo = t.pos0 + t.tok0;
+    t.qhi = t.pos0 + min(t.tok0 + NQ * a.tokens, t.span.y) - 1;
+    t.kt = key_tiles<BN>(t.qlo, t.qhi, t.len, t.prefix, a.o.window);
+    t.two = NQ == 2 && t.span.y - t.tok0 > a.tokens;
+    return t;
 }
+// What a (tile, head) pair costs: about 0.6 us per unit. A key tile of two row tiles keeps the tensor pipe busier than one of one; the start covers
+// the first scores, the last output and its way to memory.
+constexpr int PF_ONE = 2, PF_TWO = 3, PF_START = 5;
+constexpr int PF_LEAST = 8;   // units of a CTA below which fewer CTAs are used: every part holds a key tile
+static_assert(PF_LEAST >= 2 * PF_TWO, "a range within a pair holds a whole key tile");
+__device__ __forceinline__ int pf_key_cost(const PfTile& t) { return t.two ? PF_TWO : PF_ONE; }
+__device__ __forceinline__ int pf_cost(const PfTile& t) { return PF_START + t.kt.n * pf_key_cost(t); }
+// the key tiles that lie before unit v of a pair
+__device__ __forceinline__ int pf_tiles_before(const PfTile& t, int v) { return v <= PF_START ? 0 : (v - PF_START) / pf_key_cost(t); }
+
+// The walk of a CTA through its segments; every role makes its own.
+template <int NQ, int BN>
+struct PfWalk {
+    PfTile t;
+    int seq, tile, head, v, cost;
+    int64_t u, u1;
+    int i0, n, take;     // segment: key tiles [i0, i0 + n) of the pair
+    __device__ __forceinline__ void start(const PrefillArgs& a, int seq_, int tile_, int64_t base, int64_t u0, int64_t end) {
+        seq = seq_; tile = tile_; u = u0; u1 = end;
+        t = prefill_tile<NQ, BN>(a, seq, tile);
+        cost = pf_cost(t);
+        head = (int)((u0 - base) / cost);
+        v = (int)((u0 - base) - (int64_t)head * cost);
+    }
+    __device__ __forceinline__ bool more() const { return u < u1; }
+    // false: nothing to do in this one
+    __device__ __forceinline__ bool segment() {
+        take = (int)min((int64_t)(cost - v), u1 - u);
+        i0 = pf_tiles_before(t, v);
+        n = pf_tiles_before(t, v + take) - i0;
+        return n > 0 || (t.kt.n == 0 && v == 0);
+    }
+    __device__ __forceinline__ bool whole() const { return n == t.kt.n; }
+    __device__ __forceinline__ void next(const PrefillArgs& a) {
+        u += take;
+        v += take;
+        if (v < cost || u >= u1) return;
+        v = 0;
+        if (++head < a.c.kv_heads) return;
+        head = 0;
+        tile++;
+        if (tile * NQ * (int64_t)a.tokens >= t.span.y) {
+            tile = 0;
+            do seq++; while (seq < a.seqs && prefill_span(a, seq).y == 0);
+            if (seq >= a.seqs) { u = u1; return; }       // only if the lengths changed under the call
+        }
+        t = prefill_tile<NQ, BN>(a, seq, tile);
+        cost = pf_cost(t);
+    }
+};
 
 // ---- tcgen05 wrappers (cta_group::1) ---------------------------------------------------------------
 __device__ __forceinline__ void pf_tmem_alloc(uint32_t* smem_dst, uint32_t ncols) {
@@ -131,6 +179,10 @@ __device__ __forceinline__ void pf_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
 __device__ __forceinline__ void pf_commit(uint64_t* bar) {
     asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
                  "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void pf_tma_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ void pf_tma_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
@@ -247,9 +299,8 @@ struct PfCfg {
     static constexpr int RING = NQ * Q_BYTES;                // offsets in shared memory
     static constexpr int OFFS = RING + ST * KV_BYTES;        // [2][BN] row offsets
     static constexpr int BARS = OFFS + 2 * BN * 8;
-    // one row tile: the rows' running maximum, in the place of the second row tile where there is room for one
-    static constexpr int ROW_MAX = NQ == 2 ? Q_BYTES : BARS + 512;
-    static constexpr int TOTAL = BARS + 512 + (NQ == 2 ? 0 : 512);
+    static constexpr int ROW_MAX = BARS + 512;               // one row tile: the rows' running maximum
+    static constexpr int TOTAL = ROW_MAX + 512;
     static constexpr int S_COLS = BN;                        // tensor memory: two score buffers, then the outputs at column 256
     static constexpr int LAG = 2;                            // ring slots in flight behind the one being filled
     static_assert(LAG <= ST - 3, "a slot is handed over before the one that frees its successor is waited for");
@@ -258,7 +309,8 @@ struct PfCfg {
 
 // FEAT bit 0: tanh cap, bit 1: distance bias
 template <int D, int FEAT>
-__global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const PrefillArgs a) {
+__global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                                                                       const __grid_constant__ CUtensorMap v_map, const PrefillArgs a) {
     using C = PfCfg<D>;
     constexpr int BN = C::BN, ST = C::ST, ROWS = C::ROWS;
     constexpr float LOG2E = 1.4426950408889634f;
@@ -271,42 +323,83 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
     uint64_t* o_last = o_done + 2;                           // [2] the last has (a barrier of its own: with one row tile the softmax
                                                              //     may be two units ahead, which a parity cannot tell from none)
     uint64_t* turn = o_last + 2;                             // [4] one row tile: the maximum of key tile j is out, per 32 rows
-    uint64_t* q_full = turn + 4;
-    uint64_t* drain = q_full + 1;
+    uint64_t* q_full = turn + 4;                             // queries of a segment
+    uint64_t* q_empty = q_full + 1;                          // its last scores are done
+    uint64_t* meet = q_empty + 1;                            // both softmax warpgroups (a barrier whose wait is bounded)
+    uint64_t* drain = meet + 1;
     uint32_t* tmem_slot = (uint32_t*)(drain + 1);
-    int* scan = (int*)(tmem_slot + 2);                       // WARPS + 2 words
+    int* scan = (int*)(tmem_slot + 2);                       // WARPS words, then sequence, tile and (64 bits) first unit of the first tile
+    static_assert((2 * ST + 20) * 8 + (C::WARPS + 4) * 4 <= 512, "barriers and scan words");
 
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-    const int kvh = blockIdx.x % a.c.kv_heads;
-    const int chunk = blockIdx.x / a.c.kv_heads % a.chunks;
-    const int id = blockIdx.x / a.c.kv_heads / a.chunks;
-    int seq, tile;
-    if (!prefill_tile<C::WARPS, ROWS>(a, scan, id, seq, tile)) {
-        if (a.chunks > 1 && chunk == 0 && kvh == 0 && tid == 0) a.desc[id] = make_int4(0, 0, 0, 0);
+
+    // ---- this CTA's part of the work ------------------------------------------------------------------
+    int* first = (int*)(pf_smem + C::RING);                  // first tile of each sequence
+    int T = 0;
+    for (int s0 = 0; s0 < a.seqs; s0 += C::THREADS) {
+        const int s = s0 + tid;
+        const int c = s < a.seqs ? (prefill_span(a, s).y + C::NQ * a.tokens - 1) / (C::NQ * a.tokens) : 0;
+        int incl;
+        const int total = paged_block_scan<C::WARPS>(c, incl, scan);
+        if (s < a.seqs) first[s] = T + incl - c;
+        T += total;
+    }
+    __syncthreads();
+    auto find = [&](int t) {                                 // the last sequence that begins at or before tile t (empty ones begin with the next)
+        int lo = 0, hi = a.seqs - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (first[mid] <= t) lo = mid;
+            else hi = mid - 1;
+        }
+        return lo;
+    };
+    auto cost_of = [&](int t) {
+        if (t >= T) return 0;
+        const int s = find(t);
+        return pf_cost(prefill_tile<C::NQ, BN>(a, s, t - first[s]));
+    };
+    int incl, mine = cost_of(tid);
+    int part = paged_block_scan<C::WARPS>(mine, incl, scan);
+    int64_t U = part;
+    for (int t0 = C::THREADS; t0 < T; t0 += C::THREADS) {
+        int x;
+        U += paged_block_scan<C::WARPS>(cost_of(t0 + tid), x, scan);
+    }
+    U *= a.c.kv_heads;
+    const int ctas = (int)max((int64_t)1, min((int64_t)gridDim.x, U / PF_LEAST));
+    if (T == 0 || (int)blockIdx.x >= ctas) {
+        if (tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, -1);
         return;
     }
-    const int2 span = prefill_span(a, seq);
-    const int len = paged_length(a.c, a.lens[seq]);
-    const int nrows = span.y * a.G, row0 = tile * ROWS;
-    const int pos0 = len - span.y;                           // position of the sequence's first query
-    const int prefix = a.o.prefix ? min(max(a.o.prefix[seq], 0), len) : 0;
-    const int qlo = pos0 + row0 / a.G, qhi = pos0 + (min(row0 + ROWS, nrows) - 1) / a.G;
-    const KeyTiles kt = key_tiles<BN>(qlo, qhi, len, prefix, a.o.window);
-    const int per = max(a.chunk_tiles, (kt.n + a.chunks - 1) / a.chunks);  // key tiles of a chunk, also where max_ctx was too small
-    const int used = a.chunks > 1 ? max(1, (kt.n + per - 1) / per) : 1;
-    if (a.chunks > 1 && chunk == 0 && kvh == 0 && tid == 0) a.desc[id] = make_int4(seq, tile, used, 0);
-    if (chunk >= used) return;
-    const int i0 = chunk * per;
-    const int n = a.chunks > 1 ? min(per, kt.n - i0) : kt.n;   // key tiles of this CTA (0 only where nothing is visible)
-    const bool two = C::NQ == 2 && nrows - row0 > 128;
-    const int units = two ? 2 * n : n;
+    const int64_t u0 = U * blockIdx.x / ctas, u1 = U * (blockIdx.x + 1) / ctas;
+    int64_t* first_unit = (int64_t*)(scan + C::WARPS + 2);
+    int64_t base = 0;
+    for (int t0 = 0;;) {
+        if ((base + part) * a.c.kv_heads > u0) {
+            const int64_t b = (base + incl - mine) * a.c.kv_heads;
+            if (mine > 0 && b <= u0 && b + (int64_t)mine * a.c.kv_heads > u0) {
+                const int s = find(t0 + tid);
+                scan[C::WARPS] = s;
+                scan[C::WARPS + 1] = t0 + tid - first[s];
+                *first_unit = b;
+            }
+            break;
+        }
+        base += part;
+        t0 += C::THREADS;
+        mine = cost_of(t0 + tid);
+        part = paged_block_scan<C::WARPS>(mine, incl, scan);
+    }
 
     if (tid == 0) {
         for (int s = 0; s < ST; s++) { mbar_init(&full[s], 96); mbar_init(&empty[s], 1); }
         for (int b = 0; b < 2; b++) { mbar_init(&s_full[b], 1); mbar_init(&p_full[b], 128); mbar_init(&o_done[b], 1); mbar_init(&o_last[b], 1); }
         for (int w = 0; w < 4; w++) mbar_init(&turn[w], 1);
-        mbar_init(q_full, C::SM_WARPS * 32);
+        mbar_init(q_full, 96);
+        mbar_init(q_empty, 1);
+        mbar_init(meet, C::SM_WARPS * 32);
         mbar_init(drain, 1);
         mbar_fence_init();
     }
@@ -316,60 +409,58 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
     pf_fence_after();
     const uint32_t tmem = *tmem_slot;
     const uint32_t smem = smem_u32(pf_smem);
+    PfWalk<C::NQ, BN> wk;
+    wk.start(a, scan[C::WARPS], scan[C::WARPS + 1], *first_unit, u0, u1);
+    const PfTile& t = wk.t;
     bool ok = true;
 
-    // ring slots of the K and V tile of key tile j, in the order of their last use
-    auto k_slot = [&](int j) { return two ? 2 * j : j < 2 ? j : 2 * j - 1; };
-    auto v_slot = [&](int j) { return two ? 2 * j + 1 : j == n - 1 ? 2 * n - 1 : 2 * j + 2; };
+    // ring slots of the K and V tile of key tile j of a segment, in the order of their last use
+    auto k_slot = [&](int j) { return t.two ? 2 * j : j < 2 ? j : 2 * j - 1; };
+    auto v_slot = [&](int j) { return t.two ? 2 * j + 1 : j == wk.n - 1 ? 2 * wk.n - 1 : 2 * j + 2; };
 
     if (warp < C::SM_WARPS) {
         // ================================ softmax ================================
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        const int wg = warp >> 2, qt = two ? wg : 0;         // score buffer = warpgroup; row tile
+        const int wg = warp >> 2;                            // score buffer = warpgroup
         const int wr = (warp & 3) * 32, r = wr + lane;       // row within the row tile = tensor memory lane
-        {   // queries into shared memory: each warp of a row tile takes 32 rows, lane i knows where row i lies
-            constexpr int CPR = D / 8, RPI = 32 / CPR;       // 16-byte chunks per row, rows per instruction
-            const int mine = row0 + qt * 128 + r, tk = mine / a.G;
-            const int64_t at = mine < nrows ? (span.x + tk) * a.q_stride + (int64_t)(kvh * a.G + mine - tk * a.G) * D : -1;
-            const uint32_t qs = smem + qt * C::Q_BYTES;
-            const int c = lane % CPR, half = two ? 0 : wg * 16, count = two ? 32 : 16;   // one row tile: the warpgroups share its rows
-#pragma unroll 8
-            for (int i = 0; i < count; i += RPI) {
-                const int x = half + i + lane / CPR, rr = wr + x;
-                const int64_t o = __shfl_sync(0xffffffffu, at, x);
-                cp_async16_zfill(qs + (c >> 3) * (128 * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), a.q + (o < 0 ? 0 : o) + c * 8, o < 0 ? 0 : 16);
-            }
-            paged_cp_commit();
-            paged_cp_wait<0>();
-            pf_fence_async();
-            pf_arrive(q_full);
-            __syncwarp();
-        }
-        const int row = row0 + qt * 128 + r;
-        const bool live = row < nrows;
-        const int token = row / a.G, head = kvh * a.G + row - token * a.G;
-        const int qpos = pos0 + token;
-        // visible: key < pre, or klo <= key < khi
-        const int pre = prefix, khi = min(qpos + 1, len), klo = a.o.window > 0 ? qpos - a.o.window + 1 : 0;
+        const int r_token = r / a.G, r_head = r - r_token * a.G;
+        const uint32_t lanes = tmem + ((uint32_t)wr << 16);
+        const uint32_t s_addr = lanes + wg * C::S_COLS;
         // plain scores stay as the product left them, the others are brought to log2 units first
         const float c1 = FEAT ? 1.0f : a.o.scale * LOG2E;
         const float cap2 = a.o.softcap * LOG2E, cin = FEAT & 1 ? 2.0f * LOG2E * a.o.scale / a.o.softcap : a.o.scale * LOG2E;
-        const float slope = (FEAT & 2) && live ? a.o.slopes[head] * LOG2E : 0.f;
-        const uint32_t lanes = tmem + ((uint32_t)wr << 16);
-        const uint32_t s_addr = lanes + wg * C::S_COLS, o_addr = lanes + 256 + qt * D;
         float* row_max = (float*)(pf_smem + C::ROW_MAX);     // one row tile only
+        int uses = 0;                                        // of this warpgroup's score buffer
+        int turns = 0, done0 = 0, done1 = 0, last0 = 0, last1 = 0, meets = 0;  // phases the barriers have gone through
+        auto pair_sync = [&] {
+            pf_arrive(meet);
+            const bool met = __all_sync(0xffffffffu, pf_wait(meet, meets++ & 1));
+            ok = ok && met;
+        };
+        for (; wk.more() && ok; wk.next(a)) {
+        if (!wk.segment()) continue;
+        const bool two = t.two;
+        const int n = wk.n, i0 = wk.i0, qt = two ? wg : 0, len = t.len;
+        const int token = t.tok0 + qt * a.tokens + r_token;  // of the sequence
+        const bool live = r_token < a.tokens && token < t.span.y;
+        const int head = wk.head * a.G + r_head;
+        const int qpos = t.pos0 + token;
+        // visible: key < pre, or klo <= key < khi
+        const int pre = t.prefix, khi = min(qpos + 1, len), klo = a.o.window > 0 ? qpos - a.o.window + 1 : 0;
+        const float slope = (FEAT & 2) && live ? a.o.slopes[head] * LOG2E : 0.f;
+        const uint32_t o_addr = lanes + 256 + qt * D;
         float m = -INFINITY, l = 0.f;                        // reference maximum (units of the scores), sum relative to it
 
         for (int j = two ? 0 : wg; j < n; j += two ? 1 : 2) {
-            const int use = two ? j : j >> 1;                // of this warpgroup's buffer
-            ok = __all_sync(0xffffffffu, pf_wait(&s_full[wg], use & 1));
+            ok = __all_sync(0xffffffffu, pf_wait(&s_full[wg], uses & 1));
             if (!ok) break;
+            uses++;
             pf_fence_after();
             float s[BN];
 #pragma unroll
             for (int x = 0; x < BN; x += 32) pf_ld32(s_addr + x, s + x);
             pf_ld_wait();
-            const int k0 = kt.tile(i0 + j) * BN;
+            const int k0 = t.kt.tile(i0 + j) * BN;
             if (FEAT & 1) {
                 // cap tanh(x scale / cap) = cap (1 - 2 / (1 + e^(2 x scale / cap)))
 #pragma unroll
@@ -401,7 +492,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             mx[0] = max3(mx[0], s[BN - 4], s[BN - 3]);
             mx[1] = max3(mx[1], s[BN - 2], s[BN - 1]);
             if (!two && j > 0) {                             // the row's maximum so far, from the other warpgroup
-                ok = __all_sync(0xffffffffu, pf_wait(&turn[warp & 3], (j - 1) & 1));
+                ok = __all_sync(0xffffffffu, pf_wait(&turn[warp & 3], (turns + j - 1) & 1));
                 if (!ok) break;
                 const float mo = row_max[r];
                 if (mo != m) {                               // it has moved: this warpgroup's sum follows
@@ -410,7 +501,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                 }
                 __syncwarp();
             }
-            const float mnew = max3(fmaxf(m, mx[0]), mx[1], fmaxf(mx[2], mx[3]));
+            const float mnew = live ? max3(fmaxf(m, mx[0]), mx[1], fmaxf(mx[2], mx[3])) : m;   // a row without a query holds anything
             const bool move = __any_sync(0xffffffffu, (mnew - m) * c1 > 8.0f);
             const float mold = m;
             if (move) {
@@ -425,7 +516,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             }
             if (move && j > 0) {
                 const float alpha = mold == -INFINITY ? 0.f : ex2((mold - mnew) * c1);
-                ok = __all_sync(0xffffffffu, pf_wait(&o_done[qt], (j - 1) & 1));
+                ok = __all_sync(0xffffffffu, pf_wait(&o_done[qt], ((qt ? done1 : done0) + j - 1) & 1));
                 if (!ok) break;
                 pf_fence_after();
 #pragma unroll
@@ -462,29 +553,38 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             unpack2(add2(sum[0], sum[1]), l0, l1);
             l += l0 + l1;
         }
-        if (ok && n > 0) ok = __all_sync(0xffffffffu, pf_wait(&o_last[qt], 0));
-        if (!ok && lane == 0) atomicOr(a.wait_status, 1u << 26);
+        if (ok && n > 0) ok = __all_sync(0xffffffffu, pf_wait(&o_last[qt], (qt ? last1 : last0) & 1));
         int x0 = 0, x1 = D;                                  // output columns of this warpgroup
-        if (!two) {
-            // the two sums of a row meet, over the ring that nothing uses any more; each warpgroup stores half of the columns
-            float2* sums = (float2*)(pf_smem + C::RING);
-            sums[wg * 128 + r] = make_float2(m, l);
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            const float2 other = sums[(wg ^ 1) * 128 + r];
-            const float mm = fmaxf(m, other.x);              // the later of the two is the maximum O is relative to
-            l = (m == -INFINITY ? 0.f : l * ex2((m - mm) * c1)) + (other.x == -INFINITY ? 0.f : other.y * ex2((other.x - mm) * c1));
-            m = mm;
+        if (!two && n > 0) {
+            // the two sums of a row meet, relative to the last maximum; each warpgroup stores half of the columns
+            if (ok) ok = __all_sync(0xffffffffu, pf_wait(&turn[warp & 3], (turns + n - 1) & 1));
+            const float mo = row_max[r];
+            l = m == -INFINITY ? 0.f : l * ex2((m - mo) * c1);
+            m = mo;
+            pair_sync();
+            if (wg == 1) row_max[r] = l;
+            pair_sync();
+            if (wg == 0) { l += row_max[r]; row_max[r] = l; }
+            pair_sync();
+            l = row_max[r];
             x0 = wg * (D / 2);
             x1 = x0 + D / 2;
+            turns += n;
+        }
+        if (n > 0) {
+            if (two) { done1 += n - 1; last1++; }
+            done0 += n - 1;
+            last0++;
         }
         if (ok) {
             pf_fence_after();
-            const int64_t tok = span.x + token;
+            const int64_t tok = t.span.x + token;
             const float m2 = m * c1;                         // log2 units (c1 > 0)
             const float inv = l > 0.f ? 1.0f / l : 0.f;
             uint16_t* dst = a.out + tok * a.out_stride + (int64_t)head * D;
-            const int64_t cta = ((int64_t)id * a.c.kv_heads + kvh) * a.chunks + chunk;
-            float4* part = a.part + cta * (D / 4) * ROWS + qt * 128 + r;
+            const bool whole = wk.whole();
+            const int slot = 2 * blockIdx.x + (i0 > 0 ? 0 : 1);
+            float4* part = a.part + (int64_t)slot * (D / 4) * ROWS + qt * 128 + r;
 #pragma unroll 1
             for (int x = x0; x < x1; x += 32) {
                 float o[32];
@@ -497,7 +597,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                     for (int e = 0; e < 32; e++) o[e] = 0.f;
                 }
                 if (!live) continue;
-                if (used == 1) {
+                if (whole) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8)
                         *(uint4*)(dst + x + e) = make_uint4(pack_bf16x2(o[e] * inv, o[e + 1] * inv), pack_bf16x2(o[e + 2] * inv, o[e + 3] * inv),
@@ -508,20 +608,32 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                 }
             }
             if (live && x0 == 0) {
-                if (used > 1) a.ml[cta * ROWS + qt * 128 + r] = make_float2(m2, l);
+                if (!whole) a.ml[slot * ROWS + qt * 128 + r] = make_float2(m2, l);
                 else if (a.lse) a.lse[tok * a.Hq + head] = (m2 + log2f(l)) * 0.6931471805599453f;
             }
         }
+        if (!two && n > 0) pair_sync();                      // both have read O before the next segment's first weights let it be replaced
+        }
+        if (!ok && lane == 0) atomicOr(a.wait_status, 1u << 26);
     } else if (warp == C::SM_WARPS) {
         // ================================ issuer ================================
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        if (n > 0) {
-            // f32 accumulators, bf16 operands, M = 128; S: N = BN, both K-major; O: N = D, B is N-major
-            const uint32_t base = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);
-            const uint32_t idesc_s = base | ((uint32_t)(BN >> 3) << 17), idesc_o = base | (1u << 16) | ((uint32_t)(D >> 3) << 17);
-            ok = __all_sync(0xffffffffu, pf_wait(q_full, 0));
+        // f32 accumulators, bf16 operands, M = 128; S: N = BN, both K-major; O: N = D, B is N-major
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);
+        const uint32_t idesc_s = idesc | ((uint32_t)(BN >> 3) << 17), idesc_o = idesc | (1u << 16) | ((uint32_t)(D >> 3) << 17);
+        int slot0 = 0, segments = 0;                         // ring slots and segments so far
+        uint32_t uses = 0;                                   // bit b: parity of the uses of score buffer b
+        int4 begun = make_int4(0, 0, 0, -1);
+        for (; wk.more() && ok; wk.next(a)) {
+            if (!wk.segment()) continue;
+            const bool two = t.two;
+            const int n = wk.n, units = two ? 2 * n : n;
+            if (wk.i0 == 0 && !wk.whole())
+                begun = make_int4(wk.seq, wk.tile, wk.head, (int)(((wk.u - wk.v + wk.cost) * ctas + U - 1) / U) - 1);
+            if (n == 0) continue;
+            ok = __all_sync(0xffffffffu, pf_wait(q_full, segments & 1));
             auto scores = [&](int u) {
-                const int j = two ? u >> 1 : u, qt = two ? u & 1 : 0, slot = k_slot(j), st = slot % ST;
+                const int j = two ? u >> 1 : u, qt = two ? u & 1 : 0, slot = slot0 + k_slot(j), st = slot % ST;
                 ok = __all_sync(0xffffffffu, pf_wait(&full[st], (slot / ST) & 1));
                 if (!ok) return;
                 pf_fence_after();
@@ -531,13 +643,15 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                     pf_mma_ss(d, pf_desc_k(qa + (x >> 2) * (128 * 128) + (x & 3) * 32), pf_desc_k(kb + (x >> 2) * C::SLAB + (x & 3) * 32), idesc_s, x > 0);
                 pf_commit(&s_full[u & 1]);
                 if (!two || qt == 1) pf_commit(&empty[st]);
+                if (u == units - 1) pf_commit(q_empty);
             };
             if (ok) scores(0);
             if (ok && units > 1) scores(1);
             for (int u = 0; u < units && ok; u++) {
-                const int j = two ? u >> 1 : u, qt = two ? u & 1 : 0, slot = v_slot(j), st = slot % ST;
-                ok = __all_sync(0xffffffffu, pf_wait(&full[st], (slot / ST) & 1) && pf_wait(&p_full[u & 1], (u >> 1) & 1));
+                const int j = two ? u >> 1 : u, qt = two ? u & 1 : 0, slot = slot0 + v_slot(j), st = slot % ST;
+                ok = __all_sync(0xffffffffu, pf_wait(&full[st], (slot / ST) & 1) && pf_wait(&p_full[u & 1], uses >> (u & 1) & 1));
                 if (!ok) break;
+                uses ^= 1u << (u & 1);
                 pf_fence_after();
                 const uint32_t vb = smem + C::RING + st * C::KV_BYTES, pa = tmem + (u & 1) * C::S_COLS, d = tmem + 256 + qt * D;
 #pragma unroll
@@ -546,12 +660,15 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                 pf_commit(j == n - 1 ? &o_last[qt] : &o_done[qt]);   // the last commit of all is one that is waited for
                 if (u + 2 < units) scores(u + 2);
             }
-            if (!ok) {
-                if (lane == 0) atomicOr(a.wait_status, 1u << 25);
-                pf_commit(drain);                            // nothing of this CTA may still run when its memory is given back
-                pf_wait(drain, 0);
-            }
+            slot0 += 2 * n;
+            segments++;
         }
+        if (!ok) {
+            if (lane == 0) atomicOr(a.wait_status, 1u << 25);
+            pf_commit(drain);                                // nothing of this CTA may still run when its memory is given back
+            pf_wait(drain, 0);
+        }
+        if (lane == 0) a.desc[blockIdx.x] = begun;
         __syncwarp();
     } else {
         // ================================ loaders ================================
@@ -560,13 +677,19 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         constexpr int NX = (BN / 4 + 2) / 3 * 4;             // rows of a warp: every third group of four
         constexpr int PER = (NX + 31) / 32;
         int64_t* offs = (int64_t*)(pf_smem + C::OFFS);
-        const int32_t* trow = a.c.table + (int64_t)seq * a.c.table_stride;
-        const uint16_t* kbase = a.c.k + kvh * a.c.head_stride;
-        const uint16_t* vbase = a.c.v + kvh * a.c.head_stride;
-        const int lo = a.o.window > 0 ? max(0, qlo - a.o.window + 1) : 0;
+        const int boxes = a.box ? BN / a.box : 0;
+        int slot0 = 0, segments = 0, handed = 0;             // ring slots and segments so far, slots handed over (copied rows only)
+        for (; wk.more() && ok; wk.next(a)) {
+        if (!wk.segment()) continue;
+        const int n = wk.n, i0 = wk.i0, len = t.len, prefix = t.prefix, qhi = t.qhi;
+        if (n == 0) continue;
+        const int32_t* trow = a.c.table + (int64_t)wk.seq * a.c.table_stride;
+        const uint16_t* kbase = a.c.k + wk.head * a.c.head_stride;
+        const uint16_t* vbase = a.c.v + wk.head * a.c.head_stride;
+        const int lo = a.o.window > 0 ? max(0, t.qlo - a.o.window + 1) : 0;
         auto row_of = [&](int x) { return (x >> 2) * 12 + lw * 4 + (x & 3); };
         auto key_of = [&](int j, int x) {                    // -1: a row nobody sees
-            const int rr = row_of(x), key = kt.tile(i0 + j) * BN + rr;
+            const int rr = row_of(x), key = t.kt.tile(i0 + j) * BN + rr;
             return x < NX && rr < BN && key < len && (key < prefix || (key >= lo && key <= qhi)) ? key : -1;
         };
         auto free_slot = [&](int slot) {
@@ -614,10 +737,9 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             paged_cp_commit();
         };
         // ---- by pages: lane i looks after box i of a tile ----
-        const int boxes = a.box ? BN / a.box : 0;
         int box_page = 0;
         auto box_key = [&](int j) {                          // -1: nobody sees a row of the box
-            const int key = kt.tile(i0 + j) * BN + lane * a.box;
+            const int key = t.kt.tile(i0 + j) * BN + lane * a.box;
             return j < n && lane < boxes && key < len && (key < prefix || (key + a.box > lo && key <= qhi)) ? key : -1;
         };
         auto fetch_box_page = [&](int j) {
@@ -627,13 +749,13 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         auto copy_boxes = [&](int slot, const CUtensorMap* map, int j, int pages_of_tile) {
             const int key = box_key(j);
             const int in_page = key >= 0 ? key % a.c.page_size : -1;
-            const int st = slot % ST, total = boxes * (D / 64), t = lane * 3 + lw;
-            const int bx = min(t / (D / 64), 31), slab = t % (D / 64);
+            const int st = slot % ST, total = boxes * (D / 64), x = lane * 3 + lw;
+            const int bx = min(x / (D / 64), 31), slab = x % (D / 64);
             const int pg = __shfl_sync(0xffffffffu, pages_of_tile, bx), row = __shfl_sync(0xffffffffu, in_page, bx);
-            if (t < total && row >= 0) {
+            if (x < total && row >= 0) {
                 mbar_expect_tx(&full[st], a.box * 128);
-                pf_tma_4d(smem + C::RING + st * C::KV_BYTES + slab * C::SLAB + bx * a.box * 128, map, slab * 64, a.rows_first ? row : kvh,
-                          a.rows_first ? kvh : row, pg, &full[st]);
+                pf_tma_4d(smem + C::RING + st * C::KV_BYTES + slab * C::SLAB + bx * a.box * 128, map, slab * 64, a.rows_first ? row : wk.head,
+                          a.rows_first ? wk.head : row, pg, &full[st]);
             } else {
                 pf_arrive(&full[st]);
             }
@@ -645,16 +767,57 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                 paged_cp_wait<0>();
                 pf_fence_async();
                 pf_arrive(&full[slot % ST]);
-            } else if (slot >= C::LAG) {
+            } else if (slot - handed >= C::LAG) {
                 paged_cp_wait<C::LAG>();
                 pf_fence_async();
-                pf_arrive(&full[(slot - C::LAG) % ST]);
+                pf_arrive(&full[handed++ % ST]);
             }
+        };
+        // The segment's queries, when the last scores of the segment before are done: by TMA, or each warp every third 32 rows, of which
+        // lane i knows where row i lies.
+        auto load_queries = [&] {
+            if (!a.box) {                                    // nothing may be waited for here that waits for a slot in flight
+                paged_cp_wait<0>();
+                pf_fence_async();
+                while (handed < slot0 + k_slot(0) + 1) pf_arrive(&full[handed++ % ST]);
+            }
+            ok = __all_sync(0xffffffffu, pf_wait(q_empty, (segments & 1) ^ 1));
+            if (!ok) return;
+            const int tiles = t.two ? 2 : 1;
+            if (a.q_box) {                                   // tokens behind the sequence's last are somebody else's, or zeros: never stored
+                if (lw == 0 && lane < tiles * (D / 64)) {
+                    const int qt = lane / (D / 64), slab = lane % (D / 64);
+                    mbar_expect_tx(q_full, a.tokens * a.G * 128);
+                    pf_tma_3d(smem + qt * C::Q_BYTES + slab * (128 * 128), &q_map, slab * 64, wk.head * a.G, t.span.x + t.tok0 + qt * a.tokens, q_full);
+                } else {
+                    pf_arrive(q_full);
+                }
+                __syncwarp();
+                return;
+            }
+            constexpr int CPR = D / 8, RPI = 32 / CPR;       // 16-byte chunks per row, rows per instruction
+            const int c = lane % CPR;
+            for (int g0 = lw * 32; g0 < tiles * 128; g0 += 96) {
+                const int rr0 = g0 & 127, mine = rr0 + lane, tk = mine / a.G, token = t.tok0 + (g0 >> 7) * a.tokens + tk;
+                const int64_t at = tk < a.tokens && token < t.span.y
+                                       ? (t.span.x + token) * a.q_stride + (int64_t)(wk.head * a.G + mine - tk * a.G) * D : -1;
+                const uint32_t qs = smem + (g0 >> 7) * C::Q_BYTES;
+#pragma unroll 8
+                for (int i = 0; i < 32; i += RPI) {
+                    const int x = i + lane / CPR, rr = rr0 + x;
+                    const int64_t o = __shfl_sync(0xffffffffu, at, x);
+                    cp_async16_zfill(qs + (c >> 3) * (128 * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), a.q + (o < 0 ? 0 : o) + c * 8, o < 0 ? 0 : 16);
+                }
+            }
+            paged_cp_commit();
+            paged_cp_wait<0>();
+            pf_fence_async();
+            pf_arrive(q_full);
         };
         static_assert(16 * (D / 64) <= 96, "a lane issues one box");
         int v_page = 0, v_page2 = 0;                         // box pages of the K tiles whose V tile is still to come
         auto fill_k = [&](int j) {
-            const int slot = k_slot(j);
+            const int slot = slot0 + k_slot(j);
             if (!a.box) {
                 set_offsets(j);
                 fetch_pages(j + 1);
@@ -677,11 +840,11 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             hand_over(slot);
         };
         auto fill_v = [&](int j) {
-            const int slot = v_slot(j);
+            const int slot = slot0 + v_slot(j);
             if (!free_slot(slot)) return;
             if (a.box) {
-                const int pages_of_tile = two || n == 1 || j == n - 1 ? v_page : v_page2;
-                const int k0 = kt.tile(i0 + j) * BN;
+                const int pages_of_tile = t.two || j == n - 1 ? v_page : v_page2;
+                const int k0 = t.kt.tile(i0 + j) * BN;
                 const bool whole = k0 + BN <= len && (k0 + BN <= prefix || (k0 >= lo && k0 + BN - 1 <= qhi));
                 if (whole && __all_sync(0xffffffffu, box_key(j) < 0 || (unsigned)pages_of_tile < (unsigned)a.c.pages)) {
                     copy_boxes(slot, &v_map, j, pages_of_tile);
@@ -696,25 +859,28 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         };
         if (a.box) box_page = fetch_box_page(0);
         else fetch_pages(0);
-        if (two || n == 1) {
+        fill_k(0);
+        if (ok) load_queries();
+        if (t.two) {
             for (int j = 0; j < n && ok; j++) {
-                fill_k(j);
-                if (ok) fill_v(j);
+                fill_v(j);
+                if (ok && j + 1 < n) fill_k(j + 1);
             }
-        } else if (n > 1) {
-            fill_k(0);
-            if (ok) fill_k(1);
+        } else {
+            if (ok && n > 1) fill_k(1);
             for (int j = 0; j < n && ok; j++) {
                 fill_v(j);
                 if (ok && j + 2 < n) fill_k(j + 2);
             }
         }
+        slot0 += 2 * n;
+        segments++;
+        }
         // hand over the last slots
         paged_cp_wait<0>();
         if (ok && !a.box) {
             pf_fence_async();
-            const int slots = 2 * n;
-            for (int s = max(0, slots - C::LAG); s < slots; s++) pf_arrive(&full[s % ST]);
+            while (handed < slot0) pf_arrive(&full[handed++ % ST]);
         } else if (!ok && lane == 0) {
             atomicOr(a.wait_status, 1u << 24);
         }
@@ -725,23 +891,23 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
     if (warp == C::SM_WARPS) pf_tmem_dealloc(tmem, 512);
 }
 
-// Joins the chunks of a tile: a lane is a row, a thread 8 columns of it.
+// Joins the parts of the pair that begins in CTA blockIdx.x and ends in another: a lane is a row, a thread 8 columns of it.
 template <int D>
 __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const PrefillArgs a) {
     pdl_wait();
-    constexpr int ROWS = PfCfg<D>::ROWS, GROUPS = D / 8;
-    const int item = blockIdx.z * 256 + threadIdx.x, r = item % ROWS, col = item / ROWS, kvh = blockIdx.y, id = blockIdx.x;
-    const int4 ds = a.desc[id];
-    if (ds.z <= 1) return;
+    constexpr int ROWS = PfCfg<D>::ROWS;
+    const int4 ds = a.desc[blockIdx.x];
+    if (ds.w < 0) return;
+    const int item = blockIdx.y * 256 + threadIdx.x, r = item % ROWS, col = item / ROWS;
     const int2 span = prefill_span(a, ds.x);
-    const int row = ds.y * ROWS + r;
-    if (row >= span.y * a.G || col >= GROUPS) return;
-    const int64_t cta = ((int64_t)id * a.c.kv_heads + kvh) * a.chunks;
+    const int r_token = (r & 127) / a.G, token = (ds.y * PfCfg<D>::NQ + (r >> 7)) * a.tokens + r_token;
+    if (r_token >= a.tokens || token >= span.y) return;
     float m = -INFINITY, l = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int z = 0; z < ds.z; z++) {
-        const float2 ml = a.ml[(cta + z) * ROWS + r];
-        const float4* src = a.part + ((cta + z) * (D / 4) + 2 * col) * ROWS + r;
+    for (int c = blockIdx.x; c <= ds.w; c++) {
+        const int slot = 2 * c + (c == (int)blockIdx.x ? 1 : 0);
+        const float2 ml = a.ml[slot * ROWS + r];
+        const float4* src = a.part + ((int64_t)slot * (D / 4) + 2 * col) * ROWS + r;
         const float4 p = src[0], q = src[ROWS];
         const float nm = fmaxf(m, ml.x), ref = nm == -INFINITY ? 0.f : nm;
         const float e0 = ex2(m - ref), e1 = ex2(ml.x - ref);     // -inf -> 0
@@ -751,41 +917,26 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const PrefillAr
         x[4] = x[4] * e0 + q.x * e1; x[5] = x[5] * e0 + q.y * e1; x[6] = x[6] * e0 + q.z * e1; x[7] = x[7] * e0 + q.w * e1;
     }
     const float inv = l > 0.f ? 1.0f / l : 0.f;
-    const int64_t tok = span.x + row / a.G;
-    const int head = kvh * a.G + row % a.G;
+    const int64_t tok = span.x + token;
+    const int head = ds.z * a.G + (r & 127) - r_token * a.G;
     *(uint4*)(a.out + tok * a.out_stride + (int64_t)head * D + col * 8) =
         make_uint4(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv), pack_bf16x2(x[4] * inv, x[5] * inv), pack_bf16x2(x[6] * inv, x[7] * inv));
     if (a.lse && col == 0) a.lse[tok * a.Hq + head] = (m + log2f(l)) * 0.6931471805599453f;
 }
 
-struct PrefillPlan { int tiles, chunks, chunk_tiles; size_t part, ml, desc, total; };
-// Cutting the keys of a tile. A CTA holds an SM, so with `work` key tiles in all an SM has work / SMs of them to do: a tile whose keys are
-// a good deal more than half of that is cut, so that its longest piece does not decide the time (prompts: the last rows see
-// twice the average; chunks behind contexts of different lengths). Not below four key tiles: a CTA's start, its partial
-// output and the join then cost more than they save.
-static PrefillPlan prefill_plan(int D, int kv_heads, int seqs, int total_q, int q_heads, int max_ctx, int window, int has_prefix) {
+struct PrefillPlan { int ctas; size_t part, ml, desc, total; };
+// one CTA per SM, fewer where the work (bounded by max_ctx keys per sequence) has fewer parts
+static PrefillPlan prefill_plan(int D, int kv_heads, int seqs, int total_q, int q_heads, int max_ctx) {
     PrefillPlan p;
-    const int rows = D == 256 ? 128 : 256, bn = D == 256 ? 64 : 128, G = q_heads / kv_heads, sms = paged_sm_count();
-    // each sequence may end in a tile of its own; none has fewer than one row
-    p.tiles = (int)std::min<int64_t>((int64_t)total_q * G / rows + std::min(seqs, total_q), (int64_t)total_q * ((G + rows - 1) / rows));
-    const int64_t ctas = (int64_t)p.tiles * kv_heads;
-    // key tiles of the longest row tile, and of an average one: the mean over a sequence's new rows is half of them less
-    double keys = max_ctx, mean = std::max(0.5 * max_ctx, max_ctx - 0.5 * total_q / std::max(1, seqs));
-    if (window > 0 && !has_prefix) {
-        const double seen = (double)window + rows / G + bn;
-        keys = std::min(keys, seen);
-        mean = std::min(mean, seen);
-    }
-    const double longest = keys / bn, work = std::max(1.0, mean / bn) * ctas;
-    const double piece = std::max(4.0, work / (2.0 * sms));
-    p.chunks = (int)std::max(1.0, std::min(longest / piece, 1024.0));
-    p.chunk_tiles = std::max(1, (int)((longest + p.chunks - 1) / p.chunks));
+    const int rows = D == 256 ? 128 : 256, bn = D == 256 ? 64 : 128, tokens = rows / 128 * (128 / (q_heads / kv_heads));
+    const int64_t tiles = std::min<int64_t>((int64_t)total_q / tokens + seqs, total_q);   // each sequence may end in one of its own
+    const int64_t units = tiles * kv_heads * (PF_START + ((int64_t)max_ctx + bn - 1) / bn * (rows == 256 ? PF_TWO : PF_ONE));
+    p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(paged_sm_count(), units / PF_LEAST));
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
-    const size_t parts = p.chunks > 1 ? (size_t)ctas * p.chunks * rows : 0;
-    p.part = up(parts * D * 4);
-    p.ml = up(parts * 8);
-    p.desc = p.chunks > 1 ? up((size_t)p.tiles * 16) : 0;
-    p.total = std::max<size_t>(16, p.part + p.ml + p.desc);
+    p.part = up((size_t)2 * p.ctas * rows * D * 4);
+    p.ml = up((size_t)2 * p.ctas * rows * 8);
+    p.desc = up((size_t)p.ctas * 16);
+    p.total = p.part + p.ml + p.desc;
     return p;
 }
 
@@ -819,8 +970,18 @@ static bool prefill_maps(const PagedCache& c, int D, int bn, CUtensorMap* km, CU
     return true;
 }
 
+// Tensor map of the queries: boxes of 64 head dimensions by the G heads of a kv head by the tokens of a row tile.
+static bool prefill_q_map(const PrefillArgs& a, int D, CUtensorMap* qm) {
+    if (a.q_stride % D || a.q_stride >= (int64_t)1 << 38 || !encode_tiled()) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)a.Hq, (cuuint64_t)a.total_q};
+    const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)a.q_stride * 2};
+    const cuuint32_t boxes[3] = {64, (cuuint32_t)a.G, (cuuint32_t)a.tokens}, es[3] = {1, 1, 1};
+    return encode_tiled()(qm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, (void*)a.q, dims, strides, boxes, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D, int FEAT>
-static int32_t launch_prefill(cudaStream_t s, PrefillArgs a) {
+static int32_t launch_prefill(cudaStream_t s, PrefillArgs a, int ctas) {
     using C = PfCfg<D>;
     static uint32_t attr_devs = 0;
     static std::mutex mu;
@@ -833,26 +994,24 @@ static int32_t launch_prefill(cudaStream_t s, PrefillArgs a) {
             attr_devs |= 1u << (dev & 31);
         }
     }
-    const int64_t ctas = (int64_t)a.tiles * a.c.kv_heads * a.chunks;
-    CUtensorMap km = {}, vm = {};
+    CUtensorMap qm = {}, km = {}, vm = {};
+    a.q_box = prefill_q_map(a, D, &qm);
     if (!prefill_maps(a.c, D, C::BN, &km, &vm, &a.box, &a.rows_first)) a.box = 0;
-    paged_prefill_kernel<D, FEAT><<<(unsigned)ctas, C::THREADS, C::TOTAL, s>>>(km, vm, a);
+    paged_prefill_kernel<D, FEAT><<<ctas, C::THREADS, C::TOTAL, s>>>(qm, km, vm, a);
     LTHN_CUDA_TRY(cudaGetLastError());
-    if (a.chunks > 1) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(a.tiles, a.c.kv_heads, C::ROWS * (D / 8) / 256); cfg.blockDim = dim3(256); cfg.stream = s;
-        cudaLaunchAttribute at[1];
-        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        at[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = at; cfg.numAttrs = 1;
-        LTHN_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_prefill_join_kernel<D>, a));
-    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas, C::ROWS * (D / 8) / 256); cfg.blockDim = dim3(256); cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    LTHN_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_prefill_join_kernel<D>, a));
     return LTHN_OK;
 }
 template <int D>
-static int32_t launch_prefill_feat(cudaStream_t s, const PrefillArgs& a) {
+static int32_t launch_prefill_feat(cudaStream_t s, const PrefillArgs& a, int ctas) {
     const int f = (a.o.softcap > 0.f ? 1 : 0) | (a.o.slopes ? 2 : 0);
-    return f == 0 ? launch_prefill<D, 0>(s, a) : f == 1 ? launch_prefill<D, 1>(s, a) : f == 2 ? launch_prefill<D, 2>(s, a) : launch_prefill<D, 3>(s, a);
+    return f == 0 ? launch_prefill<D, 0>(s, a, ctas) : f == 1 ? launch_prefill<D, 1>(s, a, ctas) : f == 2 ? launch_prefill<D, 2>(s, a, ctas) : launch_prefill<D, 3>(s, a, ctas);
 }
 
 }  // namespace lthn
@@ -863,19 +1022,13 @@ static int32_t prefill_check(const lthn_paged_kv* cache, int32_t seqs, int32_t t
     int32_t rc;
     if ((rc = paged_check_cache("paged_prefill_attention", cache, c))) return rc;
     LTHN_REQUIRE(seqs >= 0 && total_q >= 0 && max_ctx >= 0, "paged_prefill_attention: negative size");
+    LTHN_REQUIRE(seqs <= 32768, "paged_prefill_attention: at most 32768 sequences per call");
     LTHN_REQUIRE(seqs <= cache->seqs, "paged_prefill_attention: more sequences than the page table has");
     LTHN_REQUIRE(q_heads > 0 && q_heads <= 65535 && q_heads % cache->kv_heads == 0, "paged_prefill_attention: q_heads must be a positive multiple of kv_heads");
-    LTHN_REQUIRE((int64_t)total_q * (q_heads / cache->kv_heads) < ((int64_t)1 << 31) - 512, "paged_prefill_attention: too many query rows");
+    LTHN_REQUIRE(q_heads / cache->kv_heads <= 128, "paged_prefill_attention: at most 128 query heads per kv head");
+    LTHN_REQUIRE(total_q <= 1 << 30, "paged_prefill_attention: too many query rows");
     return LTHN_OK;
 }
-static int32_t prefill_plan_for(const lthn_paged_kv* cache, const PagedCache& c, const lthn_attn_options* o, int32_t seqs, int32_t total_q, int32_t q_heads,
-                                int32_t max_ctx, PrefillPlan* p) {
-    *p = prefill_plan(cache->head_dim, cache->kv_heads, seqs, total_q, q_heads, max_ctx ? std::min(max_ctx, c.capacity) : c.capacity, o ? o->window : 0,
-                      o && o->prefix_lens);
-    LTHN_REQUIRE((int64_t)p->tiles * cache->kv_heads * p->chunks < (int64_t)1 << 31, "paged_prefill_attention: too many query rows");
-    return LTHN_OK;
-}
-
 extern "C" {
 
 int32_t lthn_paged_prefill_attention_workspace(const lthn_paged_kv* cache, int32_t seqs, int32_t total_q, int32_t q_heads, int32_t max_ctx,
@@ -883,12 +1036,9 @@ int32_t lthn_paged_prefill_attention_workspace(const lthn_paged_kv* cache, int32
     clear_error();
     LTHN_REQUIRE(bytes != nullptr, "paged_prefill_attention_workspace: bytes is NULL");
     PagedCache c;
-    PrefillPlan p;
     int32_t rc;
     if ((rc = prefill_check(cache, seqs, total_q, q_heads, max_ctx, &c))) return rc;
-    // without options: a window only makes the longest and the average tile shorter and more alike, so fewer pieces
-    if ((rc = prefill_plan_for(cache, c, nullptr, seqs, total_q, q_heads, max_ctx, &p))) return rc;
-    *bytes = p.total;
+    *bytes = prefill_plan(cache->head_dim, cache->kv_heads, seqs, total_q, q_heads, max_ctx ? std::min(max_ctx, c.capacity) : c.capacity).total;
     return LTHN_OK;
 }
 
@@ -899,7 +1049,6 @@ int32_t lthn_paged_prefill_attention(void* stream, const lthn_paged_kv* cache, c
     clear_error();
     const char* me = "paged_prefill_attention";
     PrefillArgs a = {};
-    PrefillPlan p;
     int32_t rc;
     if ((rc = prefill_check(cache, seqs, total_q, q_heads, max_ctx, &a.c))) return rc;
     const int D = cache->head_dim;
@@ -909,24 +1058,24 @@ int32_t lthn_paged_prefill_attention(void* stream, const lthn_paged_kv* cache, c
     a.q_stride = q_stride ? q_stride : (int64_t)q_heads * D;
     a.out_stride = out_stride ? out_stride : (int64_t)q_heads * D;
     LTHN_REQUIRE(((a.q_stride | a.out_stride) & 7) == 0, "paged_prefill_attention: strides must be multiples of 8 elements");
-    LTHN_REQUIRE(a.out_stride >= (int64_t)q_heads * D, "paged_prefill_attention: rows of out would overlap");
+    LTHN_REQUIRE(a.q_stride >= (int64_t)q_heads * D && a.out_stride >= (int64_t)q_heads * D, "paged_prefill_attention: rows of q or out would overlap");
     LTHN_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15) == 0, "paged_prefill_attention: q, out and workspace must be 16-byte aligned");
-    if ((rc = prefill_plan_for(cache, a.c, options, seqs, total_q, q_heads, max_ctx, &p))) return rc;
+    const PrefillPlan p = prefill_plan(D, cache->kv_heads, seqs, total_q, q_heads, max_ctx ? std::min(max_ctx, a.c.capacity) : a.c.capacity);
     LTHN_REQUIRE(workspace_bytes >= p.total, "paged_prefill_attention: workspace too small");
     if ((rc = paged_check_device(me, "the cache", cache->k))) return rc;
     if ((rc = paged_check_device(me, "q", q))) return rc;
     a.q = q; a.out = out; a.q_start = q_start; a.lens = kv_lens; a.lse = lse;
     a.seqs = seqs; a.total_q = total_q; a.Hq = q_heads; a.G = q_heads / cache->kv_heads;
-    a.tiles = p.tiles; a.chunks = p.chunks; a.chunk_tiles = p.chunk_tiles;
+    a.tokens = 128 / a.G;
     a.part = (float4*)workspace;
     a.ml = (float2*)((char*)workspace + p.part);
     a.desc = (int4*)((char*)workspace + p.part + p.ml);
     a.wait_status = device_status_word();
     a.c.status = device_paged_status_word();
     if (!a.c.status) return fail(LTHN_ERR_CUDA, "paged_prefill_attention: no device status word");
-    if (D == 64) return launch_prefill_feat<64>((cudaStream_t)stream, a);
-    if (D == 128) return launch_prefill_feat<128>((cudaStream_t)stream, a);
-    return launch_prefill_feat<256>((cudaStream_t)stream, a);
+    if (D == 64) return launch_prefill_feat<64>((cudaStream_t)stream, a, p.ctas);
+    if (D == 128) return launch_prefill_feat<128>((cudaStream_t)stream, a, p.ctas);
+    return launch_prefill_feat<256>((cudaStream_t)stream, a, p.ctas);
 }
 
 }  // extern "C"

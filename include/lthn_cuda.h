@@ -294,7 +294,8 @@ int32_t lthn_prefill_attention(void* stream, const float* q, const uint16_t* kca
  * table's table_stride*page_size rows, a sequence number >= seqs or a decreasing q_start sets bit
  * LTHN_STATUS_PAGED of the sticky device status (lthn_device_status returns LTHN_ERR_INVALID for
  * it alone). Nothing out of bounds is touched: such rows are not stored, such keys count as zero
- * vectors, lengths are cut at the table; the outputs of the call are then not valid. */
+ * vectors, lengths are cut at the table (and at 2^26 rows, the most a
+ * sequence may have); the outputs of the call are then not valid. */
 #define LTHN_STATUS_PAGED 0x40000000u
 typedef struct {
     uint16_t* k;                /* bf16 */
@@ -364,7 +365,7 @@ typedef struct {
  * row does not wait for its own block. workspace: device memory of
  * lthn_paged_sdpa_decode_workspace bytes, 16-byte aligned, uninitialised; nothing is kept in it between
  * calls, but calls that can overlap (two streams, two captured graphs) need one each. Strides are
- * elements between rows (0 -> dense), multiples of 8; q and out 16-byte aligned. */
+ * elements between rows (0 -> dense), multiples of 8; q and out 16-byte aligned. At most 65535 rows. */
 int32_t lthn_paged_sdpa_decode_workspace(const lthn_paged_kv* cache, int32_t rows, int32_t q_heads, int32_t dtype, size_t* bytes);
 int32_t lthn_paged_sdpa_decode(void* stream, const lthn_paged_kv* cache, const lthn_attn_options* options, const void* q, int32_t dtype,
                                int64_t q_stride, const int32_t* kv_lens, int32_t rows, int32_t q_heads, void* out, int64_t out_stride,
@@ -375,10 +376,11 @@ int32_t lthn_paged_sdpa_decode(void* stream, const lthn_paged_kv* cache, const l
  * decreasing, device memory) are the last of the kv_lens[s] positions of sequence s, which are all in the cache. Tokens of
  * different sequences do not see each other. Rows that q_start leaves out are not touched, neither is their
  * lse; a sequence with more query rows than positions has empty rows in front. Scores and sums are f32, the weights
- * are rounded to bf16 for the second product, as in lthn_prefill_attention. max_ctx (0: the table's rows)
- * bounds kv_lens for the choice of how the work is cut; longer sequences are still computed right. A NaN or
- * infinity in a value row that some query of a tile sees may reach the other queries of that tile (256 rows of
- * tokens times query heads of a kv head). Workspace and strides as above. */
+ * are rounded to bf16 for the second product, as in lthn_prefill_attention. The work of the call is one list that is
+ * dealt out evenly, as above. max_ctx (0: the table's rows) bounds kv_lens for the number of blocks and the workspace of a
+ * small call; longer sequences are still computed right. A NaN or infinity in a value row that some query of a tile
+ * sees may reach the other queries of that tile (up to 256 rows of tokens times query heads of a kv head). At most
+ * 32768 sequences and 128 query heads per kv head. Workspace and strides as above. */
 int32_t lthn_paged_prefill_attention_workspace(const lthn_paged_kv* cache, int32_t seqs, int32_t total_q, int32_t q_heads, int32_t max_ctx,
                                                size_t* bytes);
 int32_t lthn_paged_prefill_attention(void* stream, const lthn_paged_kv* cache, const lthn_attn_options* options, const uint16_t* q,

@@ -78,7 +78,7 @@ def test_decode_refuses(lthn, bad):
 
 @pytest.mark.parametrize("bad", [dict(seqs=-1), dict(seqs=3), dict(total=-1), dict(ctx=-1), dict(q_heads=0), dict(q_heads=5), dict(q=None), dict(out=None),
                                  dict(start=None), dict(lens=None), dict(ws=None), dict(n=8), dict(q=A + 2), dict(out=A + 8), dict(ws=A + 4), dict(qs=257),
-                                 dict(os=12), dict(os=128), dict(total=1 << 30)], ids=str)
+                                 dict(os=12), dict(os=128), dict(qs=128), dict(total=(1 << 30) + 1), dict(q_heads=258)], ids=str)
 def test_prefill_refuses(lthn, bad):
     assert prefill(lthn, desc(lthn), **bad) == 1
 
