@@ -12,7 +12,10 @@ struct PagedCache {
     const int32_t* table;
     int64_t page_stride, row_stride, head_stride;
     int pages, page_size, table_stride, seqs, kv_heads;
-    int capacity;        // rows the table can name for a sequence
+    int capacity;        // rows the table can name for a sequence, at most 2^26
+    // position / page_size for positions below 2^27: (position * div_mul) >> div_shift, with div_shift = 27 + ceil(log2 page_size) and
+    // div_mul = ceil(2^div_shift / page_size); the product's error, position * (div_mul * page_size - 2^div_shift), stays below 2^div_shift
+    uint32_t div_mul, div_shift;
     uint32_t* status;
 };
 
@@ -33,7 +36,10 @@ int32_t paged_check_device(const char* name, const char* what, const void* p);
 int paged_sm_count();
 
 #ifdef __CUDACC__
-// Element offset of kv head 0 of position pos of sequence seq, or -1 (and the status bit) for a page outside the pool.
+__device__ __forceinline__ int paged_entry(const PagedCache& c, int pos) { return (int)(((uint64_t)(uint32_t)pos * c.div_mul) >> c.div_shift); }
+__device__ __forceinline__ int paged_row(const PagedCache& c, int pos) { return pos - paged_entry(c, pos) * c.page_size; }
+
+// Element offset of kv head 0 of a row of a page, or -1 (and the status bit) for a page outside the pool.
 __device__ __forceinline__ int64_t paged_offset(const PagedCache& c, int page, int in_page) {
     if ((unsigned)page >= (unsigned)c.pages) {
         atomicOr(c.status, LTHN_STATUS_PAGED);

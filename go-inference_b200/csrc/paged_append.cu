@@ -58,6 +58,9 @@ int32_t paged_check_cache(const char* name, const lthn_paged_kv* c, PagedCache* 
     o.pages = c->pages; o.page_size = c->page_size; o.table_stride = c->table_stride; o.seqs = c->seqs; o.kv_heads = c->kv_heads;
     o.capacity = (int)std::min<int64_t>((int64_t)c->table_stride * c->page_size, 1 << 26);
     o.status = nullptr;
+    o.div_shift = 27;
+    while (((int64_t)1 << (o.div_shift - 27)) < c->page_size) o.div_shift++;
+    o.div_mul = (uint32_t)((((uint64_t)1 << o.div_shift) + c->page_size - 1) / (uint32_t)c->page_size);
     *out = o;
     return LTHN_OK;
 }
@@ -116,7 +119,7 @@ __global__ void __launch_bounds__(AP_THREADS) paged_append_kernel(const AppendAr
         if (tid == 0) atomicOr(a.c.status, LTHN_STATUS_PAGED);
         return;
     }
-    const int entry = pos / a.c.page_size;
+    const int entry = paged_entry(a.c, pos);
     const int64_t off = paged_offset(a.c, a.c.table[(int64_t)seq * a.c.table_stride + entry], pos - entry * a.c.page_size);
     if (off < 0) return;
     for (int i = tid; i < a.half_rot; i += AP_THREADS) {

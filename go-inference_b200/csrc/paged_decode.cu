@@ -72,13 +72,11 @@ __device__ __forceinline__ KeyTiles decode_tiles(const DecodeArgs& a, int row) {
     return key_tiles<DEC_TILE>(len - 1, len - 1, len, a.o.prefix ? a.o.prefix[row] : 0, a.o.window);
 }
 
-// capped, biased score in log2 units. x: the raw product
-__device__ __forceinline__ float decode_score(const AttnOpts& o, float x, float slope, int gap) {
-    constexpr float LOG2E = 1.4426950408889634f;
-    x *= o.scale;
-    if (o.softcap > 0.f) x = o.softcap * tanhf(x / o.softcap);
-    if (o.slopes) x -= slope * (float)abs(gap);
-    return x * LOG2E;
+// capped, biased score in log2 units. x: the raw product; in: scale / cap or scale * log2 e; cap, slope: times log2 e
+__device__ __forceinline__ float decode_score(float x, float in, float cap, float slope, int gap) {
+    x *= in;
+    if (cap > 0.f) x = cap * tanhf(x);
+    return fmaf(-slope, (float)abs(gap), x);
 }
 
 template <int D, int MODE>
@@ -101,11 +99,13 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
 
     pdl_trigger();
     // ---- this CTA's pieces -----------------------------------------------------------------------
-    int64_t U = 0;                                // in tiles of rows first, times the triples of a row
-    for (int r0 = 0; r0 < a.rows; r0 += DEC_THREADS) {
-        int incl;
+    int incl, mine = tid < a.rows ? decode_tiles(a, tid).n : 0;
+    int total = paged_block_scan<DEC_WARPS>(mine, incl, s_scan);
+    int64_t U = total;                            // in tiles of rows first, times the triples of a row
+    for (int r0 = DEC_THREADS; r0 < a.rows; r0 += DEC_THREADS) {
         const int r = r0 + tid;
-        U += paged_block_scan<DEC_WARPS>(r < a.rows ? decode_tiles(a, r).n : 0, incl, s_scan);
+        int x;
+        U += paged_block_scan<DEC_WARPS>(r < a.rows ? decode_tiles(a, r).n : 0, x, s_scan);
     }
     U *= triples;
     const int ctas = (int)min((int64_t)a.ctas, U);   // none of them without a piece
@@ -114,20 +114,21 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
     // the row that holds piece u0
     int64_t base = 0;
     int row = 0;
-    for (int r0 = 0; r0 < a.rows; r0 += DEC_THREADS) {
-        const int r = r0 + tid;
-        const int n = r < a.rows ? decode_tiles(a, r).n : 0;
-        int incl;
-        const int total = paged_block_scan<DEC_WARPS>(n, incl, s_scan);
+    for (int r0 = 0;;) {
         if ((base + total) * triples > u0) {
-            if (n > 0 && (base + incl) * triples > u0 && (base + incl - n) * triples <= u0) { s_row = r; s_base = incl - n; }
+            if (mine > 0 && (base + incl) * triples > u0 && (base + incl - mine) * triples <= u0) { s_row = r0 + tid; s_base = incl - mine; }
             __syncthreads();
             row = s_row;
             base = (base + s_base) * triples;     // first piece of the row
             break;
         }
         base += total;
+        r0 += DEC_THREADS;
+        mine = r0 + tid < a.rows ? decode_tiles(a, r0 + tid).n : 0;
+        total = paged_block_scan<DEC_WARPS>(mine, incl, s_scan);
     }
+    constexpr float LOG2E = 1.4426950408889634f;
+    const float s_in = a.o.softcap > 0.f ? a.o.scale / a.o.softcap : a.o.scale * LOG2E, s_cap = a.o.softcap * LOG2E;
 
     int64_t u = u0;
     while (u < u1 && row < a.rows) {
@@ -148,6 +149,43 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
         const int32_t* trow = a.c.table + (int64_t)row * a.c.table_stride;
 
         __syncthreads();                          // the ring and the query area are free
+        // ---- loads: piece i of the triple into stage i % NST ---------------------------------------
+        // lanes 0-15 keep the page of "their" key of the next piece to be loaded, fetched one piece ahead
+        auto my_key = [&](int i) {                // -1: not visible (its row is zeros)
+            const int key = kt.tile(i) * DEC_TILE + warp * DEC_WK + lane;
+            return lane < DEC_WK && key < len && (key < prefix || key >= lo) ? key : -1;
+        };
+        auto page_of = [&](int i) {
+            const int key = i < i0 + count ? my_key(i) : -1;
+            return key >= 0 ? trow[paged_entry(a.c, key)] : 0;
+        };
+        auto issue = [&](int i, int page) {
+            if (i < i0 + count) {
+                const int key = my_key(i);
+                const int64_t off = key >= 0 ? paged_offset(a.c, page, paged_row(a.c, key)) : -1;
+                constexpr int CPR = D / 8;        // 16-byte chunks per row
+                constexpr int RPI = 32 / CPR > 0 ? 32 / CPR : 1;   // rows per instruction
+                const uint32_t st = ring + (i % NST) * C::STAGE;
+                const int c = lane % CPR;
+#pragma unroll
+                for (int r0 = 0; r0 < DEC_WK; r0 += RPI) {
+                    const int r = r0 + (RPI > 1 ? lane / CPR : 0);
+                    const int64_t o = __shfl_sync(0xffffffffu, off, r);
+                    const int64_t e = (o < 0 ? 0 : o) + c * 8;
+                    const int n = o < 0 ? 0 : 16;
+                    cp_async16_zfill(st + r * PITCH + c * 16, kbase + e, n);
+                    cp_async16_zfill(st + (DEC_WK + r) * PITCH + c * 16, vbase + e, n);
+                }
+            }
+            paged_cp_commit();
+        };
+        int page = page_of(i0);
+#pragma unroll
+        for (int s = 0; s < NST - 1; s++) {
+            const int next = page_of(i0 + s + 1);
+            issue(i0 + s, page);
+            page = next;
+        }
         // ---- queries -----------------------------------------------------------------------------
         for (int i = tid; i < HB * (D / 8); i += DEC_THREADS) {
             const int h = i / (D / 8), c = i - h * (D / 8);
@@ -179,52 +217,14 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
         __syncthreads();
         float slope[2] = {0.f, 0.f};
         if (a.o.slopes) {
-            if (g < nh) slope[0] = a.o.slopes[h0 + g];
-            if (HB == 16 && g + 8 < nh) slope[1] = a.o.slopes[h0 + g + 8];
+            if (g < nh) slope[0] = a.o.slopes[h0 + g] * LOG2E;
+            if (HB == 16 && g + 8 < nh) slope[1] = a.o.slopes[h0 + g + 8] * LOG2E;
         }
 
-        // ---- loads: piece i of the triple into stage i % NST ---------------------------------------
-        // lanes 0-15 keep the page of "their" key of the next piece to be loaded, fetched one piece ahead
-        auto my_key = [&](int i) {                // -1: not visible (its row is zeros)
-            const int key = kt.tile(i) * DEC_TILE + warp * DEC_WK + lane;
-            return lane < DEC_WK && key < len && (key < prefix || key >= lo) ? key : -1;
-        };
-        auto page_of = [&](int i) {
-            const int key = i < i0 + count ? my_key(i) : -1;
-            return key >= 0 ? trow[key / a.c.page_size] : 0;
-        };
-        auto issue = [&](int i, int page) {
-            if (i < i0 + count) {
-                const int key = my_key(i);
-                const int64_t off = key >= 0 ? paged_offset(a.c, page, key % a.c.page_size) : -1;
-                constexpr int CPR = D / 8;        // 16-byte chunks per row
-                constexpr int RPI = 32 / CPR > 0 ? 32 / CPR : 1;   // rows per instruction
-                const uint32_t st = ring + (i % NST) * C::STAGE;
-                const int c = lane % CPR;
-#pragma unroll
-                for (int r0 = 0; r0 < DEC_WK; r0 += RPI) {
-                    const int r = r0 + (RPI > 1 ? lane / CPR : 0);
-                    const int64_t o = __shfl_sync(0xffffffffu, off, r);
-                    const int64_t e = (o < 0 ? 0 : o) + c * 8;
-                    const int n = o < 0 ? 0 : 16;
-                    cp_async16_zfill(st + r * PITCH + c * 16, kbase + e, n);
-                    cp_async16_zfill(st + (DEC_WK + r) * PITCH + c * 16, vbase + e, n);
-                }
-            }
-            paged_cp_commit();
-        };
         float acc[ND][4];
 #pragma unroll
         for (int n = 0; n < ND; n++) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
         float mrun[2] = {-INFINITY, -INFINITY}, lrun[2] = {0.f, 0.f};
-        int page = page_of(i0);
-#pragma unroll
-        for (int s = 0; s < NST - 1; s++) {
-            const int next = page_of(i0 + s + 1);
-            issue(i0 + s, page);
-            page = next;
-        }
-
         for (int i = i0; i < i0 + count; i++) {
             const int next = page_of(i + NST);
             paged_cp_wait<NST - 2>();
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
                     const int n = e >> 1, x = e & 1, key = key0 + n * 8 + 2 * t + x;
                     float s = c[n][2 * r + x];
                     if (MODE == DEC_F32_8) s += c[n][2 + x] + c2[n][x];
-                    s = decode_score(a.o, s, slope[r], pos - key);
+                    s = decode_score(s, s_in, s_cap, slope[r], pos - key);
                     p[r][e] = key < len && (key < prefix || key >= lo) ? s : -INFINITY;
                     mx[r] = fmaxf(mx[r], p[r][e]);
                 }
@@ -390,14 +390,15 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
 // takes parts w, w+4, ... with a running maximum, four loads in flight.
 template <int D>
 __global__ void __launch_bounds__(128) paged_decode_join_kernel(const DecodeArgs a, int HB, int out_f32) {
-    pdl_wait();
     constexpr int DL = D / 32;
     __shared__ float sm[4], sl[4];
     __shared__ float so[4][D];
     const int row = blockIdx.y, qh = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     float* of = (float*)a.out + row * a.out_stride + (int64_t)qh * D;
     uint16_t* ob = (uint16_t*)a.out + row * a.out_stride + (int64_t)qh * D;
-    if (a.lens[row] <= 0 || a.c.capacity == 0) {
+    const int len = a.lens[row];                  // not written by the kernel before: no need to wait for it
+    pdl_wait();
+    if (len <= 0 || a.c.capacity == 0) {
         for (int d = tid; d < D; d += 128) {
             if (out_f32) of[d] = 0.f;
             else ob[d] = 0;

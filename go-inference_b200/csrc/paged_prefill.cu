@@ -104,7 +104,7 @@ __device__ __forceinline__ PfTile prefill_tile(const PrefillArgs& a, int seq, in
 }
 // What a (tile, head) pair costs: about 0.6 us per unit. A key tile of two row tiles keeps the tensor pipe busier than one of one; the start covers
 // the first scores, the last output and its way to memory.
-constexpr int PF_ONE = 2, PF_TWO = 3, PF_START = 5;
+constexpr int PF_ONE = 2, PF_TWO = 3, PF_START = 6;
 constexpr int PF_LEAST = 8;   // units of a CTA below which fewer CTAs are used: every part holds a key tile
 static_assert(PF_LEAST >= 2 * PF_TWO, "a range within a pair holds a whole key tile");
 __device__ __forceinline__ int pf_key_cost(const PfTile& t) { return t.two ? PF_TWO : PF_ONE; }
@@ -702,14 +702,14 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
 #pragma unroll
             for (int e = 0; e < PER; e++) {
                 const int key = j < n ? key_of(j, lane + 32 * e) : -1;
-                page[e] = key >= 0 ? trow[key / a.c.page_size] : 0;
+                page[e] = key >= 0 ? trow[paged_entry(a.c, key)] : 0;
             }
         };
         auto set_offsets = [&](int j) {
 #pragma unroll
             for (int e = 0; e < PER; e++) {
                 const int x = lane + 32 * e, key = key_of(j, x);
-                if (x < NX && row_of(x) < BN) offs[(j & 1) * BN + row_of(x)] = key >= 0 ? paged_offset(a.c, page[e], key % a.c.page_size) : -1;
+                if (x < NX && row_of(x) < BN) offs[(j & 1) * BN + row_of(x)] = key >= 0 ? paged_offset(a.c, page[e], paged_row(a.c, key)) : -1;
             }
             __syncwarp();
         };
@@ -744,11 +744,11 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         };
         auto fetch_box_page = [&](int j) {
             const int key = box_key(j);
-            return key >= 0 ? trow[key / a.c.page_size] : 0;
+            return key >= 0 ? trow[paged_entry(a.c, key)] : 0;
         };
         auto copy_boxes = [&](int slot, const CUtensorMap* map, int j, int pages_of_tile) {
             const int key = box_key(j);
-            const int in_page = key >= 0 ? key % a.c.page_size : -1;
+            const int in_page = key >= 0 ? paged_row(a.c, key) : -1;
             const int st = slot % ST, total = boxes * (D / 64), x = lane * 3 + lw;
             const int bx = min(x / (D / 64), 31), slab = x % (D / 64);
             const int pg = __shfl_sync(0xffffffffu, pages_of_tile, bx), row = __shfl_sync(0xffffffffu, in_page, bx);
