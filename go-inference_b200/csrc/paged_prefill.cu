@@ -18,7 +18,7 @@
 //                   works on one buffer while the other's softmax runs. With two row tiles the buffers belong to them;
 //                   with one they alternate over its key tiles, and the warpgroups pass the running maximum of a row to one
 //                   another (the sums stay apart until the end), which leaves only load and maximum in sequence.
-//   loaders         three warps fetch the queries of a segment and fill a ring of K and V tiles in the 128-byte swizzle. Where the page size is a multiple of 8 (the
+//   loaders         three warps fetch the queries of an item and fill a ring of K and V tiles in the 128-byte swizzle. Where the page size is a multiple of 8 (the
 //                   swizzle's row group) by tiled TMA, one box per page, 64 head dimensions and gcd(page size, BN) rows. V rows
 //                   that nobody sees must be zeros (they may hold NaN, which a weight of zero would not silence), so a V
 //                   tile with such rows - the last of a sequence, the first of a window - and pools of other page
@@ -29,13 +29,14 @@
 // their bf16 rounding (relative) nor the f32 sums mind, and O in tensor memory needs no correction. A move multiplies
 // O by 2^(old - new) through registers; after the first tiles it is rare.
 //
-// Work. The key tiles of all (row tile, kv head) pairs form one list, weighted by what they cost; CTA c of C (one per SM) takes the
-// c-th C-th of it, whatever the lengths are, and walks through its segments without stopping: the loaders are at the next
-// segment's queries and keys while the softmax warps finish the last one. A pair that lies within one CTA is finished there; otherwise each
-// CTA that holds part of it leaves (maximum, sum, unnormalised output) in its slot of the workspace - at most two such
-// parts, its first and its last segment - and a second kernel joins them. (One CTA per tile, longest first, spent 7 us of
-// each CTA on its start and end; cut into equal chunks, the few rows of drafts against long contexts of different lengths took
-// two waves where the work was one.)
+// Work. An item is (row tile, kv head, chunk of its key tiles); the grid has one CTA per item, the longest first, but only as many
+// run as there are SMs: a CTA that is through with loading an item cancels the launch of a waiting one
+// (clusterlaunchcontrol) and takes its item over, so barriers, tensor memory and pipeline stay up and the loads of the next item run under
+// the last products and the output of this one. One of the loader warps does this and publishes the item to the other
+// roles. (One CTA per item spent 7 us of each on its start and end, 8192 tokens of 32 heads: XXX us against YYY. A fixed
+// even share per CTA of a list weighted by cost loses more than that: what a key tile costs depends on its mask and on who shares it in L2.)
+// Where there are few items the keys of a tile are cut into chunks, which leave (maximum, sum, unnormalised output)
+// in the workspace for a second kernel to join.
 //
 // Every wait is bounded: on a time-out the roles record it in the device status word, drain what they have in flight, free
 // the tensor memory and return.
@@ -63,9 +64,12 @@ struct PrefillArgs {
     int seqs, total_q, Hq, G;
     int tokens;          // of a row tile: 128 / G
     int q_box;           // queries by TMA (their row stride is a multiple of head_dim), else copied row by row
-    float4* part;        // [2*CTAs][D/4][rows] unnormalised outputs, four columns each
-    float2* ml;          // [2*CTAs][rows] maximum (log2 units) and sum
-    int4* desc;          // [CTAs] the pair that begins in the CTA and ends in another: sequence, tile, head, last CTA (-1: none)
+    int tiles;           // upper bound of the row tiles of all sequences
+    int chunks;          // chunks per row tile and kv head
+    int chunk_tiles;     // key tiles per chunk
+    float4* part;        // [tiles*kv_heads*chunks][D/4][rows] unnormalised outputs, four columns each
+    float2* ml;          // [tiles*kv_heads*chunks][rows] maximum (log2 units) and sum
+    int4* desc;          // [tiles] sequence, tile of the sequence, chunks in use
 };
 
 // The rows of sequence s, made safe: within [0, total_q).
@@ -78,80 +82,36 @@ __device__ __forceinline__ int2 prefill_span(const PrefillArgs& a, int s) {
     return make_int2(b, e - b);
 }
 
-// The tokens of one or two row tiles of a sequence.
-struct PfTile {
-    int2 span;           // the sequence's rows of q: first, count
+// What the roles need to know of an item; one lies in shared memory while the next is worked out.
+struct PfItem {
+    int seq, head;       // head < 0: no more items
+    int first, tokens;   // the sequence's rows of q
     int len, pos0;       // keys; position of the first query
     int prefix;
-    int tok0;            // first token of the tile
-    int qlo, qhi;        // positions of its first and last token
+    int tok0;            // first token of the row tiles
+    int qlo, qhi;        // positions of their first and last token
+    int two;             // both row tiles have tokens
     KeyTiles kt;
-    bool two;            // both row tiles have tokens
+    int i0, n;           // key tiles [i0, i0 + n) of kt; n = 0 where nobody sees anything
+    int part;            // place in the workspace, -1: not cut, the output is final
 };
 template <int NQ, int BN>
-__device__ __forceinline__ PfTile prefill_tile(const PrefillArgs& a, int seq, int tile) {
-    PfTile t;
-    t.span = prefill_span(a, seq);
+__device__ __forceinline__ PfItem prefill_tile(const PrefillArgs& a, int seq, int tile) {
+    PfItem t;
+    const int2 span = prefill_span(a, seq);
+    t.seq = seq;
+    t.first = span.x;
+    t.tokens = span.y;
     t.len = paged_length(a.c, a.lens[seq]);
-    t.pos0 = t.len - t.span.y;
+    t.pos0 = t.len - t.tokens;
     t.prefix = a.o.prefix ? min(max(a.o.prefix[seq], 0), t.len) : 0;
     t.tok0 = tile * NQ * a.tokens;
     t.qlo = t.pos0 + t.tok0;
-    t.qhi = t.pos0 + min(t.tok0 + NQ * a.tokens, t.span.y) - 1;
+    t.qhi = t.pos0 + min(t.tok0 + NQ * a.tokens, t.tokens) - 1;
     t.kt = key_tiles<BN>(t.qlo, t.qhi, t.len, t.prefix, a.o.window);
-    t.two = NQ == 2 && t.span.y - t.tok0 > a.tokens;
+    t.two = NQ == 2 && t.tokens - t.tok0 > a.tokens;
     return t;
 }
-// What a (tile, head) pair costs: about 0.6 us per unit. A key tile of two row tiles keeps the tensor pipe busier than one of one; the start covers
-// the first scores, the last output and its way to memory.
-constexpr int PF_ONE = 2, PF_TWO = 3, PF_START = 6;
-constexpr int PF_LEAST = 8;   // units of a CTA below which fewer CTAs are used: every part holds a key tile
-static_assert(PF_LEAST >= 2 * PF_TWO, "a range within a pair holds a whole key tile");
-__device__ __forceinline__ int pf_key_cost(const PfTile& t) { return t.two ? PF_TWO : PF_ONE; }
-__device__ __forceinline__ int pf_cost(const PfTile& t) { return PF_START + t.kt.n * pf_key_cost(t); }
-// the key tiles that lie before unit v of a pair
-__device__ __forceinline__ int pf_tiles_before(const PfTile& t, int v) { return v <= PF_START ? 0 : (v - PF_START) / pf_key_cost(t); }
-
-// The walk of a CTA through its segments; every role makes its own.
-template <int NQ, int BN>
-struct PfWalk {
-    PfTile t;
-    int seq, tile, head, v, cost;
-    int64_t u, u1;
-    int i0, n, take;     // segment: key tiles [i0, i0 + n) of the pair
-    __device__ __forceinline__ void start(const PrefillArgs& a, int seq_, int tile_, int64_t base, int64_t u0, int64_t end) {
-        seq = seq_; tile = tile_; u = u0; u1 = end;
-        t = prefill_tile<NQ, BN>(a, seq, tile);
-        cost = pf_cost(t);
-        head = (int)((u0 - base) / cost);
-        v = (int)((u0 - base) - (int64_t)head * cost);
-    }
-    __device__ __forceinline__ bool more() const { return u < u1; }
-    // false: nothing to do in this one
-    __device__ __forceinline__ bool segment() {
-        take = (int)min((int64_t)(cost - v), u1 - u);
-        i0 = pf_tiles_before(t, v);
-        n = pf_tiles_before(t, v + take) - i0;
-        return n > 0 || (t.kt.n == 0 && v == 0);
-    }
-    __device__ __forceinline__ bool whole() const { return n == t.kt.n; }
-    __device__ __forceinline__ void next(const PrefillArgs& a) {
-        u += take;
-        v += take;
-        if (v < cost || u >= u1) return;
-        v = 0;
-        if (++head < a.c.kv_heads) return;
-        head = 0;
-        tile++;
-        if (tile * NQ * (int64_t)a.tokens >= t.span.y) {
-            tile = 0;
-            do seq++; while (seq < a.seqs && prefill_span(a, seq).y == 0);
-            if (seq >= a.seqs) { u = u1; return; }       // only if the lengths changed under the call
-        }
-        t = prefill_tile<NQ, BN>(a, seq, tile);
-        cost = pf_cost(t);
-    }
-};
 
 // ---- tcgen05 wrappers (cta_group::1) ---------------------------------------------------------------
 __device__ __forceinline__ void pf_tmem_alloc(uint32_t* smem_dst, uint32_t ncols) {
@@ -187,6 +147,19 @@ __device__ __forceinline__ void pf_tma_3d(uint32_t dst, const CUtensorMap* map, 
 __device__ __forceinline__ void pf_tma_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar)) : "memory");
+}
+// Asks for the launch of a waiting CTA to be cancelled; the answer (16 bytes) comes by mbarrier. After a refusal no CTA asks again.
+__device__ __forceinline__ void pf_try_cancel(void* answer, uint64_t* bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                 ::"r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
+}
+// the block index that now is this CTA's to do, -1: none
+__device__ __forceinline__ int pf_cancelled(const void* answer) {
+    int x;
+    asm volatile("{\n\t.reg .b128 h;\n\t.reg .pred p;\n\tld.shared.b128 h, [%1];\n\tmov.b32 %0, -1;\n\t"
+                 "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+                 "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n\t}" : "=r"(x) : "r"(smem_u32(answer)) : "memory");
+    return x;
 }
 __device__ __forceinline__ void pf_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -261,6 +234,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 // the n lowest bits of a word, n of any size and sign
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+__device__ __forceinline__ int warp_sum_int(int v) { return (int)__reduce_add_sync(0xffffffffu, (unsigned)v); }
 // two f32 operations in one instruction
 __device__ __forceinline__ uint64_t pack2(float lo, float hi) {
     uint64_t d;
@@ -323,84 +297,31 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
     uint64_t* o_last = o_done + 2;                           // [2] the last has (a barrier of its own: with one row tile the softmax
                                                              //     may be two units ahead, which a parity cannot tell from none)
     uint64_t* turn = o_last + 2;                             // [4] one row tile: the maximum of key tile j is out, per 32 rows
-    uint64_t* q_full = turn + 4;                             // queries of a segment
+    uint64_t* q_full = turn + 4;                             // queries of an item
     uint64_t* q_empty = q_full + 1;                          // its last scores are done
     uint64_t* meet = q_empty + 1;                            // both softmax warpgroups (a barrier whose wait is bounded)
     uint64_t* drain = meet + 1;
-    uint32_t* tmem_slot = (uint32_t*)(drain + 1);
-    int* scan = (int*)(tmem_slot + 2);                       // WARPS words, then sequence, tile and (64 bits) first unit of the first tile
-    static_assert((2 * ST + 20) * 8 + (C::WARPS + 4) * 4 <= 512, "barriers and scan words");
+    uint64_t* item_full = drain + 1;                         // [2] the item is there
+    uint64_t* item_empty = item_full + 2;                    // [2] everybody has read it
+    uint64_t* answered = item_empty + 2;
+    uint32_t* tmem_slot = (uint32_t*)(answered + 1);
+    unsigned char* answer = pf_smem + C::BARS + 320;         // 16 bytes
+    PfItem* items = (PfItem*)(answer + 16);                  // [2]
+    static_assert((2 * ST + 21) * 8 + 8 <= 320 && 336 + 2 * sizeof(PfItem) <= 512, "barriers and items");
 
-    pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-
-    // ---- this CTA's part of the work ------------------------------------------------------------------
-    int* first = (int*)(pf_smem + C::RING);                  // first tile of each sequence
-    int T = 0;
-    for (int s0 = 0; s0 < a.seqs; s0 += C::THREADS) {
-        const int s = s0 + tid;
-        const int c = s < a.seqs ? (prefill_span(a, s).y + C::NQ * a.tokens - 1) / (C::NQ * a.tokens) : 0;
-        int incl;
-        const int total = paged_block_scan<C::WARPS>(c, incl, scan);
-        if (s < a.seqs) first[s] = T + incl - c;
-        T += total;
-    }
-    __syncthreads();
-    auto find = [&](int t) {                                 // the last sequence that begins at or before tile t (empty ones begin with the next)
-        int lo = 0, hi = a.seqs - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (first[mid] <= t) lo = mid;
-            else hi = mid - 1;
-        }
-        return lo;
-    };
-    auto cost_of = [&](int t) {
-        if (t >= T) return 0;
-        const int s = find(t);
-        return pf_cost(prefill_tile<C::NQ, BN>(a, s, t - first[s]));
-    };
-    int incl, mine = cost_of(tid);
-    int part = paged_block_scan<C::WARPS>(mine, incl, scan);
-    int64_t U = part;
-    for (int t0 = C::THREADS; t0 < T; t0 += C::THREADS) {
-        int x;
-        U += paged_block_scan<C::WARPS>(cost_of(t0 + tid), x, scan);
-    }
-    U *= a.c.kv_heads;
-    const int ctas = (int)max((int64_t)1, min((int64_t)gridDim.x, U / PF_LEAST));
-    if (T == 0 || (int)blockIdx.x >= ctas) {
-        if (tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, -1);
-        return;
-    }
-    const int64_t u0 = U * blockIdx.x / ctas, u1 = U * (blockIdx.x + 1) / ctas;
-    int64_t* first_unit = (int64_t*)(scan + C::WARPS + 2);
-    int64_t base = 0;
-    for (int t0 = 0;;) {
-        if ((base + part) * a.c.kv_heads > u0) {
-            const int64_t b = (base + incl - mine) * a.c.kv_heads;
-            if (mine > 0 && b <= u0 && b + (int64_t)mine * a.c.kv_heads > u0) {
-                const int s = find(t0 + tid);
-                scan[C::WARPS] = s;
-                scan[C::WARPS + 1] = t0 + tid - first[s];
-                *first_unit = b;
-            }
-            break;
-        }
-        base += part;
-        t0 += C::THREADS;
-        mine = cost_of(t0 + tid);
-        part = paged_block_scan<C::WARPS>(mine, incl, scan);
-    }
-
     if (tid == 0) {
         for (int s = 0; s < ST; s++) { mbar_init(&full[s], 96); mbar_init(&empty[s], 1); }
-        for (int b = 0; b < 2; b++) { mbar_init(&s_full[b], 1); mbar_init(&p_full[b], 128); mbar_init(&o_done[b], 1); mbar_init(&o_last[b], 1); }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(&s_full[b], 1); mbar_init(&p_full[b], 128); mbar_init(&o_done[b], 1); mbar_init(&o_last[b], 1);
+            mbar_init(&item_full[b], 1); mbar_init(&item_empty[b], C::WARPS);
+        }
         for (int w = 0; w < 4; w++) mbar_init(&turn[w], 1);
         mbar_init(q_full, 96);
         mbar_init(q_empty, 1);
         mbar_init(meet, C::SM_WARPS * 32);
         mbar_init(drain, 1);
+        mbar_init(answered, 1);
         mbar_fence_init();
     }
     if (warp == C::SM_WARPS) pf_tmem_alloc(tmem_slot, 512);
@@ -409,18 +330,28 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
     pf_fence_after();
     const uint32_t tmem = *tmem_slot;
     const uint32_t smem = smem_u32(pf_smem);
-    PfWalk<C::NQ, BN> wk;
-    wk.start(a, scan[C::WARPS], scan[C::WARPS + 1], *first_unit, u0, u1);
-    const PfTile& t = wk.t;
     bool ok = true;
+    PfItem t;
+    int items_read = 0;
+    // the next item for this warp; false: there are no more
+    auto next_item = [&] {
+        const int b = items_read & 1;
+        ok = __all_sync(0xffffffffu, pf_wait(&item_full[b], (items_read >> 1) & 1));
+        if (!ok) return false;
+        t = items[b];
+        __syncwarp();
+        if (lane == 0) pf_arrive(&item_empty[b]);
+        items_read++;
+        return t.head >= 0;
+    };
 
-    // ring slots of the K and V tile of key tile j of a segment, in the order of their last use
+    // ring slots of the K and V tile of key tile j of an item, in the order of their last use
     auto k_slot = [&](int j) { return t.two ? 2 * j : j < 2 ? j : 2 * j - 1; };
-    auto v_slot = [&](int j) { return t.two ? 2 * j + 1 : j == wk.n - 1 ? 2 * wk.n - 1 : 2 * j + 2; };
+    auto v_slot = [&](int j) { return t.two ? 2 * j + 1 : j == t.n - 1 ? 2 * t.n - 1 : 2 * j + 2; };
 
     if (warp < C::SM_WARPS) {
         // ================================ softmax ================================
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         const int wg = warp >> 2;                            // score buffer = warpgroup
         const int wr = (warp & 3) * 32, r = wr + lane;       // row within the row tile = tensor memory lane
         const int r_token = r / a.G, r_head = r - r_token * a.G;
@@ -437,13 +368,12 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             const bool met = __all_sync(0xffffffffu, pf_wait(meet, meets++ & 1));
             ok = ok && met;
         };
-        for (; wk.more() && ok; wk.next(a)) {
-        if (!wk.segment()) continue;
+        while (ok && next_item()) {
         const bool two = t.two;
-        const int n = wk.n, i0 = wk.i0, qt = two ? wg : 0, len = t.len;
+        const int n = t.n, i0 = t.i0, qt = two ? wg : 0, len = t.len;
         const int token = t.tok0 + qt * a.tokens + r_token;  // of the sequence
-        const bool live = r_token < a.tokens && token < t.span.y;
-        const int head = wk.head * a.G + r_head;
+        const bool live = r_token < a.tokens && token < t.tokens;
+        const int head = t.head * a.G + r_head;
         const int qpos = t.pos0 + token;
         // visible: key < pre, or klo <= key < khi
         const int pre = t.prefix, khi = min(qpos + 1, len), klo = a.o.window > 0 ? qpos - a.o.window + 1 : 0;
@@ -578,13 +508,12 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         }
         if (ok) {
             pf_fence_after();
-            const int64_t tok = t.span.x + token;
+            const int64_t tok = t.first + token;
             const float m2 = m * c1;                         // log2 units (c1 > 0)
             const float inv = l > 0.f ? 1.0f / l : 0.f;
             uint16_t* dst = a.out + tok * a.out_stride + (int64_t)head * D;
-            const bool whole = wk.whole();
-            const int slot = 2 * blockIdx.x + (i0 > 0 ? 0 : 1);
-            float4* part = a.part + (int64_t)slot * (D / 4) * ROWS + qt * 128 + r;
+            const bool whole = t.part < 0;
+            float4* part = a.part + (int64_t)t.part * (D / 4) * ROWS + qt * 128 + r;
 #pragma unroll 1
             for (int x = x0; x < x1; x += 32) {
                 float o[32];
@@ -608,30 +537,26 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                 }
             }
             if (live && x0 == 0) {
-                if (!whole) a.ml[slot * ROWS + qt * 128 + r] = make_float2(m2, l);
+                if (!whole) a.ml[(int64_t)t.part * ROWS + qt * 128 + r] = make_float2(m2, l);
                 else if (a.lse) a.lse[tok * a.Hq + head] = (m2 + log2f(l)) * 0.6931471805599453f;
             }
         }
-        if (!two && n > 0) pair_sync();                      // both have read O before the next segment's first weights let it be replaced
+        if (!two && n > 0) pair_sync();                      // both have read O before the next item's first weights let it be replaced
         }
         if (!ok && lane == 0) atomicOr(a.wait_status, 1u << 26);
     } else if (warp == C::SM_WARPS) {
         // ================================ issuer ================================
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         // f32 accumulators, bf16 operands, M = 128; S: N = BN, both K-major; O: N = D, B is N-major
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);
         const uint32_t idesc_s = idesc | ((uint32_t)(BN >> 3) << 17), idesc_o = idesc | (1u << 16) | ((uint32_t)(D >> 3) << 17);
-        int slot0 = 0, segments = 0;                         // ring slots and segments so far
+        int slot0 = 0, seen = 0;                             // ring slots and items with keys so far
         uint32_t uses = 0;                                   // bit b: parity of the uses of score buffer b
-        int4 begun = make_int4(0, 0, 0, -1);
-        for (; wk.more() && ok; wk.next(a)) {
-            if (!wk.segment()) continue;
+        while (ok && next_item()) {
             const bool two = t.two;
-            const int n = wk.n, units = two ? 2 * n : n;
-            if (wk.i0 == 0 && !wk.whole())
-                begun = make_int4(wk.seq, wk.tile, wk.head, (int)(((wk.u - wk.v + wk.cost) * ctas + U - 1) / U) - 1);
+            const int n = t.n, units = two ? 2 * n : n;
             if (n == 0) continue;
-            ok = __all_sync(0xffffffffu, pf_wait(q_full, segments & 1));
+            ok = __all_sync(0xffffffffu, pf_wait(q_full, seen & 1));
             auto scores = [&](int u) {
                 const int j = two ? u >> 1 : u, qt = two ? u & 1 : 0, slot = slot0 + k_slot(j), st = slot % ST;
                 ok = __all_sync(0xffffffffu, pf_wait(&full[st], (slot / ST) & 1));
@@ -661,31 +586,114 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                 if (u + 2 < units) scores(u + 2);
             }
             slot0 += 2 * n;
-            segments++;
+            seen++;
         }
         if (!ok) {
             if (lane == 0) atomicOr(a.wait_status, 1u << 25);
             pf_commit(drain);                                // nothing of this CTA may still run when its memory is given back
             pf_wait(drain, 0);
         }
-        if (lane == 0) a.desc[blockIdx.x] = begun;
         __syncwarp();
     } else {
         // ================================ loaders ================================
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         const int lw = warp - C::SM_WARPS - 1;
         constexpr int NX = (BN / 4 + 2) / 3 * 4;             // rows of a warp: every third group of four
         constexpr int PER = (NX + 31) / 32;
         int64_t* offs = (int64_t*)(pf_smem + C::OFFS);
         const int boxes = a.box ? BN / a.box : 0;
-        int slot0 = 0, segments = 0, handed = 0;             // ring slots and segments so far, slots handed over (copied rows only)
-        for (; wk.more() && ok; wk.next(a)) {
-        if (!wk.segment()) continue;
-        const int n = wk.n, i0 = wk.i0, len = t.len, prefix = t.prefix, qhi = t.qhi;
-        if (n == 0) continue;
-        const int32_t* trow = a.c.table + (int64_t)wk.seq * a.c.table_stride;
-        const uint16_t* kbase = a.c.k + wk.head * a.c.head_stride;
-        const uint16_t* vbase = a.c.v + wk.head * a.c.head_stride;
+        int slot0 = 0, seen = 0, handed = 0;                 // ring slots and items with keys so far, slots handed over (copied rows only)
+        // ---- the last of the three warps also finds the items ----
+        const bool finder = lw == 2;
+        int tiles_here = 0, tiles = 0, published = 0, asked = 0;  // row tiles of sequence `lane`, of all sequences; items, questions so far
+        auto tiles_of = [&](int sq) { return sq < a.seqs ? (prefill_span(a, sq).y + C::NQ * a.tokens - 1) / (C::NQ * a.tokens) : 0; };
+        auto warp_scan = [&](int v) {
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += u;
+            }
+            return v;
+        };
+        // item `id` in `x`; false: there is no such tile or chunk. Tiles are counted from the last one, the longest of a prompt.
+        auto look_up = [&](int id, PfItem& x) {
+            const int rest = id / a.c.kv_heads, chunk = rest % a.chunks, tile_id = rest / a.chunks;
+            if (tile_id >= tiles) {
+                if (a.chunks > 1 && chunk == 0 && id % a.c.kv_heads == 0 && lane == 0) a.desc[tile_id] = make_int4(0, 0, 0, 0);
+                return false;
+            }
+            int want = tiles - 1 - tile_id, sq = 0, count = tiles_here;
+            for (int s0 = 0;; s0 += 32, count = tiles_of(s0 + lane)) {
+                const int incl = warp_scan(count), total = __shfl_sync(0xffffffffu, incl, 31);
+                if (want < total) {
+                    const int l = __ffs(__ballot_sync(0xffffffffu, incl > want)) - 1;
+                    want -= __shfl_sync(0xffffffffu, incl - count, l);
+                    sq = s0 + l;
+                    break;
+                }
+                want -= total;
+                if (s0 + 32 >= a.seqs) return false;         // only if q_start changed under the call
+            }
+            x = prefill_tile<C::NQ, BN>(a, sq, want);
+            x.head = id % a.c.kv_heads;
+            const int per = max(a.chunk_tiles, (x.kt.n + a.chunks - 1) / a.chunks);   // also where max_ctx was too small
+            const int used = a.chunks > 1 ? max(1, (x.kt.n + per - 1) / per) : 1;
+            if (a.chunks > 1 && chunk == 0 && x.head == 0 && lane == 0) a.desc[tile_id] = make_int4(sq, want, used, 0);
+            if (chunk >= used) return false;
+            x.i0 = chunk * per;
+            x.n = a.chunks > 1 ? min(per, x.kt.n - x.i0) : x.kt.n;
+            x.part = used > 1 ? (tile_id * a.c.kv_heads + x.head) * a.chunks + chunk : -1;
+            return true;
+        };
+        auto publish = [&](const PfItem& x) {
+            const int b = published & 1;
+            ok = ok && __all_sync(0xffffffffu, pf_wait(&item_empty[b], ((published >> 1) & 1) ^ 1));
+            if (!ok) return;
+            if (lane == 0) {
+                items[b] = x;
+                pf_arrive(&item_full[b]);
+            }
+            published++;
+            __syncwarp();
+        };
+        auto find_next = [&] {
+            PfItem x;
+            for (;;) {
+                if (lane == 0) {
+                    pf_fence_async();                        // the last answer has been read
+                    mbar_expect_tx(answered, 16);
+                    pf_try_cancel(answer, answered);
+                }
+                __syncwarp();
+                ok = ok && __all_sync(0xffffffffu, pf_wait(answered, asked & 1));
+                if (!ok) return;
+                asked++;
+                const int id = pf_cancelled(answer);
+                __syncwarp();
+                if (id < 0) {
+                    x.head = -1;
+                    break;
+                }
+                if (look_up(id, x)) break;
+            }
+            publish(x);
+        };
+        if (finder) {
+            tiles_here = tiles_of(lane);
+            for (int s0 = 0; s0 < a.seqs; s0 += 32) tiles += warp_sum_int(s0 ? tiles_of(s0 + lane) : tiles_here);
+            PfItem x;
+            if (look_up(blockIdx.x, x)) publish(x);
+            else find_next();
+        }
+        while (ok && next_item()) {
+        const int n = t.n, i0 = t.i0, len = t.len, prefix = t.prefix, qhi = t.qhi;
+        if (n == 0) {
+            if (finder) find_next();
+            continue;
+        }
+        const int32_t* trow = a.c.table + (int64_t)t.seq * a.c.table_stride;
+        const uint16_t* kbase = a.c.k + t.head * a.c.head_stride;
+        const uint16_t* vbase = a.c.v + t.head * a.c.head_stride;
         const int lo = a.o.window > 0 ? max(0, t.qlo - a.o.window + 1) : 0;
         auto row_of = [&](int x) { return (x >> 2) * 12 + lw * 4 + (x & 3); };
         auto key_of = [&](int j, int x) {                    // -1: a row nobody sees
@@ -754,8 +762,8 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             const int pg = __shfl_sync(0xffffffffu, pages_of_tile, bx), row = __shfl_sync(0xffffffffu, in_page, bx);
             if (x < total && row >= 0) {
                 mbar_expect_tx(&full[st], a.box * 128);
-                pf_tma_4d(smem + C::RING + st * C::KV_BYTES + slab * C::SLAB + bx * a.box * 128, map, slab * 64, a.rows_first ? row : wk.head,
-                          a.rows_first ? wk.head : row, pg, &full[st]);
+                pf_tma_4d(smem + C::RING + st * C::KV_BYTES + slab * C::SLAB + bx * a.box * 128, map, slab * 64, a.rows_first ? row : t.head,
+                          a.rows_first ? t.head : row, pg, &full[st]);
             } else {
                 pf_arrive(&full[st]);
             }
@@ -773,7 +781,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                 pf_arrive(&full[handed++ % ST]);
             }
         };
-        // The segment's queries, when the last scores of the segment before are done: by TMA, or each warp every third 32 rows, of which
+        // The item's queries, when the last scores of the item before are done: by TMA, or each warp every third 32 rows, of which
         // lane i knows where row i lies.
         auto load_queries = [&] {
             if (!a.box) {                                    // nothing may be waited for here that waits for a slot in flight
@@ -781,14 +789,14 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                 pf_fence_async();
                 while (handed < slot0 + k_slot(0) + 1) pf_arrive(&full[handed++ % ST]);
             }
-            ok = __all_sync(0xffffffffu, pf_wait(q_empty, (segments & 1) ^ 1));
+            ok = __all_sync(0xffffffffu, pf_wait(q_empty, (seen & 1) ^ 1));
             if (!ok) return;
-            const int tiles = t.two ? 2 : 1;
+            const int row_tiles = t.two ? 2 : 1;
             if (a.q_box) {                                   // tokens behind the sequence's last are somebody else's, or zeros: never stored
-                if (lw == 0 && lane < tiles * (D / 64)) {
+                if (lw == 0 && lane < row_tiles * (D / 64)) {
                     const int qt = lane / (D / 64), slab = lane % (D / 64);
                     mbar_expect_tx(q_full, a.tokens * a.G * 128);
-                    pf_tma_3d(smem + qt * C::Q_BYTES + slab * (128 * 128), &q_map, slab * 64, wk.head * a.G, t.span.x + t.tok0 + qt * a.tokens, q_full);
+                    pf_tma_3d(smem + qt * C::Q_BYTES + slab * (128 * 128), &q_map, slab * 64, t.head * a.G, t.first + t.tok0 + qt * a.tokens, q_full);
                 } else {
                     pf_arrive(q_full);
                 }
@@ -797,10 +805,10 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             }
             constexpr int CPR = D / 8, RPI = 32 / CPR;       // 16-byte chunks per row, rows per instruction
             const int c = lane % CPR;
-            for (int g0 = lw * 32; g0 < tiles * 128; g0 += 96) {
+            for (int g0 = lw * 32; g0 < row_tiles * 128; g0 += 96) {
                 const int rr0 = g0 & 127, mine = rr0 + lane, tk = mine / a.G, token = t.tok0 + (g0 >> 7) * a.tokens + tk;
-                const int64_t at = tk < a.tokens && token < t.span.y
-                                       ? (t.span.x + token) * a.q_stride + (int64_t)(wk.head * a.G + mine - tk * a.G) * D : -1;
+                const int64_t at = tk < a.tokens && token < t.tokens
+                                       ? (t.first + token) * a.q_stride + (int64_t)(t.head * a.G + mine - tk * a.G) * D : -1;
                 const uint32_t qs = smem + (g0 >> 7) * C::Q_BYTES;
 #pragma unroll 8
                 for (int i = 0; i < 32; i += RPI) {
@@ -874,7 +882,8 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             }
         }
         slot0 += 2 * n;
-        segments++;
+        seen++;
+        if (finder && ok) find_next();                       // all loads of this item are on their way
         }
         // hand over the last slots
         paged_cp_wait<0>();
@@ -891,23 +900,22 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
     if (warp == C::SM_WARPS) pf_tmem_dealloc(tmem, 512);
 }
 
-// Joins the parts of the pair that begins in CTA blockIdx.x and ends in another: a lane is a row, a thread 8 columns of it.
+// Joins the chunks of a row tile: a lane is a row, a thread 8 columns of it.
 template <int D>
 __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const PrefillArgs a) {
-    pdl_wait();
     constexpr int ROWS = PfCfg<D>::ROWS;
+    const int item = blockIdx.z * 256 + threadIdx.x, r = item % ROWS, col = item / ROWS, kvh = blockIdx.y;
     const int4 ds = a.desc[blockIdx.x];
-    if (ds.w < 0) return;
-    const int item = blockIdx.y * 256 + threadIdx.x, r = item % ROWS, col = item / ROWS;
+    if (ds.z <= 1) return;
     const int2 span = prefill_span(a, ds.x);
     const int r_token = (r & 127) / a.G, token = (ds.y * PfCfg<D>::NQ + (r >> 7)) * a.tokens + r_token;
     if (r_token >= a.tokens || token >= span.y) return;
+    const int64_t first = ((int64_t)blockIdx.x * a.c.kv_heads + kvh) * a.chunks;
     float m = -INFINITY, l = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int c = blockIdx.x; c <= ds.w; c++) {
-        const int slot = 2 * c + (c == (int)blockIdx.x ? 1 : 0);
-        const float2 ml = a.ml[slot * ROWS + r];
-        const float4* src = a.part + ((int64_t)slot * (D / 4) + 2 * col) * ROWS + r;
+    for (int c = 0; c < ds.z; c++) {
+        const float2 ml = a.ml[(first + c) * ROWS + r];
+        const float4* src = a.part + ((first + c) * (D / 4) + 2 * col) * ROWS + r;
         const float4 p = src[0], q = src[ROWS];
         const float nm = fmaxf(m, ml.x), ref = nm == -INFINITY ? 0.f : nm;
         const float e0 = ex2(m - ref), e1 = ex2(ml.x - ref);     // -inf -> 0
@@ -918,25 +926,37 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const PrefillAr
     }
     const float inv = l > 0.f ? 1.0f / l : 0.f;
     const int64_t tok = span.x + token;
-    const int head = ds.z * a.G + (r & 127) - r_token * a.G;
+    const int head = kvh * a.G + (r & 127) - r_token * a.G;
     *(uint4*)(a.out + tok * a.out_stride + (int64_t)head * D + col * 8) =
         make_uint4(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv), pack_bf16x2(x[4] * inv, x[5] * inv), pack_bf16x2(x[6] * inv, x[7] * inv));
     if (a.lse && col == 0) a.lse[tok * a.Hq + head] = (m + log2f(l)) * 0.6931471805599453f;
 }
 
-struct PrefillPlan { int ctas; size_t part, ml, desc, total; };
-// one CTA per SM, fewer where the work (bounded by max_ctx keys per sequence) has fewer parts
-static PrefillPlan prefill_plan(int D, int kv_heads, int seqs, int total_q, int q_heads, int max_ctx) {
+struct PrefillPlan { int tiles, chunks, chunk_tiles; size_t part, ml, desc, total; };
+// Cutting the keys of a tile. With `work` key tiles in all an SM has work / SMs of them to do: a tile whose keys are a good deal more than half
+// of that is cut, so that its longest piece does not decide the time (prompts: the last rows see twice the average; chunks
+// behind contexts of different lengths). Not below four key tiles: a partial output and the join then cost more than they save.
+static PrefillPlan prefill_plan(int D, int kv_heads, int seqs, int total_q, int q_heads, int max_ctx, int window, bool has_prefix) {
     PrefillPlan p;
-    const int rows = D == 256 ? 128 : 256, bn = D == 256 ? 64 : 128, tokens = rows / 128 * (128 / (q_heads / kv_heads));
-    const int64_t tiles = std::min<int64_t>((int64_t)total_q / tokens + seqs, total_q);   // each sequence may end in one of its own
-    const int64_t units = tiles * kv_heads * (PF_START + ((int64_t)max_ctx + bn - 1) / bn * (rows == 256 ? PF_TWO : PF_ONE));
-    p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(paged_sm_count(), units / PF_LEAST));
+    const int rows = D == 256 ? 128 : 256, bn = D == 256 ? 64 : 128, tokens = rows / 128 * (128 / (q_heads / kv_heads)), sms = paged_sm_count();
+    p.tiles = (int)std::min<int64_t>((int64_t)total_q / tokens + std::min(seqs, total_q), total_q);   // each sequence may end in one of its own
+    const int64_t pairs = (int64_t)p.tiles * kv_heads;
+    // key tiles of the longest row tile, and of an average one: the mean over a sequence's new rows is half of them less
+    double keys = max_ctx, mean = std::max(0.5 * max_ctx, max_ctx - 0.5 * total_q / std::max(1, seqs));
+    if (window > 0 && !has_prefix) {
+        keys = std::min(keys, (double)window + tokens + bn);
+        mean = std::min(mean, keys);
+    }
+    const double longest = keys / bn, work = std::max(1.0, mean / bn) * pairs;
+    const double piece = std::max(4.0, work / (2.0 * sms));
+    p.chunks = (int)std::max(1.0, std::min(longest / piece, 1024.0));
+    p.chunk_tiles = std::max(1, (int)((longest + p.chunks - 1) / p.chunks));
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
-    p.part = up((size_t)2 * p.ctas * rows * D * 4);
-    p.ml = up((size_t)2 * p.ctas * rows * 8);
-    p.desc = up((size_t)p.ctas * 16);
-    p.total = p.part + p.ml + p.desc;
+    const size_t parts = p.chunks > 1 ? (size_t)pairs * p.chunks : 0;
+    p.part = up(parts * rows * D * 4);
+    p.ml = up(parts * rows * 8);
+    p.desc = p.chunks > 1 ? up((size_t)p.tiles * 16) : 0;
+    p.total = std::max<size_t>(16, p.part + p.ml + p.desc);
     return p;
 }
 
@@ -981,7 +1001,7 @@ static bool prefill_q_map(const PrefillArgs& a, int D, CUtensorMap* qm) {
 }
 
 template <int D, int FEAT>
-static int32_t launch_prefill(cudaStream_t s, PrefillArgs a, int ctas) {
+static int32_t launch_prefill(cudaStream_t s, PrefillArgs a) {
     using C = PfCfg<D>;
     static uint32_t attr_devs = 0;
     static std::mutex mu;
@@ -997,21 +1017,18 @@ static int32_t launch_prefill(cudaStream_t s, PrefillArgs a, int ctas) {
     CUtensorMap qm = {}, km = {}, vm = {};
     a.q_box = prefill_q_map(a, D, &qm);
     if (!prefill_maps(a.c, D, C::BN, &km, &vm, &a.box, &a.rows_first)) a.box = 0;
-    paged_prefill_kernel<D, FEAT><<<ctas, C::THREADS, C::TOTAL, s>>>(qm, km, vm, a);
+    paged_prefill_kernel<D, FEAT><<<a.tiles * a.c.kv_heads * a.chunks, C::THREADS, C::TOTAL, s>>>(qm, km, vm, a);
     LTHN_CUDA_TRY(cudaGetLastError());
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas, C::ROWS * (D / 8) / 256); cfg.blockDim = dim3(256); cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at; cfg.numAttrs = 1;
-    LTHN_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_prefill_join_kernel<D>, a));
+    if (a.chunks > 1) {
+        paged_prefill_join_kernel<D><<<dim3(a.tiles, a.c.kv_heads, C::ROWS * (D / 8) / 256), 256, 0, s>>>(a);
+        LTHN_CUDA_TRY(cudaGetLastError());
+    }
     return LTHN_OK;
 }
 template <int D>
-static int32_t launch_prefill_feat(cudaStream_t s, const PrefillArgs& a, int ctas) {
+static int32_t launch_prefill_feat(cudaStream_t s, const PrefillArgs& a) {
     const int f = (a.o.softcap > 0.f ? 1 : 0) | (a.o.slopes ? 2 : 0);
-    return f == 0 ? launch_prefill<D, 0>(s, a, ctas) : f == 1 ? launch_prefill<D, 1>(s, a, ctas) : f == 2 ? launch_prefill<D, 2>(s, a, ctas) : launch_prefill<D, 3>(s, a, ctas);
+    return f == 0 ? launch_prefill<D, 0>(s, a) : f == 1 ? launch_prefill<D, 1>(s, a) : f == 2 ? launch_prefill<D, 2>(s, a) : launch_prefill<D, 3>(s, a);
 }
 
 }  // namespace lthn
@@ -1022,7 +1039,6 @@ static int32_t prefill_check(const lthn_paged_kv* cache, int32_t seqs, int32_t t
     int32_t rc;
     if ((rc = paged_check_cache("paged_prefill_attention", cache, c))) return rc;
     LTHN_REQUIRE(seqs >= 0 && total_q >= 0 && max_ctx >= 0, "paged_prefill_attention: negative size");
-    LTHN_REQUIRE(seqs <= 32768, "paged_prefill_attention: at most 32768 sequences per call");
     LTHN_REQUIRE(seqs <= cache->seqs, "paged_prefill_attention: more sequences than the page table has");
     LTHN_REQUIRE(q_heads > 0 && q_heads <= 65535 && q_heads % cache->kv_heads == 0, "paged_prefill_attention: q_heads must be a positive multiple of kv_heads");
     LTHN_REQUIRE(q_heads / cache->kv_heads <= 128, "paged_prefill_attention: at most 128 query heads per kv head");
@@ -1038,7 +1054,8 @@ int32_t lthn_paged_prefill_attention_workspace(const lthn_paged_kv* cache, int32
     PagedCache c;
     int32_t rc;
     if ((rc = prefill_check(cache, seqs, total_q, q_heads, max_ctx, &c))) return rc;
-    *bytes = prefill_plan(cache->head_dim, cache->kv_heads, seqs, total_q, q_heads, max_ctx ? std::min(max_ctx, c.capacity) : c.capacity).total;
+    // without options: a window only makes the longest and the average tile shorter and more alike, so there are fewer pieces
+    *bytes = prefill_plan(cache->head_dim, cache->kv_heads, seqs, total_q, q_heads, max_ctx ? std::min(max_ctx, c.capacity) : c.capacity, 0, false).total;
     return LTHN_OK;
 }
 
@@ -1060,22 +1077,25 @@ int32_t lthn_paged_prefill_attention(void* stream, const lthn_paged_kv* cache, c
     LTHN_REQUIRE(((a.q_stride | a.out_stride) & 7) == 0, "paged_prefill_attention: strides must be multiples of 8 elements");
     LTHN_REQUIRE(a.q_stride >= (int64_t)q_heads * D && a.out_stride >= (int64_t)q_heads * D, "paged_prefill_attention: rows of q or out would overlap");
     LTHN_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15) == 0, "paged_prefill_attention: q, out and workspace must be 16-byte aligned");
-    const PrefillPlan p = prefill_plan(D, cache->kv_heads, seqs, total_q, q_heads, max_ctx ? std::min(max_ctx, a.c.capacity) : a.c.capacity);
+    const PrefillPlan p = prefill_plan(D, cache->kv_heads, seqs, total_q, q_heads, max_ctx ? std::min(max_ctx, a.c.capacity) : a.c.capacity, a.o.window,
+                                       a.o.prefix != nullptr);
+    LTHN_REQUIRE((int64_t)p.tiles * cache->kv_heads * p.chunks < (int64_t)1 << 31, "paged_prefill_attention: too many query rows");
     LTHN_REQUIRE(workspace_bytes >= p.total, "paged_prefill_attention: workspace too small");
     if ((rc = paged_check_device(me, "the cache", cache->k))) return rc;
     if ((rc = paged_check_device(me, "q", q))) return rc;
     a.q = q; a.out = out; a.q_start = q_start; a.lens = kv_lens; a.lse = lse;
     a.seqs = seqs; a.total_q = total_q; a.Hq = q_heads; a.G = q_heads / cache->kv_heads;
     a.tokens = 128 / a.G;
+    a.tiles = p.tiles; a.chunks = p.chunks; a.chunk_tiles = p.chunk_tiles;
     a.part = (float4*)workspace;
     a.ml = (float2*)((char*)workspace + p.part);
     a.desc = (int4*)((char*)workspace + p.part + p.ml);
     a.wait_status = device_status_word();
     a.c.status = device_paged_status_word();
     if (!a.c.status) return fail(LTHN_ERR_CUDA, "paged_prefill_attention: no device status word");
-    if (D == 64) return launch_prefill_feat<64>((cudaStream_t)stream, a, p.ctas);
-    if (D == 128) return launch_prefill_feat<128>((cudaStream_t)stream, a, p.ctas);
-    return launch_prefill_feat<256>((cudaStream_t)stream, a, p.ctas);
+    if (D == 64) return launch_prefill_feat<64>((cudaStream_t)stream, a);
+    if (D == 128) return launch_prefill_feat<128>((cudaStream_t)stream, a);
+    return launch_prefill_feat<256>((cudaStream_t)stream, a);
 }
 
 }  // extern "C"

@@ -376,11 +376,10 @@ int32_t lthn_paged_sdpa_decode(void* stream, const lthn_paged_kv* cache, const l
  * decreasing, device memory) are the last of the kv_lens[s] positions of sequence s, which are all in the cache. Tokens of
  * different sequences do not see each other. Rows that q_start leaves out are not touched, neither is their
  * lse; a sequence with more query rows than positions has empty rows in front. Scores and sums are f32, the weights
- * are rounded to bf16 for the second product, as in lthn_prefill_attention. The work of the call is one list that is
- * dealt out evenly, as above. max_ctx (0: the table's rows) bounds kv_lens for the number of blocks and the workspace of a
- * small call; longer sequences are still computed right. A NaN or infinity in a value row that some query of a tile
- * sees may reach the other queries of that tile (up to 256 rows of tokens times query heads of a kv head). At most
- * 32768 sequences and 128 query heads per kv head. Workspace and strides as above. */
+ * are rounded to bf16 for the second product, as in lthn_prefill_attention. max_ctx (0: the table's rows) bounds
+ * kv_lens for the choice of how the work is cut; longer sequences are still computed right. A NaN or infinity in a
+ * value row that some query of a tile sees may reach the other queries of that tile (up to 256 rows of tokens times
+ * query heads of a kv head). At most 128 query heads per kv head. Workspace and strides as above. */
 int32_t lthn_paged_prefill_attention_workspace(const lthn_paged_kv* cache, int32_t seqs, int32_t total_q, int32_t q_heads, int32_t max_ctx,
                                                size_t* bytes);
 int32_t lthn_paged_prefill_attention(void* stream, const lthn_paged_kv* cache, const lthn_attn_options* options, const uint16_t* q,
