@@ -292,7 +292,8 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
     uint64_t* full = (uint64_t*)(pf_smem + C::BARS);         // [ST] loaders -> issuer
     uint64_t* empty = full + ST;                             // [ST] issuer's commit -> loaders
     uint64_t* s_full = empty + ST;                           // [2] scores are there
-    uint64_t* p_full = s_full + 2;                           // [2] weights are there, O is corrected
+    uint64_t* p_half = s_full + 2;                           // [2] the first half of the weights is there, O is corrected
+    uint64_t* p_full = p_half + 2;                           // [2] the other half is
     uint64_t* o_done = p_full + 2;                           // [2] per row tile: O(u) has been added, all but the last
     uint64_t* o_last = o_done + 2;                           // [2] the last has (a barrier of its own: with one row tile the softmax
                                                              //     may be two units ahead, which a parity cannot tell from none)
@@ -307,13 +308,14 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
     uint32_t* tmem_slot = (uint32_t*)(answered + 1);
     unsigned char* answer = pf_smem + C::BARS + 320;         // 16 bytes
     PfItem* items = (PfItem*)(answer + 16);                  // [2]
-    static_assert((2 * ST + 21) * 8 + 8 <= 320 && 336 + 2 * sizeof(PfItem) <= 512, "barriers and items");
+    static_assert((2 * ST + 23) * 8 + 8 <= 320 && 336 + 2 * sizeof(PfItem) <= 512, "barriers and items");
 
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     if (tid == 0) {
         for (int s = 0; s < ST; s++) { mbar_init(&full[s], 96); mbar_init(&empty[s], 1); }
         for (int b = 0; b < 2; b++) {
-            mbar_init(&s_full[b], 1); mbar_init(&p_full[b], 128); mbar_init(&o_done[b], 1); mbar_init(&o_last[b], 1);
+            mbar_init(&s_full[b], 1); mbar_init(&p_half[b], 128); mbar_init(&p_full[b], 128);
+            mbar_init(&o_done[b], 1); mbar_init(&o_last[b], 1);
             mbar_init(&item_full[b], 1); mbar_init(&item_empty[b], C::WARPS);
         }
         for (int w = 0; w < 4; w++) mbar_init(&turn[w], 1);
@@ -475,10 +477,12 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                     w[e / 2] = pack_bf16x2(p0, p1);
                 }
                 pf_st16(s_addr + x / 2, w);
+                if (x == BN / 2 - 32 || x == BN - 32) {      // the product with V begins with the first half
+                    pf_st_wait();
+                    pf_fence_before();
+                    pf_arrive(x == BN - 32 ? &p_full[wg] : &p_half[wg]);
+                }
             }
-            pf_st_wait();
-            pf_fence_before();
-            pf_arrive(&p_full[wg]);
             float l0, l1;
             unpack2(add2(sum[0], sum[1]), l0, l1);
             l += l0 + l1;
@@ -574,13 +578,18 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             if (ok && units > 1) scores(1);
             for (int u = 0; u < units && ok; u++) {
                 const int j = two ? u >> 1 : u, qt = two ? u & 1 : 0, slot = slot0 + v_slot(j), st = slot % ST;
-                ok = __all_sync(0xffffffffu, pf_wait(&full[st], (slot / ST) & 1) && pf_wait(&p_full[u & 1], uses >> (u & 1) & 1));
-                if (!ok) break;
-                uses ^= 1u << (u & 1);
-                pf_fence_after();
                 const uint32_t vb = smem + C::RING + st * C::KV_BYTES, pa = tmem + (u & 1) * C::S_COLS, d = tmem + 256 + qt * D;
+                ok = __all_sync(0xffffffffu, pf_wait(&full[st], (slot / ST) & 1) && pf_wait(&p_half[u & 1], uses >> (u & 1) & 1));
+                if (!ok) break;
+                pf_fence_after();
 #pragma unroll
-                for (int x = 0; x < BN / 16; x++) pf_mma_ts(d, pa + x * 8, pf_desc_n(vb + x * 2048, C::SLAB), idesc_o, j > 0 || x > 0);
+                for (int x = 0; x < BN / 32; x++) pf_mma_ts(d, pa + x * 8, pf_desc_n(vb + x * 2048, C::SLAB), idesc_o, j > 0 || x > 0);
+                ok = __all_sync(0xffffffffu, pf_wait(&p_full[u & 1], uses >> (u & 1) & 1));
+                if (!ok) break;
+                pf_fence_after();
+                uses ^= 1u << (u & 1);
+#pragma unroll
+                for (int x = BN / 32; x < BN / 16; x++) pf_mma_ts(d, pa + x * 8, pf_desc_n(vb + x * 2048, C::SLAB), idesc_o, 1u);
                 if (!two || qt == 1) pf_commit(&empty[st]);
                 pf_commit(j == n - 1 ? &o_last[qt] : &o_done[qt]);   // the last commit of all is one that is waited for
                 if (u + 2 < units) scores(u + 2);
@@ -900,30 +909,60 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
     if (warp == C::SM_WARPS) pf_tmem_dealloc(tmem, 512);
 }
 
-// Joins the chunks of a row tile: a lane is a row, a thread 8 columns of it.
-template <int D>
+// Joins the chunks of a row tile. A lane is a row, a warp 8 columns of 32 rows and every CG-th chunk; with CG > 1 the warps of a column group
+// meet in shared memory. CG = 1 for up to 8 chunks: no barrier, few CTAs (4 chunks of 68 tiles: 3 us, 17 with CG = 8). CG = 8
+// above: one thread's chain of loads over the chunks would take longer than the CTAs it saves (18 chunks: 3 us less).
+template <int D, int CG>
 __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const PrefillArgs a) {
-    constexpr int ROWS = PfCfg<D>::ROWS;
-    const int item = blockIdx.z * 256 + threadIdx.x, r = item % ROWS, col = item / ROWS, kvh = blockIdx.y;
+    constexpr int ROWS = PfCfg<D>::ROWS, GROUPS = 8 / CG;        // column groups of a CTA
+    __shared__ float2 s_ml[CG > 1 ? 8 : 1][32];
+    __shared__ float s_x[CG > 1 ? 8 : 1][8][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kvh = blockIdx.y;
+    constexpr int PER_ROWS = D / 8 / GROUPS;                     // CTAs per 32 rows
+    const int r = blockIdx.z / PER_ROWS * 32 + lane, col = blockIdx.z % PER_ROWS * GROUPS + warp / CG;
     const int4 ds = a.desc[blockIdx.x];
     if (ds.z <= 1) return;
     const int2 span = prefill_span(a, ds.x);
     const int r_token = (r & 127) / a.G, token = (ds.y * PfCfg<D>::NQ + (r >> 7)) * a.tokens + r_token;
-    if (r_token >= a.tokens || token >= span.y) return;
+    const bool live = r_token < a.tokens && token < span.y;
     const int64_t first = ((int64_t)blockIdx.x * a.c.kv_heads + kvh) * a.chunks;
     float m = -INFINITY, l = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (live) {
 #pragma unroll 4
-    for (int c = 0; c < ds.z; c++) {
-        const float2 ml = a.ml[(first + c) * ROWS + r];
-        const float4* src = a.part + ((first + c) * (D / 4) + 2 * col) * ROWS + r;
-        const float4 p = src[0], q = src[ROWS];
-        const float nm = fmaxf(m, ml.x), ref = nm == -INFINITY ? 0.f : nm;
-        const float e0 = ex2(m - ref), e1 = ex2(ml.x - ref);     // -inf -> 0
-        m = nm;
-        l = l * e0 + ml.y * e1;
-        x[0] = x[0] * e0 + p.x * e1; x[1] = x[1] * e0 + p.y * e1; x[2] = x[2] * e0 + p.z * e1; x[3] = x[3] * e0 + p.w * e1;
-        x[4] = x[4] * e0 + q.x * e1; x[5] = x[5] * e0 + q.y * e1; x[6] = x[6] * e0 + q.z * e1; x[7] = x[7] * e0 + q.w * e1;
+        for (int c = warp % CG; c < ds.z; c += CG) {
+            const float2 ml = a.ml[(first + c) * ROWS + r];
+            const float4* src = a.part + ((first + c) * (D / 4) + 2 * col) * ROWS + r;
+            const float4 p = src[0], q = src[ROWS];
+            const float nm = fmaxf(m, ml.x), ref = nm == -INFINITY ? 0.f : nm;
+            const float e0 = ex2(m - ref), e1 = ex2(ml.x - ref);     // -inf -> 0
+            m = nm;
+            l = l * e0 + ml.y * e1;
+            x[0] = x[0] * e0 + p.x * e1; x[1] = x[1] * e0 + p.y * e1; x[2] = x[2] * e0 + p.z * e1; x[3] = x[3] * e0 + p.w * e1;
+            x[4] = x[4] * e0 + q.x * e1; x[5] = x[5] * e0 + q.y * e1; x[6] = x[6] * e0 + q.z * e1; x[7] = x[7] * e0 + q.w * e1;
+        }
     }
+    if (CG > 1) {
+        s_ml[warp % 8][lane] = make_float2(m, l);
+#pragma unroll
+        for (int e = 0; e < 8; e++) s_x[warp % 8][e][lane] = x[e];
+        __syncthreads();
+        if (warp > 0) return;
+#pragma unroll
+        for (int w = 0; w < CG; w++) m = fmaxf(m, s_ml[w][lane].x);
+        const float ref = m == -INFINITY ? 0.f : m;
+        l = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < CG; w++) {
+            const float2 ml = s_ml[w][lane];
+            const float e1 = ex2(ml.x - ref);
+            l = fmaf(ml.y, e1, l);
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = fmaf(s_x[w][e][lane], e1, x[e]);
+        }
+    }
+    if (!live) return;
     const float inv = l > 0.f ? 1.0f / l : 0.f;
     const int64_t tok = span.x + token;
     const int head = kvh * a.G + (r & 127) - r_token * a.G;
@@ -935,7 +974,8 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const PrefillAr
 struct PrefillPlan { int tiles, chunks, chunk_tiles; size_t part, ml, desc, total; };
 // Cutting the keys of a tile. With `work` key tiles in all an SM has work / SMs of them to do: a tile whose keys are a good deal more than half
 // of that is cut, so that its longest piece does not decide the time (prompts: the last rows see twice the average; chunks
-// behind contexts of different lengths). Not below four key tiles: a partial output and the join then cost more than they save.
+// behind contexts of different lengths). Not below 512 keys: the partial outputs and the join then cost what they save (1024 tokens of 8 heads
+// of 256: 35 us uncut, 29 us at 512 keys, 29 at 256; 4 drafts on contexts up to 40000: 62 us at half of an SM's work, 65 at a third, 70 at a quarter).
 static PrefillPlan prefill_plan(int D, int kv_heads, int seqs, int total_q, int q_heads, int max_ctx, int window, bool has_prefix) {
     PrefillPlan p;
     const int rows = D == 256 ? 128 : 256, bn = D == 256 ? 64 : 128, tokens = rows / 128 * (128 / (q_heads / kv_heads)), sms = paged_sm_count();
@@ -948,7 +988,7 @@ static PrefillPlan prefill_plan(int D, int kv_heads, int seqs, int total_q, int 
         mean = std::min(mean, keys);
     }
     const double longest = keys / bn, work = std::max(1.0, mean / bn) * pairs;
-    const double piece = std::max(4.0, work / (2.0 * sms));
+    const double piece = std::max(512.0 / bn, work / (2.0 * sms));
     p.chunks = (int)std::max(1.0, std::min(longest / piece, 1024.0));
     p.chunk_tiles = std::max(1, (int)((longest + p.chunks - 1) / p.chunks));
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
@@ -1020,7 +1060,8 @@ static int32_t launch_prefill(cudaStream_t s, PrefillArgs a) {
     paged_prefill_kernel<D, FEAT><<<a.tiles * a.c.kv_heads * a.chunks, C::THREADS, C::TOTAL, s>>>(qm, km, vm, a);
     LTHN_CUDA_TRY(cudaGetLastError());
     if (a.chunks > 1) {
-        paged_prefill_join_kernel<D><<<dim3(a.tiles, a.c.kv_heads, C::ROWS * (D / 8) / 256), 256, 0, s>>>(a);
+        if (a.chunks <= 8) paged_prefill_join_kernel<D, 1><<<dim3(a.tiles, a.c.kv_heads, C::ROWS / 32 * (D / 64)), 256, 0, s>>>(a);
+        else paged_prefill_join_kernel<D, 8><<<dim3(a.tiles, a.c.kv_heads, C::ROWS / 32 * (D / 8)), 256, 0, s>>>(a);
         LTHN_CUDA_TRY(cudaGetLastError());
     }
     return LTHN_OK;
