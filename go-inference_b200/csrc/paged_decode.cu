@@ -7,15 +7,17 @@
 // heads per kv head it does not on the FMA pipe (G/2 multiply-adds per byte), so the products run on mma.sync with the query heads
 // as the M rows, where up to 16 heads cost what one costs.
 //
-// Work. The pieces (64 keys) of all (row, kv head, bundle of query heads) triples form one list, row by row; CTA c of C takes pieces
-// [U c / C, U (c+1) / C) of the U, so every CTA has the same work whatever the lengths are, and no host knowledge of
-// them is needed. A triple that lies within one CTA is finished there; otherwise each CTA that holds part of it leaves (max, sum,
-// unnormalised output) in its slot of the workspace - a CTA has at most two such parts, its first and its last - and
-// a second kernel joins them.
+// Work. The pieces (64 keys) of all (row, kv head, bundle of query heads) triples form one list, row by row, in which a triple begins with
+// a unit for its start; CTA c of C takes units [U c / C, U (c+1) / C) of the U, so every CTA has the same work whatever the
+// lengths are, and no host knowledge of them is needed. (Without the start's unit the CTAs with many short
+// triples came last: 32 rows of 257 to 4608 keys, first CTA done after 66 us, last after 99.) A triple that lies within one CTA
+// is finished there; otherwise each CTA that holds part of it leaves (max, sum, unnormalised output) in its slot of the workspace
+// - a CTA has at most two such parts, its first and its last - and a second kernel joins them.
 //
 // A warp owns 16 keys of each piece and runs on its own: its own ring of shared-memory stages filled by its own cp.async (16 bytes,
 // rows padded by 16 bytes so that ldmatrix is free of bank conflicts), its own running maximum, sum and output; the
-// four warps meet at the end of a triple only. Rows outside the visible range are filled with zeros instead of
+// four warps meet at the end of a triple only, in the one stage of their rings that the next triple's first keys, already
+// on their way then, leave free. Rows outside the visible range are filled with zeros instead of
 // read: they may hold NaN, which a weight of zero would not silence.
 //
 // Types. K and V are exact in bf16. Bundles of up to 8 heads leave half of the 16 MMA rows free, and the free rows carry
@@ -45,7 +47,7 @@ struct DecodeArgs {
     int ctas;
     float* part;          // [2*ctas][HB][D] unnormalised outputs
     float2* ml;           // [2*ctas][HB] maximum (log2 units) and sum
-    int2* desc;           // [rows][kv_heads*nb] first and last CTA of a triple that several CTAs hold, (-1, .) otherwise
+    int64_t* base;        // [rows + 1] units before each row, and of all (written where there are more rows than the join scans)
 };
 
 constexpr int DEC_WARPS = 4;
@@ -64,13 +66,24 @@ struct DecCfg {
     static constexpr int RING = DEC_WARPS * NST * STAGE;
     static constexpr size_t SMEM = (size_t)RING + Q_BYTES;
     static constexpr int CTAS_PER_SM = D == 256 ? 1 : 2;
-    static_assert(HB * D * 4 <= NST * STAGE, "a warp's ring holds its output for the join");
+    static_assert((SMEM + 2048) * CTAS_PER_SM <= 233472, "shared memory of an SM");
+    static_assert(HB * D * 4 <= STAGE, "a stage holds a warp's output");
 };
 
 __device__ __forceinline__ KeyTiles decode_tiles(const DecodeArgs& a, int row) {
     const int len = paged_length(a.c, a.lens[row]);
     return key_tiles<DEC_TILE>(len - 1, len - 1, len, a.o.prefix ? a.o.prefix[row] : 0, a.o.window);
 }
+
+// Units of a triple of n pieces: its start and end cost about what two pieces cost (32 rows of 257 to 4608 keys: 97.8 us with 1, 96.6 with 2, 96.9 with 3).
+constexpr int DEC_START = 2;
+__device__ __forceinline__ int decode_units(int n) { return n > 0 ? n + DEC_START : 0; }
+// n / d for n >= 0, d > 0: in 32 bits where they fit (a 64-bit division is a long call, and it stands before a CTA's first load)
+__device__ __forceinline__ int64_t decode_div(int64_t n, int64_t d) {
+    return ((n | d) >> 32) == 0 ? (int64_t)((uint32_t)n / (uint32_t)d) : n / d;
+}
+// the CTA that holds unit x
+__device__ __forceinline__ int decode_cta_of(int64_t x, int64_t U, int ctas) { return (int)decode_div((x + 1) * ctas - 1, U); }
 
 // capped, biased score in log2 units. x: the raw product; in: scale / cap or scale * log2 e; cap, slope: times log2 e
 __device__ __forceinline__ float decode_score(float x, float in, float cap, float slope, int gap) {
@@ -79,12 +92,22 @@ __device__ __forceinline__ float decode_score(float x, float in, float cap, floa
     return fmaf(-slope, (float)abs(gap), x);
 }
 
+// part of a triple
+struct DecSeg {
+    int row, kvh, bundle;
+    int len, prefix, lo;  // visible: key < prefix, or lo <= key < len
+    KeyTiles kt;
+    int i0, i1;           // pieces
+};
+
 template <int D, int MODE>
 __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) paged_decode_kernel(const DecodeArgs a) {
     using C = DecCfg<D, MODE>;
     constexpr int HB = C::HB, NST = C::NST, PITCH = C::PITCH;
     constexpr int KS = D / 16;                    // k-steps of q.k
     constexpr int ND = D / 8;                     // output n-tiles
+    constexpr int NR = MODE == DEC_BF16_16 ? 2 : 1;   // head rows of a thread
+    constexpr float LOG2E = 1.4426950408889634f;
     extern __shared__ __align__(128) unsigned char dec_smem[];
     __shared__ float s_m[DEC_WARPS][16], s_l[DEC_WARPS][16];
     __shared__ int s_scan[DEC_WARPS];
@@ -98,20 +121,25 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
     const int triples = a.c.kv_heads * a.nb;      // per row
 
     pdl_trigger();
-    // ---- this CTA's pieces -----------------------------------------------------------------------
-    int incl, mine = tid < a.rows ? decode_tiles(a, tid).n : 0;
+    // ---- this CTA's units ------------------------------------------------------------------------------
+    auto units_of = [&](int r) { return r < a.rows ? decode_units(decode_tiles(a, r).n) : 0; };
+    int incl, mine = units_of(tid);
     int total = paged_block_scan<DEC_WARPS>(mine, incl, s_scan);
-    int64_t U = total;                            // in tiles of rows first, times the triples of a row
+    int64_t U = total;                            // per triple of a row first
+    const bool note = a.rows > DEC_THREADS && blockIdx.x == 0;   // the join looks them up
+    if (note) a.base[tid] = incl - mine;
     for (int r0 = DEC_THREADS; r0 < a.rows; r0 += DEC_THREADS) {
-        const int r = r0 + tid;
         int x;
-        U += paged_block_scan<DEC_WARPS>(r < a.rows ? decode_tiles(a, r).n : 0, x, s_scan);
+        const int n = units_of(r0 + tid), more = paged_block_scan<DEC_WARPS>(n, x, s_scan);
+        if (note && r0 + tid < a.rows) a.base[r0 + tid] = U + x - n;
+        U += more;
     }
+    if (note && tid == 0) a.base[a.rows] = U;
     U *= triples;
-    const int ctas = (int)min((int64_t)a.ctas, U);   // none of them without a piece
+    const int ctas = (int)min((int64_t)a.ctas, U);   // none of them without a unit
     if ((int)blockIdx.x >= ctas) return;
-    const int64_t u0 = U * blockIdx.x / ctas, u1 = U * (blockIdx.x + 1) / ctas;
-    // the row that holds piece u0
+    const int64_t u0 = decode_div(U * blockIdx.x, ctas), u1 = decode_div(U * (blockIdx.x + 1), ctas);
+    // the row that holds unit u0
     int64_t base = 0;
     int row = 0;
     for (int r0 = 0;;) {
@@ -119,119 +147,210 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
             if (mine > 0 && (base + incl) * triples > u0 && (base + incl - mine) * triples <= u0) { s_row = r0 + tid; s_base = incl - mine; }
             __syncthreads();
             row = s_row;
-            base = (base + s_base) * triples;     // first piece of the row
+            base = (base + s_base) * triples;     // first unit of the row
             break;
         }
         base += total;
         r0 += DEC_THREADS;
-        mine = r0 + tid < a.rows ? decode_tiles(a, r0 + tid).n : 0;
+        mine = units_of(r0 + tid);
         total = paged_block_scan<DEC_WARPS>(mine, incl, s_scan);
     }
-    constexpr float LOG2E = 1.4426950408889634f;
     const float s_in = a.o.softcap > 0.f ? a.o.scale / a.o.softcap : a.o.scale * LOG2E, s_cap = a.o.softcap * LOG2E;
 
     int64_t u = u0;
-    while (u < u1 && row < a.rows) {
-        const KeyTiles kt = decode_tiles(a, row);
-        if (kt.n == 0) { row++; continue; }
-        const int v = (int)(u - base);            // piece within the row
-        const int triple = v / kt.n, i0 = v - triple * kt.n;
-        const int count = (int)min((int64_t)(kt.n - i0), u1 - u);
-        const int kvh = triple / a.nb, bundle = triple - kvh * a.nb;
-        const int len = paged_length(a.c, a.lens[row]);
-        const int pos = len - 1;
-        const int prefix = a.o.prefix ? min(max(a.o.prefix[row], 0), len) : 0;
-        const int lo = a.o.window > 0 ? max(0, len - a.o.window) : 0;
-        const int h0 = kvh * a.G + bundle * HB;   // first query head
-        const int nh = min(HB, a.G - bundle * HB);
-        const uint16_t* kbase = a.c.k + kvh * a.c.head_stride;
-        const uint16_t* vbase = a.c.v + kvh * a.c.head_stride;
-        const int32_t* trow = a.c.table + (int64_t)row * a.c.table_stride;
+    auto next_seg = [&](DecSeg& d) {              // the next part of a triple; false: there is none
+        while (u < u1 && row < a.rows) {
+            const KeyTiles kt = decode_tiles(a, row);
+            const int w = decode_units(kt.n);
+            if (w == 0) { row++; continue; }
+            const int64_t in_row = u - base;
+            const int triple = (int)decode_div(in_row, w), v = (int)(in_row - (int64_t)triple * w), take = (int)min((int64_t)(w - v), u1 - u);
+            u += take;
+            const int at = row;
+            if (u - base >= (int64_t)w * triples) { base += (int64_t)w * triples; row++; }
+            d.i0 = max(v - DEC_START, 0);
+            d.i1 = max(v + take - DEC_START, 0);
+            if (d.i0 >= d.i1) continue;           // its start alone: the next CTA begins it
+            d.row = at;
+            d.kvh = triple / a.nb;
+            d.bundle = triple - d.kvh * a.nb;
+            d.len = paged_length(a.c, a.lens[at]);
+            d.prefix = a.o.prefix ? min(max(a.o.prefix[at], 0), d.len) : 0;
+            d.lo = a.o.window > 0 ? max(0, d.len - a.o.window) : 0;
+            d.kt = kt;
+            return true;
+        }
+        return false;
+    };
 
-        __syncthreads();                          // the ring and the query area are free
-        // ---- loads: piece i of the triple into stage i % NST ---------------------------------------
-        // lanes 0-15 keep the page of "their" key of the next piece to be loaded, fetched one piece ahead
-        auto my_key = [&](int i) {                // -1: not visible (its row is zeros)
-            const int key = kt.tile(i) * DEC_TILE + warp * DEC_WK + lane;
-            return lane < DEC_WK && key < len && (key < prefix || key >= lo) ? key : -1;
-        };
-        auto page_of = [&](int i) {
-            const int key = i < i0 + count ? my_key(i) : -1;
-            return key >= 0 ? trow[paged_entry(a.c, key)] : 0;
-        };
-        auto issue = [&](int i, int page) {
-            if (i < i0 + count) {
-                const int key = my_key(i);
-                const int64_t off = key >= 0 ? paged_offset(a.c, page, paged_row(a.c, key)) : -1;
-                constexpr int CPR = D / 8;        // 16-byte chunks per row
-                constexpr int RPI = 32 / CPR > 0 ? 32 / CPR : 1;   // rows per instruction
-                const uint32_t st = ring + (i % NST) * C::STAGE;
-                const int c = lane % CPR;
+    // ---- loads: piece i of a part goes to stage (sb + i - i0) % NST of this warp's ring, where sb counts the pieces before ------
+    // lanes 0-15 keep the page of their key of the next piece to be loaded, fetched one piece ahead
+    DecSeg S, N;                                  // the part at work, and the one after
+    int sb = 0;
+    auto my_key = [&](const DecSeg& d, int i) {   // -1: not visible (its row is zeros)
+        const int key = d.kt.tile(i) * DEC_TILE + warp * DEC_WK + lane;
+        return i < d.i1 && lane < DEC_WK && key < d.len && (key < d.prefix || key >= d.lo) ? key : -1;
+    };
+    auto page_of = [&](const DecSeg& d, int i) {
+        const int key = my_key(d, i);
+        return key >= 0 ? a.c.table[(int64_t)d.row * a.c.table_stride + paged_entry(a.c, key)] : 0;
+    };
+    auto issue = [&](const DecSeg& d, int first, int i, int page) {
+        if (i < d.i1) {
+            const int key = my_key(d, i);
+            const int64_t off = key >= 0 ? paged_offset(a.c, page, paged_row(a.c, key)) : -1;
+            const uint16_t* kbase = a.c.k + d.kvh * a.c.head_stride;
+            const uint16_t* vbase = a.c.v + d.kvh * a.c.head_stride;
+            constexpr int CPR = D / 8;            // 16-byte chunks per row
+            constexpr int RPI = 32 / CPR > 0 ? 32 / CPR : 1;   // rows per instruction
+            const uint32_t st = ring + ((first + i - d.i0) % NST) * C::STAGE;
+            const int c = lane % CPR;
 #pragma unroll
-                for (int r0 = 0; r0 < DEC_WK; r0 += RPI) {
-                    const int r = r0 + (RPI > 1 ? lane / CPR : 0);
-                    const int64_t o = __shfl_sync(0xffffffffu, off, r);
-                    const int64_t e = (o < 0 ? 0 : o) + c * 8;
-                    const int n = o < 0 ? 0 : 16;
-                    cp_async16_zfill(st + r * PITCH + c * 16, kbase + e, n);
-                    cp_async16_zfill(st + (DEC_WK + r) * PITCH + c * 16, vbase + e, n);
-                }
+            for (int r0 = 0; r0 < DEC_WK; r0 += RPI) {
+                const int r = r0 + (RPI > 1 ? lane / CPR : 0);
+                const int64_t o = __shfl_sync(0xffffffffu, off, r);
+                const int64_t e = (o < 0 ? 0 : o) + c * 8;
+                const int n = o < 0 ? 0 : 16;
+                cp_async16_zfill(st + r * PITCH + c * 16, kbase + e, n);
+                cp_async16_zfill(st + (DEC_WK + r) * PITCH + c * 16, vbase + e, n);
             }
-            paged_cp_commit();
-        };
-        int page = page_of(i0);
-#pragma unroll
+        }
+        paged_cp_commit();
+    };
+    int page = 0;
+    auto begin = [&](const DecSeg& d, int first) {   // the first NST - 1 pieces
+        page = page_of(d, d.i0);
+#pragma unroll 1
         for (int s = 0; s < NST - 1; s++) {
-            const int next = page_of(i0 + s + 1);
-            issue(i0 + s, page);
+            const int next = page_of(d, d.i0 + s + 1);
+            issue(d, first, d.i0 + s, page);
             page = next;
         }
-        // ---- queries -----------------------------------------------------------------------------
-        for (int i = tid; i < HB * (D / 8); i += DEC_THREADS) {
-            const int h = i / (D / 8), c = i - h * (D / 8);
+    };
+    // queries of a part: this thread's chunks of 8 elements; f32 ones as three bf16 parts
+    constexpr int NQ = (HB * (D / 8) + DEC_THREADS - 1) / DEC_THREADS;
+    constexpr int QW = MODE == DEC_F32_8 ? 8 : 4; // words of a chunk
+    auto load_queries = [&](const DecSeg& d, uint32_t (&x)[NQ][QW]) {
+        const int h0 = d.kvh * a.G + d.bundle * HB, nh = min(HB, a.G - d.bundle * HB);
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            const int i = tid + n * DEC_THREADS, h = i / (D / 8), c = i - h * (D / 8);
+            const int64_t at = d.row * a.q_stride + (int64_t)(h0 + h) * D + c * 8;
+#pragma unroll
+            for (int v = 0; v < QW / 4; v++) {
+                uint4 y = make_uint4(0, 0, 0, 0);
+                if (h < nh) y = MODE == DEC_F32_8 ? *(const uint4*)((const float*)a.q + at + 4 * v) : *(const uint4*)((const uint16_t*)a.q + at);
+                x[n][4 * v] = y.x; x[n][4 * v + 1] = y.y; x[n][4 * v + 2] = y.z; x[n][4 * v + 3] = y.w;
+            }
+        }
+    };
+    auto store_queries = [&](uint32_t (&x)[NQ][QW]) {
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            const int i = tid + n * DEC_THREADS, h = i / (D / 8), c = i - h * (D / 8);
+            if (h >= HB) break;
             unsigned char* dst = q_sm + h * PITCH + c * 16;
             if (MODE == DEC_F32_8) {
-                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (h < nh) {
-                    const float* src = (const float*)a.q + row * a.q_stride + (int64_t)(h0 + h) * D + c * 8;
-                    const float4 p = *(const float4*)src, r = *(const float4*)(src + 4);
-                    x[0] = p.x; x[1] = p.y; x[2] = p.z; x[3] = p.w; x[4] = r.x; x[5] = r.y; x[6] = r.z; x[7] = r.w;
-                }
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) f[e] = __uint_as_float(x[n][e % QW]);
 #pragma unroll
                 for (int part = 0; part < 3; part++) {
                     uint32_t w[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        w[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
-                        x[2 * e] -= __uint_as_float(w[e] << 16);
-                        x[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
+                        w[e] = pack_bf16x2(f[2 * e], f[2 * e + 1]);
+                        f[2 * e] -= __uint_as_float(w[e] << 16);
+                        f[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
                     }
                     *(uint4*)(dst + part * 8 * PITCH) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             } else {
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (h < nh) x = *(const uint4*)((const uint16_t*)a.q + row * a.q_stride + (int64_t)(h0 + h) * D + c * 8);
-                *(uint4*)dst = x;
+                *(uint4*)dst = make_uint4(x[n][0], x[n][1], x[n][2], x[n][3]);
             }
         }
-        __syncthreads();
+    };
+
+    // One round: the next part's first keys set out, the last part's warps meet in the stage they leave free and store it, then the next part
+    // is worked through. (One copy of this code: it is long, and a short call waits for its instructions too.)
+    float acc[ND][4], mrun[2], lrun[2];
+    bool have = false;
+    for (int sn = 0;; sn = (sb + S.i1 - S.i0) % NST, have = true) {
+        const bool more = next_seg(N);
+        if (more) begin(N, sn);
+        const int red_at = ((sn + NST - 1) % NST) * C::STAGE;
+        if (have) {
+            float* red = (float*)(dec_smem + warp * NST * C::STAGE + red_at);   // [HB][D]
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                float l = lrun[r];
+                l += __shfl_xor_sync(0xffffffffu, l, 1);
+                l += __shfl_xor_sync(0xffffffffu, l, 2);
+                if (t == 0) { s_m[warp][g + 8 * r] = mrun[r]; s_l[warp][g + 8 * r] = l; }
+            }
+#pragma unroll
+            for (int n = 0; n < ND; n++) {
+                if (MODE == DEC_BF16_16) {
+                    *(float2*)(red + g * D + n * 8 + 2 * t) = make_float2(acc[n][0], acc[n][1]);
+                    *(float2*)(red + (g + 8) * D + n * 8 + 2 * t) = make_float2(acc[n][2], acc[n][3]);
+                } else {
+                    *(float2*)(red + g * D + n * 8 + 2 * t) = make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]);
+                }
+            }
+            __syncthreads();
+        }
+        uint32_t qx[NQ][QW];
+        if (more) load_queries(N, qx);
+        if (have) {
+            const int h0 = S.kvh * a.G + S.bundle * HB, nh = min(HB, a.G - S.bundle * HB);   // first query head, heads
+            const bool whole = S.i1 - S.i0 == S.kt.n;
+            const int slot = 2 * blockIdx.x + (S.i0 > 0 ? 0 : 1);
+            for (int idx = tid; idx < nh * (D / 4); idx += DEC_THREADS) {
+                const int h = idx / (D / 4), d = (idx - h * (D / 4)) * 4;
+                const float m = fmaxf(fmaxf(s_m[0][h], s_m[1][h]), fmaxf(s_m[2][h], s_m[3][h]));
+                const float ref = m == -INFINITY ? 0.f : m;
+                float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < DEC_WARPS; w++) {
+                    const float e = ex2(s_m[w][h] - ref);
+                    const float4 y = *(const float4*)((const float*)(dec_smem + w * NST * C::STAGE + red_at) + h * D + d);
+                    l = fmaf(s_l[w][h], e, l);
+                    x[0] = fmaf(y.x, e, x[0]); x[1] = fmaf(y.y, e, x[1]); x[2] = fmaf(y.z, e, x[2]); x[3] = fmaf(y.w, e, x[3]);
+                }
+                if (whole) {
+                    const float inv = l > 0.f ? 1.0f / l : 0.f;
+                    const int64_t at = S.row * a.out_stride + (int64_t)(h0 + h) * D + d;
+                    if (MODE == DEC_F32_8) *(float4*)((float*)a.out + at) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+                    else *(uint2*)((uint16_t*)a.out + at) = make_uint2(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv));
+                    if (a.lse && d == 0) a.lse[(int64_t)S.row * a.Hq + h0 + h] = (m + log2f(l)) * 0.6931471805599453f;
+                } else {
+                    *(float4*)(a.part + ((int64_t)slot * HB + h) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+                    if (d == 0) a.ml[slot * HB + h] = make_float2(m, l);
+                }
+            }
+        }
+        if (!more) break;
+        store_queries(qx);                                    // (all warps are through with the last part's)
+        S = N;
+        sb = sn;
+        __syncthreads();                                      // the queries are there, the stage is free
+        const int h0 = S.kvh * a.G + S.bundle * HB, nh = min(HB, a.G - S.bundle * HB);
         float slope[2] = {0.f, 0.f};
         if (a.o.slopes) {
             if (g < nh) slope[0] = a.o.slopes[h0 + g] * LOG2E;
             if (HB == 16 && g + 8 < nh) slope[1] = a.o.slopes[h0 + g + 8] * LOG2E;
         }
-
-        float acc[ND][4];
 #pragma unroll
         for (int n = 0; n < ND; n++) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-        float mrun[2] = {-INFINITY, -INFINITY}, lrun[2] = {0.f, 0.f};
-        for (int i = i0; i < i0 + count; i++) {
-            const int next = page_of(i + NST);
+        mrun[0] = mrun[1] = -INFINITY;
+        lrun[0] = lrun[1] = 0.f;
+        for (int i = S.i0; i < S.i1; i++) {
+            const int next = page_of(S, i + NST);
             paged_cp_wait<NST - 2>();
             __syncwarp();                         // piece i has landed for every lane; nobody still reads the stage that is filled next
-            issue(i + NST - 1, page);
+            issue(S, sb, i + NST - 1, page);
             page = next;
-            const uint32_t kst = ring + (i % NST) * C::STAGE, vst = kst + DEC_WK * PITCH;
+            const uint32_t kst = ring + ((sb + i - S.i0) % NST) * C::STAGE, vst = kst + DEC_WK * PITCH;
             const int mi = lane >> 3;
             // ---- scores: c[n][e], n-tile n = keys 8n.., e: row g (e < 2) or g + 8, key 2t + (e & 1) ----
             float c[2][4] = {}, c2[2][4] = {};
@@ -256,7 +375,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
                     mma_bf16_16816(c2[1], qa[0], 0u, qa[2], 0u, kb[2], kb[3]);
                 }
             }
-            const int key0 = kt.tile(i) * DEC_TILE + warp * DEC_WK;
+            const int key0 = S.kt.tile(i) * DEC_TILE + warp * DEC_WK;
             constexpr int NR = MODE == DEC_BF16_16 ? 2 : 1;   // head rows of this thread
             float p[NR][4];                                   // [row][n-tile*2 + key]
             float mx[NR];
@@ -268,8 +387,8 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
                     const int n = e >> 1, x = e & 1, key = key0 + n * 8 + 2 * t + x;
                     float s = c[n][2 * r + x];
                     if (MODE == DEC_F32_8) s += c[n][2 + x] + c2[n][x];
-                    s = decode_score(s, s_in, s_cap, slope[r], pos - key);
-                    p[r][e] = key < len && (key < prefix || key >= lo) ? s : -INFINITY;
+                    s = decode_score(s, s_in, s_cap, slope[r], S.len - 1 - key);
+                    p[r][e] = key < S.len && (key < S.prefix || key >= S.lo) ? s : -INFINITY;
                     mx[r] = fmaxf(mx[r], p[r][e]);
                 }
                 mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
@@ -326,79 +445,39 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
             }
             __syncwarp();                                     // the stage may be refilled
         }
-        paged_cp_wait<0>();
-
-        // ---- join the four warps --------------------------------------------------------------------------
-        __syncwarp();
-        float* red = (float*)(dec_smem + warp * NST * C::STAGE);   // this warp's ring, [HB][D]
-        constexpr int NR = MODE == DEC_BF16_16 ? 2 : 1;
-#pragma unroll
-        for (int r = 0; r < NR; r++) {
-            float l = lrun[r];
-            l += __shfl_xor_sync(0xffffffffu, l, 1);
-            l += __shfl_xor_sync(0xffffffffu, l, 2);
-            if (t == 0) { s_m[warp][g + 8 * r] = mrun[r]; s_l[warp][g + 8 * r] = l; }
-        }
-#pragma unroll
-        for (int n = 0; n < ND; n++) {
-            if (MODE == DEC_BF16_16) {
-                *(float2*)(red + g * D + n * 8 + 2 * t) = make_float2(acc[n][0], acc[n][1]);
-                *(float2*)(red + (g + 8) * D + n * 8 + 2 * t) = make_float2(acc[n][2], acc[n][3]);
-            } else {
-                *(float2*)(red + g * D + n * 8 + 2 * t) = make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]);
-            }
-        }
-        __syncthreads();
-        const bool whole = count == kt.n;
-        const int slot = 2 * blockIdx.x + (i0 > 0 ? 0 : 1);
-        for (int idx = tid; idx < nh * (D / 4); idx += DEC_THREADS) {
-            const int h = idx / (D / 4), d = (idx - h * (D / 4)) * 4;
-            float m = s_m[0][h];
-#pragma unroll
-            for (int w = 1; w < DEC_WARPS; w++) m = fmaxf(m, s_m[w][h]);
-            const float ref = m == -INFINITY ? 0.f : m;
-            float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int w = 0; w < DEC_WARPS; w++) {
-                const float e = ex2(s_m[w][h] - ref);
-                const float4 y = *(const float4*)((const float*)(dec_smem + w * NST * C::STAGE) + h * D + d);
-                l = fmaf(s_l[w][h], e, l);
-                x[0] = fmaf(y.x, e, x[0]); x[1] = fmaf(y.y, e, x[1]); x[2] = fmaf(y.z, e, x[2]); x[3] = fmaf(y.w, e, x[3]);
-            }
-            if (whole) {
-                const float inv = l > 0.f ? 1.0f / l : 0.f;
-                const int64_t at = row * a.out_stride + (int64_t)(h0 + h) * D + d;
-                if (MODE == DEC_F32_8) *(float4*)((float*)a.out + at) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-                else *(uint2*)((uint16_t*)a.out + at) = make_uint2(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv));
-                if (a.lse && d == 0) a.lse[(int64_t)row * a.Hq + h0 + h] = (m + log2f(l)) * 0.6931471805599453f;
-            } else {
-                *(float4*)(a.part + ((int64_t)slot * HB + h) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
-                if (d == 0) a.ml[slot * HB + h] = make_float2(m, l);
-            }
-        }
-        if (i0 == 0 && tid == 0) {
-            // the CTAs that hold the rest: the last piece u - i0 + n - 1 lies in CTA ceil((u + n) C / U) - 1
-            const int last = (int)(((u + kt.n) * ctas + U - 1) / U) - 1;
-            a.desc[(int64_t)row * triples + triple] = make_int2(whole ? -1 : (int)blockIdx.x, last);
-        }
-        u += count;
-        if (u - base >= (int64_t)kt.n * triples) { base += (int64_t)kt.n * triples; row++; }
     }
+    paged_cp_wait<0>();
 }
 
 // Joins the parts of triples that several CTAs hold, and writes the rows that see nothing. One CTA per (row, query head); warp w
-// takes parts w, w+4, ... with a running maximum, four loads in flight.
+// takes parts w, w+4, ... with a running maximum, four loads in flight. Which CTAs those are follows from the lengths, which
+// do not have to be waited for.
 template <int D>
 __global__ void __launch_bounds__(128) paged_decode_join_kernel(const DecodeArgs a, int HB, int out_f32) {
     constexpr int DL = D / 32;
     __shared__ float sm[4], sl[4];
     __shared__ float so[4][D];
+    __shared__ int s_scan[4];
+    __shared__ int s_base;
     const int row = blockIdx.y, qh = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     float* of = (float*)a.out + row * a.out_stride + (int64_t)qh * D;
     uint16_t* ob = (uint16_t*)a.out + row * a.out_stride + (int64_t)qh * D;
-    const int len = a.lens[row];                  // not written by the kernel before: no need to wait for it
-    pdl_wait();
-    if (len <= 0 || a.c.capacity == 0) {
+    const int n = decode_tiles(a, row).n;
+    int64_t base = 0, U = 0;
+    if (a.rows <= 128) {
+        int incl;
+        const int mine = tid < a.rows ? decode_units(decode_tiles(a, tid).n) : 0;
+        U = paged_block_scan<4>(mine, incl, s_scan);
+        if (tid == row) s_base = incl - mine;
+        __syncthreads();
+        base = s_base;
+        pdl_wait();
+    } else {
+        pdl_wait();
+        base = a.base[row];
+        U = a.base[a.rows];
+    }
+    if (n == 0) {
         for (int d = tid; d < D; d += 128) {
             if (out_f32) of[d] = 0.f;
             else ob[d] = 0;
@@ -406,21 +485,25 @@ __global__ void __launch_bounds__(128) paged_decode_join_kernel(const DecodeArgs
         if (a.lse && tid == 0) a.lse[(int64_t)row * a.Hq + qh] = -INFINITY;
         return;
     }
+    const int triples = a.c.kv_heads * a.nb;
+    U *= triples;
+    const int ctas = (int)min((int64_t)a.ctas, U);
     const int kvh = qh / a.G, in = qh - kvh * a.G, bundle = in / HB, h = in - bundle * HB;
-    const int2 ds = a.desc[((int64_t)row * a.c.kv_heads + kvh) * a.nb + bundle];
-    if (ds.x < 0) return;
+    base = base * triples + (int64_t)(kvh * a.nb + bundle) * decode_units(n) + DEC_START;   // the first piece
+    const int first = decode_cta_of(base, U, ctas), last = decode_cta_of(base + n - 1, U, ctas);
+    if (first == last) return;
     float m = -INFINITY, l = 0.f, acc[DL];
 #pragma unroll
     for (int i = 0; i < DL; i++) acc[i] = 0.f;
     constexpr int B = 4;
-    for (int c0 = ds.x + warp; c0 <= ds.y; c0 += 4 * B) {
+    for (int c0 = first + warp; c0 <= last; c0 += 4 * B) {
         float2 ml[B];
         float2 x[B][DL / 2];
 #pragma unroll
         for (int b = 0; b < B; b++) {
             const int c = c0 + 4 * b;
-            const bool live = c <= ds.y;
-            const int64_t at = (int64_t)(2 * (live ? c : c0) + ((live ? c : c0) == ds.x ? 1 : 0)) * HB + h;
+            const bool live = c <= last;
+            const int64_t at = (int64_t)(2 * (live ? c : c0) + ((live ? c : c0) == first ? 1 : 0)) * HB + h;
             ml[b] = live ? a.ml[at] : make_float2(-INFINITY, 0.f);
 #pragma unroll
             for (int i = 0; i < DL / 2; i++) x[b][i] = ((const float2*)(a.part + at * D))[lane + 32 * i];
@@ -468,19 +551,22 @@ __global__ void __launch_bounds__(128) paged_decode_join_kernel(const DecodeArgs
 static int decode_mode(int dtype, int G) { return dtype == LTHN_DTYPE_F32 ? DEC_F32_8 : G <= 8 ? DEC_BF16_8 : DEC_BF16_16; }
 static int decode_bundle(int mode) { return mode == DEC_BF16_16 ? 16 : 8; }
 
-struct DecodePlan { int mode, HB, nb, ctas; size_t part, ml, desc, total; };
-static DecodePlan decode_plan(int D, int kv_heads, int rows, int q_heads, int dtype) {
+struct DecodePlan { int mode, HB, nb, ctas; size_t part, ml, base, total; };
+// capacity: the most keys a row can have
+static DecodePlan decode_plan(int D, int kv_heads, int rows, int q_heads, int dtype, int capacity) {
     DecodePlan p;
     const int G = q_heads / kv_heads;
     p.mode = decode_mode(dtype, G);
     p.HB = decode_bundle(p.mode);
     p.nb = (G + p.HB - 1) / p.HB;
-    p.ctas = paged_sm_count() * (D == 256 ? 1 : 2);
+    // as many as run at once; a short table has fewer units than that
+    const int64_t most = (int64_t)rows * kv_heads * p.nb * (((int64_t)capacity + DEC_TILE - 1) / DEC_TILE + DEC_START);
+    p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(paged_sm_count() * (D == 256 ? 1 : 2), most));
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
     p.part = up((size_t)2 * p.ctas * p.HB * D * 4);
     p.ml = up((size_t)2 * p.ctas * p.HB * 8);
-    p.desc = up((size_t)rows * kv_heads * p.nb * 8);
-    p.total = p.part + p.ml + p.desc;
+    p.base = up((size_t)(rows + 1) * 8);
+    p.total = p.part + p.ml + p.base;
     return p;
 }
 
@@ -538,7 +624,7 @@ int32_t lthn_paged_sdpa_decode_workspace(const lthn_paged_kv* cache, int32_t row
     PagedCache c;
     int32_t rc;
     if ((rc = decode_check(cache, rows, q_heads, dtype, &c))) return rc;
-    *bytes = decode_plan(cache->head_dim, cache->kv_heads, rows, q_heads, dtype).total;
+    *bytes = decode_plan(cache->head_dim, cache->kv_heads, rows, q_heads, dtype, c.capacity).total;
     return LTHN_OK;
 }
 
@@ -559,7 +645,7 @@ int32_t lthn_paged_sdpa_decode(void* stream, const lthn_paged_kv* cache, const l
     LTHN_REQUIRE(((a.q_stride | a.out_stride) & 7) == 0, "paged_sdpa_decode: strides must be multiples of 8 elements");
     LTHN_REQUIRE(a.out_stride >= (int64_t)q_heads * D, "paged_sdpa_decode: rows of out would overlap");
     LTHN_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15) == 0, "paged_sdpa_decode: q, out and workspace must be 16-byte aligned");
-    const DecodePlan p = decode_plan(D, cache->kv_heads, rows, q_heads, dtype);
+    const DecodePlan p = decode_plan(D, cache->kv_heads, rows, q_heads, dtype, a.c.capacity);
     LTHN_REQUIRE(workspace_bytes >= p.total, "paged_sdpa_decode: workspace too small");
     if ((rc = paged_check_device(me, "the cache", cache->k))) return rc;
     if ((rc = paged_check_device(me, "workspace", workspace))) return rc;
@@ -567,7 +653,7 @@ int32_t lthn_paged_sdpa_decode(void* stream, const lthn_paged_kv* cache, const l
     a.nb = p.nb; a.ctas = p.ctas;
     a.part = (float*)workspace;
     a.ml = (float2*)((char*)workspace + p.part);
-    a.desc = (int2*)((char*)workspace + p.part + p.ml);
+    a.base = (int64_t*)((char*)workspace + p.part + p.ml);
     a.c.status = device_paged_status_word();
     if (!a.c.status) return fail(LTHN_ERR_CUDA, "paged_sdpa_decode: no device status word");
     if (D == 64) return launch_decode_mode<64>((cudaStream_t)stream, a, p.mode);

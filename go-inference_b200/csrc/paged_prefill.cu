@@ -148,19 +148,6 @@ __device__ __forceinline__ void pf_tma_4d(uint32_t dst, const CUtensorMap* map, 
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar)) : "memory");
 }
-// Asks for the launch of a waiting CTA to be cancelled; the answer (16 bytes) comes by mbarrier. After a refusal no CTA asks again.
-__device__ __forceinline__ void pf_try_cancel(void* answer, uint64_t* bar) {
-    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
-                 ::"r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
-}
-// the block index that now is this CTA's to do, -1: none
-__device__ __forceinline__ int pf_cancelled(const void* answer) {
-    int x;
-    asm volatile("{\n\t.reg .b128 h;\n\t.reg .pred p;\n\tld.shared.b128 h, [%1];\n\tmov.b32 %0, -1;\n\t"
-                 "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
-                 "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n\t}" : "=r"(x) : "r"(smem_u32(answer)) : "memory");
-    return x;
-}
 __device__ __forceinline__ void pf_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -195,25 +182,6 @@ __device__ __forceinline__ void pf_st16(uint32_t taddr, const uint32_t (&r)[16])
           "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
 __device__ __forceinline__ void pf_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// Bounded wait on an mbarrier phase: try_wait parks the thread for a while each time; after 0.2 s of wall time it gives up.
-__device__ __forceinline__ bool pf_wait(uint64_t* bar, uint32_t parity) {
-    uint32_t done = 0;
-    uint64_t t0 = 0;
-    for (uint32_t it = 0;; ++it) {
-        asm volatile("{\n\t.reg .pred p;\n\t"
-                     "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-                     "selp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-        if (done) return true;
-        if ((it & 63) == 63) {
-            uint64_t now;
-            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
-            if (t0 == 0) t0 = now;
-            else if (now - t0 > 200000000ull) return false;
-        }
-    }
-}
 
 // Shared-memory operands in the 128-byte swizzle: slabs of 64 elements, rows 128 bytes apart, 8-row groups 1024.
 // K-major (Q and K): a K = 16 step is 32 bytes further in the slab.
@@ -338,7 +306,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
     // the next item for this warp; false: there are no more
     auto next_item = [&] {
         const int b = items_read & 1;
-        ok = __all_sync(0xffffffffu, pf_wait(&item_full[b], (items_read >> 1) & 1));
+        ok = __all_sync(0xffffffffu, paged_wait(&item_full[b], (items_read >> 1) & 1));
         if (!ok) return false;
         t = items[b];
         __syncwarp();
@@ -367,7 +335,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         int turns = 0, done0 = 0, done1 = 0, last0 = 0, last1 = 0, meets = 0;  // phases the barriers have gone through
         auto pair_sync = [&] {
             pf_arrive(meet);
-            const bool met = __all_sync(0xffffffffu, pf_wait(meet, meets++ & 1));
+            const bool met = __all_sync(0xffffffffu, paged_wait(meet, meets++ & 1));
             ok = ok && met;
         };
         while (ok && next_item()) {
@@ -384,7 +352,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         float m = -INFINITY, l = 0.f;                        // reference maximum (units of the scores), sum relative to it
 
         for (int j = two ? 0 : wg; j < n; j += two ? 1 : 2) {
-            ok = __all_sync(0xffffffffu, pf_wait(&s_full[wg], uses & 1));
+            ok = __all_sync(0xffffffffu, paged_wait(&s_full[wg], uses & 1));
             if (!ok) break;
             uses++;
             pf_fence_after();
@@ -424,7 +392,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             mx[0] = max3(mx[0], s[BN - 4], s[BN - 3]);
             mx[1] = max3(mx[1], s[BN - 2], s[BN - 1]);
             if (!two && j > 0) {                             // the row's maximum so far, from the other warpgroup
-                ok = __all_sync(0xffffffffu, pf_wait(&turn[warp & 3], (turns + j - 1) & 1));
+                ok = __all_sync(0xffffffffu, paged_wait(&turn[warp & 3], (turns + j - 1) & 1));
                 if (!ok) break;
                 const float mo = row_max[r];
                 if (mo != m) {                               // it has moved: this warpgroup's sum follows
@@ -448,7 +416,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             }
             if (move && j > 0) {
                 const float alpha = mold == -INFINITY ? 0.f : ex2((mold - mnew) * c1);
-                ok = __all_sync(0xffffffffu, pf_wait(&o_done[qt], ((qt ? done1 : done0) + j - 1) & 1));
+                ok = __all_sync(0xffffffffu, paged_wait(&o_done[qt], ((qt ? done1 : done0) + j - 1) & 1));
                 if (!ok) break;
                 pf_fence_after();
 #pragma unroll
@@ -487,11 +455,11 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             unpack2(add2(sum[0], sum[1]), l0, l1);
             l += l0 + l1;
         }
-        if (ok && n > 0) ok = __all_sync(0xffffffffu, pf_wait(&o_last[qt], (qt ? last1 : last0) & 1));
+        if (ok && n > 0) ok = __all_sync(0xffffffffu, paged_wait(&o_last[qt], (qt ? last1 : last0) & 1));
         int x0 = 0, x1 = D;                                  // output columns of this warpgroup
         if (!two && n > 0) {
             // the two sums of a row meet, relative to the last maximum; each warpgroup stores half of the columns
-            if (ok) ok = __all_sync(0xffffffffu, pf_wait(&turn[warp & 3], (turns + n - 1) & 1));
+            if (ok) ok = __all_sync(0xffffffffu, paged_wait(&turn[warp & 3], (turns + n - 1) & 1));
             const float mo = row_max[r];
             l = m == -INFINITY ? 0.f : l * ex2((m - mo) * c1);
             m = mo;
@@ -560,10 +528,10 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             const bool two = t.two;
             const int n = t.n, units = two ? 2 * n : n;
             if (n == 0) continue;
-            ok = __all_sync(0xffffffffu, pf_wait(q_full, seen & 1));
+            ok = __all_sync(0xffffffffu, paged_wait(q_full, seen & 1));
             auto scores = [&](int u) {
                 const int j = two ? u >> 1 : u, qt = two ? u & 1 : 0, slot = slot0 + k_slot(j), st = slot % ST;
-                ok = __all_sync(0xffffffffu, pf_wait(&full[st], (slot / ST) & 1));
+                ok = __all_sync(0xffffffffu, paged_wait(&full[st], (slot / ST) & 1));
                 if (!ok) return;
                 pf_fence_after();
                 const uint32_t qa = smem + qt * C::Q_BYTES, kb = smem + C::RING + st * C::KV_BYTES, d = tmem + (u & 1) * C::S_COLS;
@@ -579,12 +547,12 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             for (int u = 0; u < units && ok; u++) {
                 const int j = two ? u >> 1 : u, qt = two ? u & 1 : 0, slot = slot0 + v_slot(j), st = slot % ST;
                 const uint32_t vb = smem + C::RING + st * C::KV_BYTES, pa = tmem + (u & 1) * C::S_COLS, d = tmem + 256 + qt * D;
-                ok = __all_sync(0xffffffffu, pf_wait(&full[st], (slot / ST) & 1) && pf_wait(&p_half[u & 1], uses >> (u & 1) & 1));
+                ok = __all_sync(0xffffffffu, paged_wait(&full[st], (slot / ST) & 1) && paged_wait(&p_half[u & 1], uses >> (u & 1) & 1));
                 if (!ok) break;
                 pf_fence_after();
 #pragma unroll
                 for (int x = 0; x < BN / 32; x++) pf_mma_ts(d, pa + x * 8, pf_desc_n(vb + x * 2048, C::SLAB), idesc_o, j > 0 || x > 0);
-                ok = __all_sync(0xffffffffu, pf_wait(&p_full[u & 1], uses >> (u & 1) & 1));
+                ok = __all_sync(0xffffffffu, paged_wait(&p_full[u & 1], uses >> (u & 1) & 1));
                 if (!ok) break;
                 pf_fence_after();
                 uses ^= 1u << (u & 1);
@@ -600,7 +568,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         if (!ok) {
             if (lane == 0) atomicOr(a.wait_status, 1u << 25);
             pf_commit(drain);                                // nothing of this CTA may still run when its memory is given back
-            pf_wait(drain, 0);
+            paged_wait(drain, 0);
         }
         __syncwarp();
     } else {
@@ -656,7 +624,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         };
         auto publish = [&](const PfItem& x) {
             const int b = published & 1;
-            ok = ok && __all_sync(0xffffffffu, pf_wait(&item_empty[b], ((published >> 1) & 1) ^ 1));
+            ok = ok && __all_sync(0xffffffffu, paged_wait(&item_empty[b], ((published >> 1) & 1) ^ 1));
             if (!ok) return;
             if (lane == 0) {
                 items[b] = x;
@@ -671,13 +639,13 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                 if (lane == 0) {
                     pf_fence_async();                        // the last answer has been read
                     mbar_expect_tx(answered, 16);
-                    pf_try_cancel(answer, answered);
+                    paged_try_cancel(answer, answered);
                 }
                 __syncwarp();
-                ok = ok && __all_sync(0xffffffffu, pf_wait(answered, asked & 1));
+                ok = ok && __all_sync(0xffffffffu, paged_wait(answered, asked & 1));
                 if (!ok) return;
                 asked++;
-                const int id = pf_cancelled(answer);
+                const int id = paged_cancelled(answer);
                 __syncwarp();
                 if (id < 0) {
                     x.head = -1;
@@ -710,7 +678,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             return x < NX && rr < BN && key < len && (key < prefix || (key >= lo && key <= qhi)) ? key : -1;
         };
         auto free_slot = [&](int slot) {
-            ok = __all_sync(0xffffffffu, pf_wait(&empty[slot % ST], ((slot / ST) & 1) ^ 1));
+            ok = __all_sync(0xffffffffu, paged_wait(&empty[slot % ST], ((slot / ST) & 1) ^ 1));
             return ok;
         };
         // ---- row by row ----
@@ -798,7 +766,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                 pf_fence_async();
                 while (handed < slot0 + k_slot(0) + 1) pf_arrive(&full[handed++ % ST]);
             }
-            ok = __all_sync(0xffffffffu, pf_wait(q_empty, (seen & 1) ^ 1));
+            ok = __all_sync(0xffffffffu, paged_wait(q_empty, (seen & 1) ^ 1));
             if (!ok) return;
             const int row_tiles = t.two ? 2 : 1;
             if (a.q_box) {                                   // tokens behind the sequence's last are somebody else's, or zeros: never stored
