@@ -8,9 +8,14 @@
 // Every element is read once and written once, so the kernel is bound by memory. A head is D/8 threads: thread j holds
 // elements 4j..4j+3 of either half of the head, which makes both kinds of pairs, (i, i + D/2) and (2i, 2i+1), meet in one
 // thread; the norm needs one shuffle reduction over the head's threads and nothing else crosses threads. One CTA is
-// one token row: its D/2 angles are formed once, by one thread each, and read by all of the row's heads. The angle is the
-// only place where 32 bits are not enough (position 200000 leaves an f32 angle 0.01 off), so it is formed in f64, in
-// turns, reduced there to [-1/2, 1/2], and handed to sincospif.
+// one token row: its D/2 angles are formed once, by one thread each, and read by all of the row's heads. Position, page,
+// angles and norm are a chain of latencies, so what counts is how many rows an SM has at work: the first heads are loaded before
+// position and page are known, and CTAs are small (8190 rows of 64 heads of 128, bf16, 268 MB: 64 us with 4 CTAs of 256 threads per SM,
+// 53.5 us = 5.0 TB/s with 10 of 128; fetching the next row under this one instead: 67 us). For a few rows the chain is all
+// there is, and a row's heads are shared between CTAs (1 row of 16 heads of 256, f32: 3.9 us, shared 3.4; 64 rows of 48 heads
+// of 128, bf16: 3.3, 2.6). The angle is the only place
+// where 32 bits are not enough (position 200000 leaves an f32 angle 0.01 off), so it is formed in f64, in turns, reduced
+// there to [-1/2, 1/2], and handed to sincospif.
 #include "paged.cuh"
 
 #include <algorithm>
@@ -90,123 +95,151 @@ struct AppendArgs {
     int Hq, half_rot, interleaved;
 };
 
-__device__ __forceinline__ void load4(const float* p, float (&x)[4]) {
-    const float4 v = *(const float4*)p;
-    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-}
-__device__ __forceinline__ void load4(const uint16_t* p, float (&x)[4]) {
-    const uint2 v = *(const uint2*)p;
-    x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
-    x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
-}
+// four elements as they lie in memory, and as f32
+template <typename T> struct Four;
+template <> struct Four<float> {
+    typedef float4 raw;
+    static __device__ __forceinline__ void widen(const raw& v, float (&x)[4]) { x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
+};
+template <> struct Four<uint16_t> {
+    typedef uint2 raw;
+    static __device__ __forceinline__ void widen(const raw& v, float (&x)[4]) {
+        x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
+        x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
+    }
+};
 __device__ __forceinline__ void store4(float* p, const float (&x)[4]) { *(float4*)p = make_float4(x[0], x[1], x[2], x[3]); }
 __device__ __forceinline__ void store4(uint16_t* p, const float (&x)[4]) {
     *(uint2*)p = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
 }
 
-constexpr int AP_THREADS = 256;
+constexpr int AP_THREADS = 128;
+constexpr int AP_BATCH = 4;    // heads of a thread whose loads go out together
 
 template <int D, typename TI, typename TQ>
-__global__ void __launch_bounds__(AP_THREADS) paged_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(AP_THREADS, sizeof(TI) == 2 ? 10 : 6) paged_append_kernel(const AppendArgs a) {
     constexpr int TPH = D / 8;                 // threads per head: 8, 16 or 32
     constexpr int HPP = AP_THREADS / TPH;      // heads per pass
-    __shared__ float2 turn[D / 2];             // (cos, sin) of each rotated pair
-    const int row = blockIdx.x, tid = threadIdx.x;
+    typedef typename Four<TI>::raw raw;
+    __shared__ __align__(16) float2 turn[D / 2];   // (cos, sin) of each rotated pair
+    const int row = blockIdx.x, tid = threadIdx.x, j = tid % TPH, heads = a.Hq + 2 * a.c.kv_heads;
     const int seq = a.row_seq[row];
-    if (seq < 0) return;                       // padding row
     const int pos = a.row_pos[row];
+    const TI* q_row = (const TI*)a.q + row * a.q_stride + 4 * j;
+    const TI* k_row = (const TI*)a.k + row * a.k_stride + 4 * j - (int64_t)a.Hq * D;   // so that head h of q, k, v lies at h * D
+    const TI* v_row = (const TI*)a.v + row * a.v_stride + 4 * j - (int64_t)(a.Hq + a.c.kv_heads) * D;
+    raw lo[AP_BATCH], hi[AP_BATCH];            // elements 4j.. of the first and of the second half of this thread's heads
+    auto load = [&](int h0) {
+#pragma unroll
+        for (int b = 0; b < AP_BATCH; b++) {
+            const int h = h0 + b * HPP + tid / TPH;
+            lo[b] = raw{};
+            hi[b] = raw{};
+            if (h < heads) {
+                const TI* src = (h < a.Hq ? q_row : h < a.Hq + a.c.kv_heads ? k_row : v_row) + h * D;
+                lo[b] = *(const raw*)src;
+                hi[b] = *(const raw*)(src + D / 2);
+            }
+        }
+    };
+    load(HPP * AP_BATCH * blockIdx.y);                                   // needs neither position nor page: under way while those are looked up
+    if (seq < 0) return;                       // padding row
     if (seq >= a.c.seqs || pos < 0 || pos >= a.c.capacity) {
         if (tid == 0) atomicOr(a.c.status, LTHN_STATUS_PAGED);
         return;
     }
     const int entry = paged_entry(a.c, pos);
-    const int64_t off = paged_offset(a.c, a.c.table[(int64_t)seq * a.c.table_stride + entry], pos - entry * a.c.page_size);
-    if (off < 0) return;
+    const int page = a.c.table[(int64_t)seq * a.c.table_stride + entry];
     for (int i = tid; i < a.half_rot; i += AP_THREADS) {
         const double turns = (double)pos * a.inv_freq[i] * 0.15915494309189535;  // of a full circle
         float s, c;
         sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
         turn[i] = make_float2(c, s);
     }
+    const int64_t off = paged_offset(a.c, page, pos - entry * a.c.page_size);
+    if (off < 0) return;                       // (the same for all threads)
     __syncthreads();
-    const int j = tid % TPH, heads = a.Hq + 2 * a.c.kv_heads;
+    // What this thread's pairs are multiplied with is the same for all its heads. Pair e: (x[e], y[e]), or of neighbours (x0 x1) (x2 x3)
+    // (y0 y1) (y2 y3).
     const bool norms = a.q_norm || a.k_norm;
-    for (int h0 = 0; h0 < heads; h0 += HPP) {  // the same trip count for all: the reduction below takes every thread
-        const int h = h0 + tid / TPH;
-        const bool live = h < heads, is_q = h < a.Hq, is_v = h >= a.Hq + a.c.kv_heads;
-        const int kh = is_q ? h : is_v ? h - a.Hq - a.c.kv_heads : h - a.Hq;
-        const TI* src = is_q ? (const TI*)a.q + row * a.q_stride : is_v ? (const TI*)a.v + row * a.v_stride : (const TI*)a.k + row * a.k_stride;
-        src += (int64_t)kh * D + 4 * j;
-        float lo[4] = {0.f, 0.f, 0.f, 0.f}, hi[4] = {0.f, 0.f, 0.f, 0.f};  // elements 4j.. of the first and of the second half
-        if (live) {
-            load4(src, lo);
-            load4(src + D / 2, hi);
-        }
-        float ss = 0.f;
-        if (norms) {
+    float2 rot[4];
+    bool turned[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) ss += lo[e] * lo[e] + hi[e] * hi[e];
+    for (int e = 0; e < 4; e++) {
+        const int i = a.interleaved ? 2 * j + (e & 1) + (e >> 1) * (D / 4) : 4 * j + e;
+        turned[e] = i < a.half_rot;
+        rot[e] = turned[e] ? turn[i] : make_float2(1.f, 0.f);
+    }
+    auto rotate = [](float& p, float& q, float2 t) {
+        const float u = p, v = q;
+        p = u * t.x - v * t.y;
+        q = u * t.y + v * t.x;
+    };
+    TQ* q_dst = (TQ*)a.q_out + row * a.q_out_stride + 4 * j;
+    uint16_t* k_dst = a.c.k + off + 4 * j;
+    uint16_t* v_dst = a.c.v + off + 4 * j;
+    for (int h0 = HPP * AP_BATCH * blockIdx.y;;) {                       // the same trip count for all: the reduction takes every thread
 #pragma unroll
-            for (int o = TPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, TPH);
-        }
-        if (!live) continue;
-        if (!is_v) {
-            const float* w = is_q ? a.q_norm : a.k_norm;
-            if (w) {
-                const float r = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
-                float wl[4], wh[4];
-                load4(w + 4 * j, wl);
-                load4(w + 4 * j + D / 2, wh);
+        for (int b = 0; b < AP_BATCH; b++) {
+            const int h = h0 + b * HPP + tid / TPH;
+            const bool live = h < heads, is_q = h < a.Hq, is_v = h >= a.Hq + a.c.kv_heads;
+            float x[4], y[4];
+            Four<TI>::widen(lo[b], x);
+            Four<TI>::widen(hi[b], y);
+            if (norms) {
+                float ss = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; e++) { lo[e] = lo[e] * r * wl[e]; hi[e] = hi[e] * r * wh[e]; }
-            }
-            if (a.interleaved) {
+                for (int e = 0; e < 4; e++) ss = fmaf(x[e], x[e], fmaf(y[e], y[e], ss));
 #pragma unroll
-                for (int e = 0; e < 4; e += 2) {
-                    const int p0 = 2 * j + e / 2, p1 = D / 4 + p0;
-                    if (p0 < a.half_rot) {
-                        const float2 t = turn[p0];
-                        const float x = lo[e], y = lo[e + 1];
-                        lo[e] = x * t.x - y * t.y;
-                        lo[e + 1] = x * t.y + y * t.x;
-                    }
-                    if (p1 < a.half_rot) {
-                        const float2 t = turn[p1];
-                        const float x = hi[e], y = hi[e + 1];
-                        hi[e] = x * t.x - y * t.y;
-                        hi[e + 1] = x * t.y + y * t.x;
-                    }
+                for (int o = TPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, TPH);
+                const float* w = is_q ? a.q_norm : a.k_norm;
+                if (w && live && !is_v) {
+                    const float r = rsqrtf(fmaf(ss, 1.0f / D, a.eps));   // two units in the last place
+                    const float4 wl = *(const float4*)(w + 4 * j), wh = *(const float4*)(w + 4 * j + D / 2);
+                    x[0] *= r * wl.x; x[1] *= r * wl.y; x[2] *= r * wl.z; x[3] *= r * wl.w;
+                    y[0] *= r * wh.x; y[1] *= r * wh.y; y[2] *= r * wh.z; y[3] *= r * wh.w;
                 }
+            }
+            if (!live) continue;
+            if (!is_v) {
+                if (a.interleaved) {
+                    if (turned[0]) rotate(x[0], x[1], rot[0]);
+                    if (turned[1]) rotate(x[2], x[3], rot[1]);
+                    if (turned[2]) rotate(y[0], y[1], rot[2]);
+                    if (turned[3]) rotate(y[2], y[3], rot[3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (turned[e]) rotate(x[e], y[e], rot[e]);
+                }
+            }
+            if (is_q) {
+                TQ* dst = q_dst + h * D;
+                store4(dst, x);
+                store4(dst + D / 2, y);
             } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if (4 * j + e >= a.half_rot) continue;
-                    const float2 t = turn[4 * j + e];
-                    const float x = lo[e], y = hi[e];
-                    lo[e] = x * t.x - y * t.y;
-                    hi[e] = x * t.y + y * t.x;
-                }
+                uint16_t* dst = is_v ? v_dst + (h - a.Hq - a.c.kv_heads) * a.c.head_stride : k_dst + (h - a.Hq) * a.c.head_stride;
+                store4(dst, x);
+                store4(dst + D / 2, y);
             }
         }
-        if (is_q) {
-            TQ* dst = (TQ*)a.q_out + row * a.q_out_stride + (int64_t)kh * D + 4 * j;
-            store4(dst, lo);
-            store4(dst + D / 2, hi);
-        } else {
-            uint16_t* dst = (is_v ? a.c.v : a.c.k) + off + kh * a.c.head_stride + 4 * j;
-            store4(dst, lo);
-            store4(dst + D / 2, hi);
-        }
+        h0 += HPP * AP_BATCH * gridDim.y;
+        if (h0 >= heads) break;
+        load(h0);
     }
 }
 
 template <int D>
 static void launch_append(cudaStream_t s, const AppendArgs& a, int rows, int dtype, int q_dtype) {
     const bool fi = dtype == LTHN_DTYPE_F32, fq = q_dtype == LTHN_DTYPE_F32;
-    if (fi && fq) paged_append_kernel<D, float, float><<<rows, AP_THREADS, 0, s>>>(a);
-    else if (fi) paged_append_kernel<D, float, uint16_t><<<rows, AP_THREADS, 0, s>>>(a);
-    else if (fq) paged_append_kernel<D, uint16_t, float><<<rows, AP_THREADS, 0, s>>>(a);
-    else paged_append_kernel<D, uint16_t, uint16_t><<<rows, AP_THREADS, 0, s>>>(a);
+    // Rows that leave SMs idle are shared between CTAs, AP_BATCH heads of a thread each; each forms the row's angles anew.
+    constexpr int share = AP_THREADS / (D / 8) * AP_BATCH;
+    const int shares = (a.Hq + 2 * a.c.kv_heads + share - 1) / share;
+    const dim3 grid(rows, (int64_t)rows * shares <= 4 * 148 ? shares : 1);
+    if (fi && fq) paged_append_kernel<D, float, float><<<grid, AP_THREADS, 0, s>>>(a);
+    else if (fi) paged_append_kernel<D, float, uint16_t><<<grid, AP_THREADS, 0, s>>>(a);
+    else if (fq) paged_append_kernel<D, uint16_t, float><<<grid, AP_THREADS, 0, s>>>(a);
+    else paged_append_kernel<D, uint16_t, uint16_t><<<grid, AP_THREADS, 0, s>>>(a);
 }
 
 }  // namespace lthn

@@ -384,6 +384,9 @@ class Buf:
         check(lib().lthn_memcpy_d2h(out.ctypes.data, self.ptr, out.nbytes, stream.h if stream else None))
         return out
 
+    def data_ptr(self) -> int:
+        return self.ptr
+
     def zero(self, stream=None):
         check(lib().lthn_memset(self.ptr, 0, self.nbytes, stream.h if stream else None))
 
@@ -539,9 +542,7 @@ def qmv_host(x_bf16: np.ndarray, packed: np.ndarray, scales: np.ndarray, biases:
 # cudaStream_t as an int.
 
 def _p(x):
-    if x is None:
-        return None
-    return x.ptr if isinstance(x, Buf) else x.data_ptr()
+    return None if x is None else x.data_ptr()
 
 
 def _raw(stream):
