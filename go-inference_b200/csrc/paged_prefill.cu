@@ -5,10 +5,10 @@
 // 4*D flops per visible (query, key) pair against 4*D bytes of K and V per key and tile of query rows: bound by the tensor pipe
 // for prompts, by HBM for a few rows against a long context.
 //
-// Rows. The query rows of a tile are the (token, query head) pairs of one kv head, token by token, as many whole tokens as 128
-// rows hold, so the heads that share K and V share their loads, a chunk of a few tokens still fills a tile, and the
-// queries of a tile are one TMA box per 64 head dimensions. A CTA works on one or two tiles of 128 rows (two: two accumulators of head_dim columns fit the tensor memory beside two score tiles for head_dim 64 and 128) and on
-// BN keys at a time.
+// Rows. The query rows of a tile are the (token, query head) pairs of one kv head, token by token, as many whole tokens as
+// 128 rows hold, so the heads that share K and V share their loads, a chunk of a few tokens still fills a tile, and the
+// queries of a tile are one TMA box per 64 head dimensions. A CTA works on BN keys at a time and on one tile of 128 rows,
+// or two for head_dim 64 and 128, where two accumulators fit the tensor memory beside two score tiles.
 //
 //   softmax warps   two warpgroups, one per score buffer, one thread per row: tcgen05.ld the row's BN scores, mask, maximum, ex2,
 //                   sum - all within the thread - and tcgen05.st the weights as bf16 over the scores they came from.
@@ -18,12 +18,12 @@
 //                   works on one buffer while the other's softmax runs. With two row tiles the buffers belong to them;
 //                   with one they alternate over its key tiles, and the warpgroups pass the running maximum of a row to one
 //                   another (the sums stay apart until the end), which leaves only load and maximum in sequence.
-//   loaders         three warps fetch the queries of an item and fill a ring of K and V tiles in the 128-byte swizzle. Where the page size is a multiple of 8 (the
-//                   swizzle's row group) by tiled TMA, one box per page, 64 head dimensions and gcd(page size, BN) rows. V rows
-//                   that nobody sees must be zeros (they may hold NaN, which a weight of zero would not silence), so a V
-//                   tile with such rows - the last of a sequence, the first of a window - and pools of other page
-//                   sizes come row by row with cp.async of 16 bytes, zero-filled; unseen K rows may hold anything, their
-//                   scores are replaced. 8192 tokens of 32 heads: 1007 us with cp.async throughout, 541 us with TMA.
+//   loaders         three warps fetch the queries of an item and fill a ring of K and V tiles in the 128-byte swizzle. Where
+//                   the page size is a multiple of 8 (the swizzle's row group) by tiled TMA, one box per page, 64 head
+//                   dimensions and gcd(page size, BN) rows. V rows that nobody sees must be zeros (they may hold NaN,
+//                   which a weight of zero would not silence), so a V tile with such rows - the last of a sequence, the
+//                   first of a window - and pools of other page sizes come row by row with cp.async of 16 bytes,
+//                   zero-filled; unseen K rows may hold anything, their scores are replaced. 8192 tokens of 32 heads: 1007 us with cp.async throughout, 541 us with TMA.
 //
 // The running maximum is only moved when a row's grew by more than 2^8: until then weights are up to 2^8, which neither
 // their bf16 rounding (relative) nor the f32 sums mind, and O in tensor memory needs no correction. A move multiplies
@@ -33,7 +33,7 @@
 // run as there are SMs: a CTA that is through with loading an item cancels the launch of a waiting one
 // (clusterlaunchcontrol) and takes its item over, so barriers, tensor memory and pipeline stay up and the loads of the next item run under
 // the last products and the output of this one. One of the loader warps does this and publishes the item to the other
-// roles. (One CTA per item spent 7 us of each on its start and end, 8192 tokens of 32 heads: XXX us against YYY. A fixed
+// roles. (One CTA per item spent 7 us of each on its start and end: 7 packed chunks of up to 1500 tokens took 201 us against 186. A fixed
 // even share per CTA of a list weighted by cost loses more than that: what a key tile costs depends on its mask and on who shares it in L2.)
 // Where there are few items the keys of a tile are cut into chunks, which leave (maximum, sum, unnormalised output)
 // in the workspace for a second kernel to join.
@@ -95,16 +95,28 @@ struct PfItem {
     int i0, n;           // key tiles [i0, i0 + n) of kt; n = 0 where nobody sees anything
     int part;            // place in the workspace, -1: not cut, the output is final
 };
+// What a call says of a sequence.
+struct PfSeq { int first, tokens, len, prefix; };
+__device__ __forceinline__ PfSeq prefill_seq(const PrefillArgs& a, int s) {
+    PfSeq q = {0, 0, 0, 0};
+    if (s >= a.seqs) return q;
+    const int len = a.lens[s], prefix = a.o.prefix ? a.o.prefix[s] : 0;
+    const int2 span = prefill_span(a, s);
+    q.first = span.x;
+    q.tokens = span.y;
+    q.len = paged_length(a.c, len);
+    q.prefix = min(max(prefix, 0), q.len);
+    return q;
+}
 template <int NQ, int BN>
-__device__ __forceinline__ PfItem prefill_tile(const PrefillArgs& a, int seq, int tile) {
+__device__ __forceinline__ PfItem prefill_tile(const PrefillArgs& a, const PfSeq& q, int seq, int tile) {
     PfItem t;
-    const int2 span = prefill_span(a, seq);
     t.seq = seq;
-    t.first = span.x;
-    t.tokens = span.y;
-    t.len = paged_length(a.c, a.lens[seq]);
+    t.first = q.first;
+    t.tokens = q.tokens;
+    t.len = q.len;
     t.pos0 = t.len - t.tokens;
-    t.prefix = a.o.prefix ? min(max(a.o.prefix[seq], 0), t.len) : 0;
+    t.prefix = q.prefix;
     t.tok0 = tile * NQ * a.tokens;
     t.qlo = t.pos0 + t.tok0;
     t.qhi = t.pos0 + min(t.tok0 + NQ * a.tokens, t.tokens) - 1;
@@ -279,6 +291,9 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
     static_assert((2 * ST + 23) * 8 + 8 <= 320 && 336 + 2 * sizeof(PfItem) <= 512, "barriers and items");
 
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    pdl_trigger();                                           // of the join, which waits for the end of this grid
+    PfSeq seq_here = {0, 0, 0, 0};                           // the last warp, which finds the items: sequence `lane`
+    if (warp == C::WARPS - 1) seq_here = prefill_seq(a, lane);
     if (tid == 0) {
         for (int s = 0; s < ST; s++) { mbar_init(&full[s], 96); mbar_init(&empty[s], 1); }
         for (int b = 0; b < 2; b++) {
@@ -339,181 +354,181 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             ok = ok && met;
         };
         while (ok && next_item()) {
-        const bool two = t.two;
-        const int n = t.n, i0 = t.i0, qt = two ? wg : 0, len = t.len;
-        const int token = t.tok0 + qt * a.tokens + r_token;  // of the sequence
-        const bool live = r_token < a.tokens && token < t.tokens;
-        const int head = t.head * a.G + r_head;
-        const int qpos = t.pos0 + token;
-        // visible: key < pre, or klo <= key < khi
-        const int pre = t.prefix, khi = min(qpos + 1, len), klo = a.o.window > 0 ? qpos - a.o.window + 1 : 0;
-        const float slope = (FEAT & 2) && live ? a.o.slopes[head] * LOG2E : 0.f;
-        const uint32_t o_addr = lanes + 256 + qt * D;
-        float m = -INFINITY, l = 0.f;                        // reference maximum (units of the scores), sum relative to it
+            const bool two = t.two;
+            const int n = t.n, i0 = t.i0, qt = two ? wg : 0, len = t.len;
+            const int token = t.tok0 + qt * a.tokens + r_token;  // of the sequence
+            const bool live = r_token < a.tokens && token < t.tokens;
+            const int head = t.head * a.G + r_head;
+            const int qpos = t.pos0 + token;
+            // visible: key < pre, or klo <= key < khi
+            const int pre = t.prefix, khi = min(qpos + 1, len), klo = a.o.window > 0 ? qpos - a.o.window + 1 : 0;
+            const float slope = (FEAT & 2) && live ? a.o.slopes[head] * LOG2E : 0.f;
+            const uint32_t o_addr = lanes + 256 + qt * D;
+            float m = -INFINITY, l = 0.f;                        // reference maximum (units of the scores), sum relative to it
 
-        for (int j = two ? 0 : wg; j < n; j += two ? 1 : 2) {
-            ok = __all_sync(0xffffffffu, paged_wait(&s_full[wg], uses & 1));
-            if (!ok) break;
-            uses++;
-            pf_fence_after();
-            float s[BN];
-#pragma unroll
-            for (int x = 0; x < BN; x += 32) pf_ld32(s_addr + x, s + x);
-            pf_ld_wait();
-            const int k0 = t.kt.tile(i0 + j) * BN;
-            if (FEAT & 1) {
-                // cap tanh(x scale / cap) = cap (1 - 2 / (1 + e^(2 x scale / cap)))
-#pragma unroll
-                for (int x = 0; x < BN; x++) s[x] = fmaf(-2.0f * cap2, rcp_approx(1.0f + ex2(s[x] * cin)), cap2);
-            }
-            if (FEAT & 2) {
-                const float gap = (float)(qpos - k0);
-#pragma unroll
-                for (int x = 0; x < BN; x++) s[x] = fmaf(-slope, fabsf(gap - (float)x), FEAT & 1 ? s[x] : s[x] * cin);
-            }
-            const bool all = !live || k0 + BN <= pre || (k0 >= klo && k0 + BN <= khi);
-            if (!__all_sync(0xffffffffu, all)) {
-                const int p = pre - k0, lo = klo - k0, hi = khi - k0;
-#pragma unroll
-                for (int x0 = 0; x0 < BN; x0 += 32) {
-                    const uint32_t seen = low_bits(p - x0) | (low_bits(hi - x0) & ~low_bits(lo - x0));
-#pragma unroll
-                    for (int x = 0; x < 32; x++) s[x0 + x] = seen >> x & 1 ? s[x0 + x] : -INFINITY;
-                }
-            }
-            float mx[4];                                     // four chains
-#pragma unroll
-            for (int x = 0; x < 4; x++) mx[x] = max3(s[x], s[x + 4], s[x + 8]);
-#pragma unroll
-            for (int x = 12; x + 8 <= BN; x += 8)
-#pragma unroll
-                for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], s[x + e], s[x + 4 + e]);
-            static_assert((BN - 12) % 8 == 4, "the last four scores");
-            mx[0] = max3(mx[0], s[BN - 4], s[BN - 3]);
-            mx[1] = max3(mx[1], s[BN - 2], s[BN - 1]);
-            if (!two && j > 0) {                             // the row's maximum so far, from the other warpgroup
-                ok = __all_sync(0xffffffffu, paged_wait(&turn[warp & 3], (turns + j - 1) & 1));
+            for (int j = two ? 0 : wg; j < n; j += two ? 1 : 2) {
+                ok = __all_sync(0xffffffffu, paged_wait(&s_full[wg], uses & 1));
                 if (!ok) break;
-                const float mo = row_max[r];
-                if (mo != m) {                               // it has moved: this warpgroup's sum follows
-                    l = m == -INFINITY ? 0.f : l * ex2((m - mo) * c1);
-                    m = mo;
-                }
-                __syncwarp();
-            }
-            const float mnew = live ? max3(fmaxf(m, mx[0]), mx[1], fmaxf(mx[2], mx[3])) : m;   // a row without a query holds anything
-            const bool move = __any_sync(0xffffffffu, (mnew - m) * c1 > 8.0f);
-            const float mold = m;
-            if (move) {
-                l = m == -INFINITY ? 0.f : l * ex2((m - mnew) * c1);
-                m = mnew;
-            }
-            if (!two) {
-                row_max[r] = m;
-                __syncwarp();
-                if (lane == 0) pf_arrive(&turn[warp & 3]);
-                __syncwarp();
-            }
-            if (move && j > 0) {
-                const float alpha = mold == -INFINITY ? 0.f : ex2((mold - mnew) * c1);
-                ok = __all_sync(0xffffffffu, paged_wait(&o_done[qt], ((qt ? done1 : done0) + j - 1) & 1));
-                if (!ok) break;
+                uses++;
                 pf_fence_after();
+                float s[BN];
 #pragma unroll
-                for (int x = 0; x < D; x += 32) {
-                    float o[32];
-                    pf_ld32(o_addr + x, o);
-                    pf_ld_wait();
+                for (int x = 0; x < BN; x += 32) pf_ld32(s_addr + x, s + x);
+                pf_ld_wait();
+                const int k0 = t.kt.tile(i0 + j) * BN;
+                if (FEAT & 1) {
+                    // cap tanh(x scale / cap) = cap (1 - 2 / (1 + e^(2 x scale / cap)))
 #pragma unroll
-                    for (int e = 0; e < 32; e++) o[e] *= alpha;
-                    pf_st32(o_addr + x, o);
+                    for (int x = 0; x < BN; x++) s[x] = fmaf(-2.0f * cap2, rcp_approx(1.0f + ex2(s[x] * cin)), cap2);
                 }
+                if (FEAT & 2) {
+                    const float gap = (float)(qpos - k0);
+#pragma unroll
+                    for (int x = 0; x < BN; x++) s[x] = fmaf(-slope, fabsf(gap - (float)x), FEAT & 1 ? s[x] : s[x] * cin);
+                }
+                const bool all = !live || k0 + BN <= pre || (k0 >= klo && k0 + BN <= khi);
+                if (!__all_sync(0xffffffffu, all)) {
+                    const int p = pre - k0, lo = klo - k0, hi = khi - k0;
+#pragma unroll
+                    for (int x0 = 0; x0 < BN; x0 += 32) {
+                        const uint32_t seen = low_bits(p - x0) | (low_bits(hi - x0) & ~low_bits(lo - x0));
+#pragma unroll
+                        for (int x = 0; x < 32; x++) s[x0 + x] = seen >> x & 1 ? s[x0 + x] : -INFINITY;
+                    }
+                }
+                float mx[4];                                     // four chains
+#pragma unroll
+                for (int x = 0; x < 4; x++) mx[x] = max3(s[x], s[x + 4], s[x + 8]);
+#pragma unroll
+                for (int x = 12; x + 8 <= BN; x += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], s[x + e], s[x + 4 + e]);
+                static_assert((BN - 12) % 8 == 4, "the last four scores");
+                mx[0] = max3(mx[0], s[BN - 4], s[BN - 3]);
+                mx[1] = max3(mx[1], s[BN - 2], s[BN - 1]);
+                if (!two && j > 0) {                             // the row's maximum so far, from the other warpgroup
+                    ok = __all_sync(0xffffffffu, paged_wait(&turn[warp & 3], (turns + j - 1) & 1));
+                    if (!ok) break;
+                    const float mo = row_max[r];
+                    if (mo != m) {                               // it has moved: this warpgroup's sum follows
+                        l = m == -INFINITY ? 0.f : l * ex2((m - mo) * c1);
+                        m = mo;
+                    }
+                    __syncwarp();
+                }
+                const float mnew = live ? max3(fmaxf(m, mx[0]), mx[1], fmaxf(mx[2], mx[3])) : m;   // a row without a query holds anything
+                const bool move = __any_sync(0xffffffffu, (mnew - m) * c1 > 8.0f);
+                const float mold = m;
+                if (move) {
+                    l = m == -INFINITY ? 0.f : l * ex2((m - mnew) * c1);
+                    m = mnew;
+                }
+                if (!two) {
+                    row_max[r] = m;
+                    __syncwarp();
+                    if (lane == 0) pf_arrive(&turn[warp & 3]);
+                    __syncwarp();
+                }
+                if (move && j > 0) {
+                    const float alpha = mold == -INFINITY ? 0.f : ex2((mold - mnew) * c1);
+                    ok = __all_sync(0xffffffffu, paged_wait(&o_done[qt], ((qt ? done1 : done0) + j - 1) & 1));
+                    if (!ok) break;
+                    pf_fence_after();
+#pragma unroll
+                    for (int x = 0; x < D; x += 32) {
+                        float o[32];
+                        pf_ld32(o_addr + x, o);
+                        pf_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] *= alpha;
+                        pf_st32(o_addr + x, o);
+                    }
+                }
+                const float neg = m == -INFINITY ? 0.f : -m * c1;
+                const uint64_t c2 = pack2(c1, c1), n2 = pack2(neg, neg);
+                uint64_t sum[2] = {0, 0};
+#pragma unroll
+                for (int x = 0; x < BN; x += 32) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float p0, p1;
+                        unpack2(fma2(pack2(s[x + e], s[x + e + 1]), c2, n2), p0, p1);
+                        p0 = ex2(p0);
+                        p1 = ex2(p1);
+                        sum[e / 2 & 1] = add2(sum[e / 2 & 1], pack2(p0, p1));
+                        w[e / 2] = pack_bf16x2(p0, p1);
+                    }
+                    pf_st16(s_addr + x / 2, w);
+                    if (x == BN / 2 - 32 || x == BN - 32) {      // the product with V begins with the first half
+                        pf_st_wait();
+                        pf_fence_before();
+                        pf_arrive(x == BN - 32 ? &p_full[wg] : &p_half[wg]);
+                    }
+                }
+                float l0, l1;
+                unpack2(add2(sum[0], sum[1]), l0, l1);
+                l += l0 + l1;
             }
-            const float neg = m == -INFINITY ? 0.f : -m * c1;
-            const uint64_t c2 = pack2(c1, c1), n2 = pack2(neg, neg);
-            uint64_t sum[2] = {0, 0};
-#pragma unroll
-            for (int x = 0; x < BN; x += 32) {
-                uint32_t w[16];
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    float p0, p1;
-                    unpack2(fma2(pack2(s[x + e], s[x + e + 1]), c2, n2), p0, p1);
-                    p0 = ex2(p0);
-                    p1 = ex2(p1);
-                    sum[e / 2 & 1] = add2(sum[e / 2 & 1], pack2(p0, p1));
-                    w[e / 2] = pack_bf16x2(p0, p1);
-                }
-                pf_st16(s_addr + x / 2, w);
-                if (x == BN / 2 - 32 || x == BN - 32) {      // the product with V begins with the first half
-                    pf_st_wait();
-                    pf_fence_before();
-                    pf_arrive(x == BN - 32 ? &p_full[wg] : &p_half[wg]);
-                }
+            if (ok && n > 0) ok = __all_sync(0xffffffffu, paged_wait(&o_last[qt], (qt ? last1 : last0) & 1));
+            int x0 = 0, x1 = D;                                  // output columns of this warpgroup
+            if (!two && n > 0) {
+                // the two sums of a row meet, relative to the last maximum; each warpgroup stores half of the columns
+                if (ok) ok = __all_sync(0xffffffffu, paged_wait(&turn[warp & 3], (turns + n - 1) & 1));
+                const float mo = row_max[r];
+                l = m == -INFINITY ? 0.f : l * ex2((m - mo) * c1);
+                m = mo;
+                pair_sync();
+                if (wg == 1) row_max[r] = l;
+                pair_sync();
+                if (wg == 0) { l += row_max[r]; row_max[r] = l; }
+                pair_sync();
+                l = row_max[r];
+                x0 = wg * (D / 2);
+                x1 = x0 + D / 2;
+                turns += n;
             }
-            float l0, l1;
-            unpack2(add2(sum[0], sum[1]), l0, l1);
-            l += l0 + l1;
-        }
-        if (ok && n > 0) ok = __all_sync(0xffffffffu, paged_wait(&o_last[qt], (qt ? last1 : last0) & 1));
-        int x0 = 0, x1 = D;                                  // output columns of this warpgroup
-        if (!two && n > 0) {
-            // the two sums of a row meet, relative to the last maximum; each warpgroup stores half of the columns
-            if (ok) ok = __all_sync(0xffffffffu, paged_wait(&turn[warp & 3], (turns + n - 1) & 1));
-            const float mo = row_max[r];
-            l = m == -INFINITY ? 0.f : l * ex2((m - mo) * c1);
-            m = mo;
-            pair_sync();
-            if (wg == 1) row_max[r] = l;
-            pair_sync();
-            if (wg == 0) { l += row_max[r]; row_max[r] = l; }
-            pair_sync();
-            l = row_max[r];
-            x0 = wg * (D / 2);
-            x1 = x0 + D / 2;
-            turns += n;
-        }
-        if (n > 0) {
-            if (two) { done1 += n - 1; last1++; }
-            done0 += n - 1;
-            last0++;
-        }
-        if (ok) {
-            pf_fence_after();
-            const int64_t tok = t.first + token;
-            const float m2 = m * c1;                         // log2 units (c1 > 0)
-            const float inv = l > 0.f ? 1.0f / l : 0.f;
-            uint16_t* dst = a.out + tok * a.out_stride + (int64_t)head * D;
-            const bool whole = t.part < 0;
-            float4* part = a.part + (int64_t)t.part * (D / 4) * ROWS + qt * 128 + r;
+            if (n > 0) {
+                if (two) { done1 += n - 1; last1++; }
+                done0 += n - 1;
+                last0++;
+            }
+            if (ok) {
+                pf_fence_after();
+                const int64_t tok = t.first + token;
+                const float m2 = m * c1;                         // log2 units (c1 > 0)
+                const float inv = l > 0.f ? 1.0f / l : 0.f;
+                uint16_t* dst = a.out + tok * a.out_stride + (int64_t)head * D;
+                const bool whole = t.part < 0;
+                float4* part = a.part + (int64_t)t.part * (D / 4) * ROWS + qt * 128 + r;
 #pragma unroll 1
-            for (int x = x0; x < x1; x += 32) {
-                float o[32];
-                __syncwarp();                                // the stores below are not made by all lanes, the loads have to be
-                if (n > 0) {
-                    pf_ld32(o_addr + x, o);
-                    pf_ld_wait();
-                } else {
+                for (int x = x0; x < x1; x += 32) {
+                    float o[32];
+                    __syncwarp();                                // the stores below are not made by all lanes, the loads have to be
+                    if (n > 0) {
+                        pf_ld32(o_addr + x, o);
+                        pf_ld_wait();
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 32; e++) o[e] = 0.f;
+                        for (int e = 0; e < 32; e++) o[e] = 0.f;
+                    }
+                    if (!live) continue;
+                    if (whole) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8)
+                            *(uint4*)(dst + x + e) = make_uint4(pack_bf16x2(o[e] * inv, o[e + 1] * inv), pack_bf16x2(o[e + 2] * inv, o[e + 3] * inv),
+                                                                pack_bf16x2(o[e + 4] * inv, o[e + 5] * inv), pack_bf16x2(o[e + 6] * inv, o[e + 7] * inv));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) part[(x + e) / 4 * ROWS] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    }
                 }
-                if (!live) continue;
-                if (whole) {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 8)
-                        *(uint4*)(dst + x + e) = make_uint4(pack_bf16x2(o[e] * inv, o[e + 1] * inv), pack_bf16x2(o[e + 2] * inv, o[e + 3] * inv),
-                                                            pack_bf16x2(o[e + 4] * inv, o[e + 5] * inv), pack_bf16x2(o[e + 6] * inv, o[e + 7] * inv));
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4) part[(x + e) / 4 * ROWS] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                if (live && x0 == 0) {
+                    if (!whole) a.ml[(int64_t)t.part * ROWS + qt * 128 + r] = make_float2(m2, l);
+                    else if (a.lse) a.lse[tok * a.Hq + head] = (m2 + log2f(l)) * 0.6931471805599453f;
                 }
             }
-            if (live && x0 == 0) {
-                if (!whole) a.ml[(int64_t)t.part * ROWS + qt * 128 + r] = make_float2(m2, l);
-                else if (a.lse) a.lse[tok * a.Hq + head] = (m2 + log2f(l)) * 0.6931471805599453f;
-            }
-        }
-        if (!two && n > 0) pair_sync();                      // both have read O before the next item's first weights let it be replaced
+            if (!two && n > 0) pair_sync();                      // both have read O before the next item's first weights let it be replaced
         }
         if (!ok && lane == 0) atomicOr(a.wait_status, 1u << 26);
     } else if (warp == C::SM_WARPS) {
@@ -583,7 +598,8 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         // ---- the last of the three warps also finds the items ----
         const bool finder = lw == 2;
         int tiles_here = 0, tiles = 0, published = 0, asked = 0;  // row tiles of sequence `lane`, of all sequences; items, questions so far
-        auto tiles_of = [&](int sq) { return sq < a.seqs ? (prefill_span(a, sq).y + C::NQ * a.tokens - 1) / (C::NQ * a.tokens) : 0; };
+        auto tiles_in = [&](int tokens) { return (tokens + C::NQ * a.tokens - 1) / (C::NQ * a.tokens); };
+        auto tiles_of = [&](int sq) { return sq < a.seqs ? tiles_in(prefill_span(a, sq).y) : 0; };
         auto warp_scan = [&](int v) {
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -611,7 +627,16 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                 want -= total;
                 if (s0 + 32 >= a.seqs) return false;         // only if q_start changed under the call
             }
-            x = prefill_tile<C::NQ, BN>(a, sq, want);
+            PfSeq of;
+            if (sq < 32) {
+                of.first = __shfl_sync(0xffffffffu, seq_here.first, sq);
+                of.tokens = __shfl_sync(0xffffffffu, seq_here.tokens, sq);
+                of.len = __shfl_sync(0xffffffffu, seq_here.len, sq);
+                of.prefix = __shfl_sync(0xffffffffu, seq_here.prefix, sq);
+            } else {
+                of = prefill_seq(a, sq);
+            }
+            x = prefill_tile<C::NQ, BN>(a, of, sq, want);
             x.head = id % a.c.kv_heads;
             const int per = max(a.chunk_tiles, (x.kt.n + a.chunks - 1) / a.chunks);   // also where max_ctx was too small
             const int used = a.chunks > 1 ? max(1, (x.kt.n + per - 1) / per) : 1;
@@ -656,211 +681,211 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             publish(x);
         };
         if (finder) {
-            tiles_here = tiles_of(lane);
+            tiles_here = tiles_in(seq_here.tokens);
             for (int s0 = 0; s0 < a.seqs; s0 += 32) tiles += warp_sum_int(s0 ? tiles_of(s0 + lane) : tiles_here);
             PfItem x;
             if (look_up(blockIdx.x, x)) publish(x);
             else find_next();
         }
         while (ok && next_item()) {
-        const int n = t.n, i0 = t.i0, len = t.len, prefix = t.prefix, qhi = t.qhi;
-        if (n == 0) {
-            if (finder) find_next();
-            continue;
-        }
-        const int32_t* trow = a.c.table + (int64_t)t.seq * a.c.table_stride;
-        const uint16_t* kbase = a.c.k + t.head * a.c.head_stride;
-        const uint16_t* vbase = a.c.v + t.head * a.c.head_stride;
-        const int lo = a.o.window > 0 ? max(0, t.qlo - a.o.window + 1) : 0;
-        auto row_of = [&](int x) { return (x >> 2) * 12 + lw * 4 + (x & 3); };
-        auto key_of = [&](int j, int x) {                    // -1: a row nobody sees
-            const int rr = row_of(x), key = t.kt.tile(i0 + j) * BN + rr;
-            return x < NX && rr < BN && key < len && (key < prefix || (key >= lo && key <= qhi)) ? key : -1;
-        };
-        auto free_slot = [&](int slot) {
-            ok = __all_sync(0xffffffffu, paged_wait(&empty[slot % ST], ((slot / ST) & 1) ^ 1));
-            return ok;
-        };
-        // ---- row by row ----
-        int page[PER];                                       // of this lane's rows of the next tile
-        auto fetch_pages = [&](int j) {
-#pragma unroll
-            for (int e = 0; e < PER; e++) {
-                const int key = j < n ? key_of(j, lane + 32 * e) : -1;
-                page[e] = key >= 0 ? trow[paged_entry(a.c, key)] : 0;
+            const int n = t.n, i0 = t.i0, len = t.len, prefix = t.prefix, qhi = t.qhi;
+            if (n == 0) {
+                if (finder) find_next();
+                continue;
             }
-        };
-        auto set_offsets = [&](int j) {
+            const int32_t* trow = a.c.table + (int64_t)t.seq * a.c.table_stride;
+            const uint16_t* kbase = a.c.k + t.head * a.c.head_stride;
+            const uint16_t* vbase = a.c.v + t.head * a.c.head_stride;
+            const int lo = a.o.window > 0 ? max(0, t.qlo - a.o.window + 1) : 0;
+            auto row_of = [&](int x) { return (x >> 2) * 12 + lw * 4 + (x & 3); };
+            auto key_of = [&](int j, int x) {                    // -1: a row nobody sees
+                const int rr = row_of(x), key = t.kt.tile(i0 + j) * BN + rr;
+                return x < NX && rr < BN && key < len && (key < prefix || (key >= lo && key <= qhi)) ? key : -1;
+            };
+            auto free_slot = [&](int slot) {
+                ok = __all_sync(0xffffffffu, paged_wait(&empty[slot % ST], ((slot / ST) & 1) ^ 1));
+                return ok;
+            };
+            // ---- row by row ----
+            int page[PER];                                       // of this lane's rows of the next tile
+            auto fetch_pages = [&](int j) {
 #pragma unroll
-            for (int e = 0; e < PER; e++) {
-                const int x = lane + 32 * e, key = key_of(j, x);
-                if (x < NX && row_of(x) < BN) offs[(j & 1) * BN + row_of(x)] = key >= 0 ? paged_offset(a.c, page[e], paged_row(a.c, key)) : -1;
-            }
-            __syncwarp();
-        };
-        auto copy_rows = [&](int slot, const uint16_t* src, int j) {
-            const int64_t* off = offs + (j & 1) * BN;
-            const uint32_t dst = smem + C::RING + slot % ST * C::KV_BYTES;
-            constexpr int CPR = D / 8, RPI = 32 / CPR, B = 4;    // 16-byte chunks per row, rows per instruction, instructions at once
-            const int c = lane % CPR;
-            src += c * 8;
-#pragma unroll 1
-            for (int x0 = 0; x0 < NX; x0 += RPI * B) {
-                int64_t o[B];
-#pragma unroll
-                for (int b = 0; b < B; b++) {
-                    const int x = x0 + b * RPI + lane / CPR;
-                    o[b] = x < NX && row_of(x) < BN ? off[row_of(x)] : -2;
+                for (int e = 0; e < PER; e++) {
+                    const int key = j < n ? key_of(j, lane + 32 * e) : -1;
+                    page[e] = key >= 0 ? trow[paged_entry(a.c, key)] : 0;
                 }
+            };
+            auto set_offsets = [&](int j) {
 #pragma unroll
-                for (int b = 0; b < B; b++) {
-                    const int rr = row_of(x0 + b * RPI + lane / CPR);
-                    if (o[b] > -2)
-                        cp_async16_zfill(dst + (c >> 3) * C::SLAB + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), src + max(o[b], (int64_t)0), o[b] < 0 ? 0 : 16);
-                }
-            }
-            paged_cp_commit();
-        };
-        // ---- by pages: lane i looks after box i of a tile ----
-        int box_page = 0;
-        auto box_key = [&](int j) {                          // -1: nobody sees a row of the box
-            const int key = t.kt.tile(i0 + j) * BN + lane * a.box;
-            return j < n && lane < boxes && key < len && (key < prefix || (key + a.box > lo && key <= qhi)) ? key : -1;
-        };
-        auto fetch_box_page = [&](int j) {
-            const int key = box_key(j);
-            return key >= 0 ? trow[paged_entry(a.c, key)] : 0;
-        };
-        auto copy_boxes = [&](int slot, const CUtensorMap* map, int j, int pages_of_tile) {
-            const int key = box_key(j);
-            const int in_page = key >= 0 ? paged_row(a.c, key) : -1;
-            const int st = slot % ST, total = boxes * (D / 64), x = lane * 3 + lw;
-            const int bx = min(x / (D / 64), 31), slab = x % (D / 64);
-            const int pg = __shfl_sync(0xffffffffu, pages_of_tile, bx), row = __shfl_sync(0xffffffffu, in_page, bx);
-            if (x < total && row >= 0) {
-                mbar_expect_tx(&full[st], a.box * 128);
-                pf_tma_4d(smem + C::RING + st * C::KV_BYTES + slab * C::SLAB + bx * a.box * 128, map, slab * 64, a.rows_first ? row : t.head,
-                          a.rows_first ? t.head : row, pg, &full[st]);
-            } else {
-                pf_arrive(&full[st]);
-            }
-            __syncwarp();
-        };
-        // rows copied one by one are handed over when they have landed: LAG slots later where every slot is copied so
-        auto hand_over = [&](int slot) {
-            if (a.box) {
-                paged_cp_wait<0>();
-                pf_fence_async();
-                pf_arrive(&full[slot % ST]);
-            } else if (slot - handed >= C::LAG) {
-                paged_cp_wait<C::LAG>();
-                pf_fence_async();
-                pf_arrive(&full[handed++ % ST]);
-            }
-        };
-        // The item's queries, when the last scores of the item before are done: by TMA, or each warp every third 32 rows, of which
-        // lane i knows where row i lies.
-        auto load_queries = [&] {
-            if (!a.box) {                                    // nothing may be waited for here that waits for a slot in flight
-                paged_cp_wait<0>();
-                pf_fence_async();
-                while (handed < slot0 + k_slot(0) + 1) pf_arrive(&full[handed++ % ST]);
-            }
-            ok = __all_sync(0xffffffffu, paged_wait(q_empty, (seen & 1) ^ 1));
-            if (!ok) return;
-            const int row_tiles = t.two ? 2 : 1;
-            if (a.q_box) {                                   // tokens behind the sequence's last are somebody else's, or zeros: never stored
-                if (lw == 0 && lane < row_tiles * (D / 64)) {
-                    const int qt = lane / (D / 64), slab = lane % (D / 64);
-                    mbar_expect_tx(q_full, a.tokens * a.G * 128);
-                    pf_tma_3d(smem + qt * C::Q_BYTES + slab * (128 * 128), &q_map, slab * 64, t.head * a.G, t.first + t.tok0 + qt * a.tokens, q_full);
-                } else {
-                    pf_arrive(q_full);
+                for (int e = 0; e < PER; e++) {
+                    const int x = lane + 32 * e, key = key_of(j, x);
+                    if (x < NX && row_of(x) < BN) offs[(j & 1) * BN + row_of(x)] = key >= 0 ? paged_offset(a.c, page[e], paged_row(a.c, key)) : -1;
                 }
                 __syncwarp();
-                return;
-            }
-            constexpr int CPR = D / 8, RPI = 32 / CPR;       // 16-byte chunks per row, rows per instruction
-            const int c = lane % CPR;
-            for (int g0 = lw * 32; g0 < row_tiles * 128; g0 += 96) {
-                const int rr0 = g0 & 127, mine = rr0 + lane, tk = mine / a.G, token = t.tok0 + (g0 >> 7) * a.tokens + tk;
-                const int64_t at = tk < a.tokens && token < t.tokens
-                                       ? (t.first + token) * a.q_stride + (int64_t)(t.head * a.G + mine - tk * a.G) * D : -1;
-                const uint32_t qs = smem + (g0 >> 7) * C::Q_BYTES;
+            };
+            auto copy_rows = [&](int slot, const uint16_t* src, int j) {
+                const int64_t* off = offs + (j & 1) * BN;
+                const uint32_t dst = smem + C::RING + slot % ST * C::KV_BYTES;
+                constexpr int CPR = D / 8, RPI = 32 / CPR, B = 4;    // 16-byte chunks per row, rows per instruction, instructions at once
+                const int c = lane % CPR;
+                src += c * 8;
+#pragma unroll 1
+                for (int x0 = 0; x0 < NX; x0 += RPI * B) {
+                    int64_t o[B];
+#pragma unroll
+                    for (int b = 0; b < B; b++) {
+                        const int x = x0 + b * RPI + lane / CPR;
+                        o[b] = x < NX && row_of(x) < BN ? off[row_of(x)] : -2;
+                    }
+#pragma unroll
+                    for (int b = 0; b < B; b++) {
+                        const int rr = row_of(x0 + b * RPI + lane / CPR);
+                        if (o[b] > -2)
+                            cp_async16_zfill(dst + (c >> 3) * C::SLAB + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), src + max(o[b], (int64_t)0), o[b] < 0 ? 0 : 16);
+                    }
+                }
+                paged_cp_commit();
+            };
+            // ---- by pages: lane i looks after box i of a tile ----
+            int box_page = 0;
+            auto box_key = [&](int j) {                          // -1: nobody sees a row of the box
+                const int key = t.kt.tile(i0 + j) * BN + lane * a.box;
+                return j < n && lane < boxes && key < len && (key < prefix || (key + a.box > lo && key <= qhi)) ? key : -1;
+            };
+            auto fetch_box_page = [&](int j) {
+                const int key = box_key(j);
+                return key >= 0 ? trow[paged_entry(a.c, key)] : 0;
+            };
+            auto copy_boxes = [&](int slot, const CUtensorMap* map, int j, int pages_of_tile) {
+                const int key = box_key(j);
+                const int in_page = key >= 0 ? paged_row(a.c, key) : -1;
+                const int st = slot % ST, total = boxes * (D / 64), x = lane * 3 + lw;
+                const int bx = min(x / (D / 64), 31), slab = x % (D / 64);
+                const int pg = __shfl_sync(0xffffffffu, pages_of_tile, bx), row = __shfl_sync(0xffffffffu, in_page, bx);
+                if (x < total && row >= 0) {
+                    mbar_expect_tx(&full[st], a.box * 128);
+                    pf_tma_4d(smem + C::RING + st * C::KV_BYTES + slab * C::SLAB + bx * a.box * 128, map, slab * 64, a.rows_first ? row : t.head,
+                              a.rows_first ? t.head : row, pg, &full[st]);
+                } else {
+                    pf_arrive(&full[st]);
+                }
+                __syncwarp();
+            };
+            // rows copied one by one are handed over when they have landed: LAG slots later where every slot is copied so
+            auto hand_over = [&](int slot) {
+                if (a.box) {
+                    paged_cp_wait<0>();
+                    pf_fence_async();
+                    pf_arrive(&full[slot % ST]);
+                } else if (slot - handed >= C::LAG) {
+                    paged_cp_wait<C::LAG>();
+                    pf_fence_async();
+                    pf_arrive(&full[handed++ % ST]);
+                }
+            };
+            // The item's queries, when the last scores of the item before are done: by TMA, or each warp every third 32 rows, of which
+            // lane i knows where row i lies.
+            auto load_queries = [&] {
+                if (!a.box) {                                    // nothing may be waited for here that waits for a slot in flight
+                    paged_cp_wait<0>();
+                    pf_fence_async();
+                    while (handed < slot0 + k_slot(0) + 1) pf_arrive(&full[handed++ % ST]);
+                }
+                ok = __all_sync(0xffffffffu, paged_wait(q_empty, (seen & 1) ^ 1));
+                if (!ok) return;
+                const int row_tiles = t.two ? 2 : 1;
+                if (a.q_box) {                                   // tokens behind the sequence's last are somebody else's, or zeros: never stored
+                    if (lw == 0 && lane < row_tiles * (D / 64)) {
+                        const int qt = lane / (D / 64), slab = lane % (D / 64);
+                        mbar_expect_tx(q_full, a.tokens * a.G * 128);
+                        pf_tma_3d(smem + qt * C::Q_BYTES + slab * (128 * 128), &q_map, slab * 64, t.head * a.G, t.first + t.tok0 + qt * a.tokens, q_full);
+                    } else {
+                        pf_arrive(q_full);
+                    }
+                    __syncwarp();
+                    return;
+                }
+                constexpr int CPR = D / 8, RPI = 32 / CPR;       // 16-byte chunks per row, rows per instruction
+                const int c = lane % CPR;
+                for (int g0 = lw * 32; g0 < row_tiles * 128; g0 += 96) {
+                    const int rr0 = g0 & 127, mine = rr0 + lane, tk = mine / a.G, token = t.tok0 + (g0 >> 7) * a.tokens + tk;
+                    const int64_t at = tk < a.tokens && token < t.tokens
+                                           ? (t.first + token) * a.q_stride + (int64_t)(t.head * a.G + mine - tk * a.G) * D : -1;
+                    const uint32_t qs = smem + (g0 >> 7) * C::Q_BYTES;
 #pragma unroll 8
-                for (int i = 0; i < 32; i += RPI) {
-                    const int x = i + lane / CPR, rr = rr0 + x;
-                    const int64_t o = __shfl_sync(0xffffffffu, at, x);
-                    cp_async16_zfill(qs + (c >> 3) * (128 * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), a.q + (o < 0 ? 0 : o) + c * 8, o < 0 ? 0 : 16);
+                    for (int i = 0; i < 32; i += RPI) {
+                        const int x = i + lane / CPR, rr = rr0 + x;
+                        const int64_t o = __shfl_sync(0xffffffffu, at, x);
+                        cp_async16_zfill(qs + (c >> 3) * (128 * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), a.q + (o < 0 ? 0 : o) + c * 8, o < 0 ? 0 : 16);
+                    }
                 }
-            }
-            paged_cp_commit();
-            paged_cp_wait<0>();
-            pf_fence_async();
-            pf_arrive(q_full);
-        };
-        static_assert(16 * (D / 64) <= 96, "a lane issues one box");
-        int v_page = 0, v_page2 = 0;                         // box pages of the K tiles whose V tile is still to come
-        auto fill_k = [&](int j) {
-            const int slot = slot0 + k_slot(j);
-            if (!a.box) {
-                set_offsets(j);
-                fetch_pages(j + 1);
+                paged_cp_commit();
+                paged_cp_wait<0>();
+                pf_fence_async();
+                pf_arrive(q_full);
+            };
+            static_assert(16 * (D / 64) <= 96, "a lane issues one box");
+            int v_page = 0, v_page2 = 0;                         // box pages of the K tiles whose V tile is still to come
+            auto fill_k = [&](int j) {
+                const int slot = slot0 + k_slot(j);
+                if (!a.box) {
+                    set_offsets(j);
+                    fetch_pages(j + 1);
+                    if (!free_slot(slot)) return;
+                    copy_rows(slot, kbase, j);
+                } else {
+                    const int pages_of_tile = box_page;
+                    box_page = fetch_box_page(j + 1);
+                    v_page2 = v_page;
+                    v_page = pages_of_tile;
+                    if (!free_slot(slot)) return;
+                    if (__all_sync(0xffffffffu, box_key(j) < 0 || (unsigned)pages_of_tile < (unsigned)a.c.pages)) {
+                        copy_boxes(slot, &k_map, j, pages_of_tile);
+                        return;
+                    }
+                    fetch_pages(j);                              // a bad page: reported, and zeros
+                    set_offsets(j);
+                    copy_rows(slot, kbase, j);
+                }
+                hand_over(slot);
+            };
+            auto fill_v = [&](int j) {
+                const int slot = slot0 + v_slot(j);
                 if (!free_slot(slot)) return;
-                copy_rows(slot, kbase, j);
+                if (a.box) {
+                    const int pages_of_tile = t.two || j == n - 1 ? v_page : v_page2;
+                    const int k0 = t.kt.tile(i0 + j) * BN;
+                    const bool whole = k0 + BN <= len && (k0 + BN <= prefix || (k0 >= lo && k0 + BN - 1 <= qhi));
+                    if (whole && __all_sync(0xffffffffu, box_key(j) < 0 || (unsigned)pages_of_tile < (unsigned)a.c.pages)) {
+                        copy_boxes(slot, &v_map, j, pages_of_tile);
+                        return;
+                    }
+                    fetch_pages(j);
+                    set_offsets(j);
+                }
+                copy_rows(slot, vbase, j);
+                hand_over(slot);
+                __syncwarp();                                    // the offsets may be replaced
+            };
+            if (a.box) box_page = fetch_box_page(0);
+            else fetch_pages(0);
+            fill_k(0);
+            if (ok) load_queries();
+            if (t.two) {
+                for (int j = 0; j < n && ok; j++) {
+                    fill_v(j);
+                    if (ok && j + 1 < n) fill_k(j + 1);
+                }
             } else {
-                const int pages_of_tile = box_page;
-                box_page = fetch_box_page(j + 1);
-                v_page2 = v_page;
-                v_page = pages_of_tile;
-                if (!free_slot(slot)) return;
-                if (__all_sync(0xffffffffu, box_key(j) < 0 || (unsigned)pages_of_tile < (unsigned)a.c.pages)) {
-                    copy_boxes(slot, &k_map, j, pages_of_tile);
-                    return;
+                if (ok && n > 1) fill_k(1);
+                for (int j = 0; j < n && ok; j++) {
+                    fill_v(j);
+                    if (ok && j + 2 < n) fill_k(j + 2);
                 }
-                fetch_pages(j);                              // a bad page: reported, and zeros
-                set_offsets(j);
-                copy_rows(slot, kbase, j);
             }
-            hand_over(slot);
-        };
-        auto fill_v = [&](int j) {
-            const int slot = slot0 + v_slot(j);
-            if (!free_slot(slot)) return;
-            if (a.box) {
-                const int pages_of_tile = t.two || j == n - 1 ? v_page : v_page2;
-                const int k0 = t.kt.tile(i0 + j) * BN;
-                const bool whole = k0 + BN <= len && (k0 + BN <= prefix || (k0 >= lo && k0 + BN - 1 <= qhi));
-                if (whole && __all_sync(0xffffffffu, box_key(j) < 0 || (unsigned)pages_of_tile < (unsigned)a.c.pages)) {
-                    copy_boxes(slot, &v_map, j, pages_of_tile);
-                    return;
-                }
-                fetch_pages(j);
-                set_offsets(j);
-            }
-            copy_rows(slot, vbase, j);
-            hand_over(slot);
-            __syncwarp();                                    // the offsets may be replaced
-        };
-        if (a.box) box_page = fetch_box_page(0);
-        else fetch_pages(0);
-        fill_k(0);
-        if (ok) load_queries();
-        if (t.two) {
-            for (int j = 0; j < n && ok; j++) {
-                fill_v(j);
-                if (ok && j + 1 < n) fill_k(j + 1);
-            }
-        } else {
-            if (ok && n > 1) fill_k(1);
-            for (int j = 0; j < n && ok; j++) {
-                fill_v(j);
-                if (ok && j + 2 < n) fill_k(j + 2);
-            }
-        }
-        slot0 += 2 * n;
-        seen++;
-        if (finder && ok) find_next();                       // all loads of this item are on their way
+            slot0 += 2 * n;
+            seen++;
+            if (finder && ok) find_next();                       // all loads of this item are on their way
         }
         // hand over the last slots
         paged_cp_wait<0>();
@@ -888,8 +913,9 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const PrefillAr
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kvh = blockIdx.y;
     constexpr int PER_ROWS = D / 8 / GROUPS;                     // CTAs per 32 rows
     const int r = blockIdx.z / PER_ROWS * 32 + lane, col = blockIdx.z % PER_ROWS * GROUPS + warp / CG;
+    pdl_wait();
     const int4 ds = a.desc[blockIdx.x];
-    if (ds.z <= 1) return;
+    if (ds.z <= 1 || ds.z > a.chunks || (unsigned)ds.x >= (unsigned)a.seqs || (unsigned)ds.y >= (unsigned)a.tiles) return;   // (a CTA that gave up)
     const int2 span = prefill_span(a, ds.x);
     const int r_token = (r & 127) / a.G, token = (ds.y * PfCfg<D>::NQ + (r >> 7)) * a.tokens + r_token;
     const bool live = r_token < a.tokens && token < span.y;
@@ -942,8 +968,10 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const PrefillAr
 struct PrefillPlan { int tiles, chunks, chunk_tiles; size_t part, ml, desc, total; };
 // Cutting the keys of a tile. With `work` key tiles in all an SM has work / SMs of them to do: a tile whose keys are a good deal more than half
 // of that is cut, so that its longest piece does not decide the time (prompts: the last rows see twice the average; chunks
-// behind contexts of different lengths). Not below 512 keys: the partial outputs and the join then cost what they save (1024 tokens of 8 heads
-// of 256: 35 us uncut, 29 us at 512 keys, 29 at 256; 4 drafts on contexts up to 40000: 62 us at half of an SM's work, 65 at a third, 70 at a quarter).
+// behind contexts of different lengths: 4 drafts on contexts up to 40000 take 62 us at half of an SM's work, 65 at a third, 70 at a quarter).
+// Where that is less than 512 keys, a tile is cut as far as all pieces still run at once, into 256 keys at least, or else into 512:
+// below, the partial outputs and the join cost what they save (1024 tokens of 8 heads of 256, 64 tiles: 26.9 us in 96 pieces of up to 512
+// keys, 24.8 in 120 of up to 384, 28.9 in 160 of up to 256, which do not all run at once).
 static PrefillPlan prefill_plan(int D, int kv_heads, int seqs, int total_q, int q_heads, int max_ctx, int window, bool has_prefix) {
     PrefillPlan p;
     const int rows = D == 256 ? 128 : 256, bn = D == 256 ? 64 : 128, tokens = rows / 128 * (128 / (q_heads / kv_heads)), sms = paged_sm_count();
@@ -956,7 +984,9 @@ static PrefillPlan prefill_plan(int D, int kv_heads, int seqs, int total_q, int 
         mean = std::min(mean, keys);
     }
     const double longest = keys / bn, work = std::max(1.0, mean / bn) * pairs;
-    const double piece = std::max(512.0 / bn, work / (2.0 * sms));
+    const double mean_pieces = (double)sms / pairs - 0.5;        // of a tile, when all run at once; the last piece of a tile is half full
+    const double fit = mean_pieces > 0 ? std::max(256.0 / bn, mean / bn / mean_pieces) : 512.0 / bn;
+    const double piece = std::max(std::min(fit, 512.0 / bn), work / (2.0 * sms));
     p.chunks = (int)std::max(1.0, std::min(longest / piece, 1024.0));
     p.chunk_tiles = std::max(1, (int)((longest + p.chunks - 1) / p.chunks));
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
@@ -1028,9 +1058,14 @@ static int32_t launch_prefill(cudaStream_t s, PrefillArgs a) {
     paged_prefill_kernel<D, FEAT><<<a.tiles * a.c.kv_heads * a.chunks, C::THREADS, C::TOTAL, s>>>(qm, km, vm, a);
     LTHN_CUDA_TRY(cudaGetLastError());
     if (a.chunks > 1) {
-        if (a.chunks <= 8) paged_prefill_join_kernel<D, 1><<<dim3(a.tiles, a.c.kv_heads, C::ROWS / 32 * (D / 64)), 256, 0, s>>>(a);
-        else paged_prefill_join_kernel<D, 8><<<dim3(a.tiles, a.c.kv_heads, C::ROWS / 32 * (D / 8)), 256, 0, s>>>(a);
-        LTHN_CUDA_TRY(cudaGetLastError());
+        const bool few = a.chunks <= 8;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(a.tiles, a.c.kv_heads, C::ROWS / 32 * (few ? D / 64 : D / 8)); cfg.blockDim = dim3(256); cfg.stream = s;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = at; cfg.numAttrs = 1;
+        LTHN_CUDA_TRY(few ? cudaLaunchKernelEx(&cfg, paged_prefill_join_kernel<D, 1>, a) : cudaLaunchKernelEx(&cfg, paged_prefill_join_kernel<D, 8>, a));
     }
     return LTHN_OK;
 }
