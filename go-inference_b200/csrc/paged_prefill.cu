@@ -45,6 +45,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 #include <numeric>
 
@@ -66,7 +67,8 @@ struct PrefillArgs {
     int q_box;           // queries by TMA (their row stride is a multiple of head_dim), else copied row by row
     int tiles;           // upper bound of the row tiles of all sequences
     int chunks;          // chunks per row tile and kv head
-    int chunk_tiles;     // key tiles per chunk
+    int chunk_tiles;     // key tiles per chunk, unless the lengths call for others
+    int levels, sms;     // key tiles of max_ctx
     float4* part;        // [tiles*kv_heads*chunks][D/4][rows] unnormalised outputs, four columns each
     float2* ml;          // [tiles*kv_heads*chunks][rows] maximum (log2 units) and sum
     int4* desc;          // [tiles] sequence, tile of the sequence, chunks in use
@@ -330,6 +332,9 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         return t.head >= 0;
     };
 
+    // The j-th key tile of an item. A distance bias lets scores rise towards the query, and with them the maximum at every tile, so
+    // those go from the newest keys to the oldest (4 drafts on contexts up to 40000: 61 us against 59).
+    auto tile_at = [&](int j) { return t.kt.tile(FEAT & 2 ? t.i0 + t.n - 1 - j : t.i0 + j); };
     // ring slots of the K and V tile of key tile j of an item, in the order of their last use
     auto k_slot = [&](int j) { return t.two ? 2 * j : j < 2 ? j : 2 * j - 1; };
     auto v_slot = [&](int j) { return t.two ? 2 * j + 1 : j == t.n - 1 ? 2 * t.n - 1 : 2 * j + 2; };
@@ -355,7 +360,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         };
         while (ok && next_item()) {
             const bool two = t.two;
-            const int n = t.n, i0 = t.i0, qt = two ? wg : 0, len = t.len;
+            const int n = t.n, qt = two ? wg : 0, len = t.len;
             const int token = t.tok0 + qt * a.tokens + r_token;  // of the sequence
             const bool live = r_token < a.tokens && token < t.tokens;
             const int head = t.head * a.G + r_head;
@@ -375,7 +380,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
 #pragma unroll
                 for (int x = 0; x < BN; x += 32) pf_ld32(s_addr + x, s + x);
                 pf_ld_wait();
-                const int k0 = t.kt.tile(i0 + j) * BN;
+                const int k0 = tile_at(j) * BN;
                 if (FEAT & 1) {
                     // cap tanh(x scale / cap) = cap (1 - 2 / (1 + e^(2 x scale / cap)))
 #pragma unroll
@@ -598,6 +603,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         // ---- the last of the three warps also finds the items ----
         const bool finder = lw == 2;
         int tiles_here = 0, tiles = 0, published = 0, asked = 0;  // row tiles of sequence `lane`, of all sequences; items, questions so far
+        int levels = 0, chunk_tiles = a.chunk_tiles;         // key tiles of the longest sequence, of a chunk
         auto tiles_in = [&](int tokens) { return (tokens + C::NQ * a.tokens - 1) / (C::NQ * a.tokens); };
         auto tiles_of = [&](int sq) { return sq < a.seqs ? tiles_in(prefill_span(a, sq).y) : 0; };
         auto warp_scan = [&](int v) {
@@ -608,24 +614,42 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             }
             return v;
         };
-        // item `id` in `x`; false: there is no such tile or chunk. Tiles are counted from the last one, the longest of a prompt.
+        // Item `id` in `x`; false: there is no such tile or chunk. First chunks come before second ones, so that what is left of a tile's
+        // keys comes last, and the row tiles in the order of their last key, the farthest first; with more than 32 sequences that
+        // holds within a sequence only.
         auto look_up = [&](int id, PfItem& x) {
-            const int rest = id / a.c.kv_heads, chunk = rest % a.chunks, tile_id = rest / a.chunks;
+            const int rest = id / a.c.kv_heads, chunk = rest / a.tiles, tile_id = rest % a.tiles;
             if (tile_id >= tiles) {
                 if (a.chunks > 1 && chunk == 0 && id % a.c.kv_heads == 0 && lane == 0) a.desc[tile_id] = make_int4(0, 0, 0, 0);
                 return false;
             }
             int want = tiles - 1 - tile_id, sq = 0, count = tiles_here;
-            for (int s0 = 0;; s0 += 32, count = tiles_of(s0 + lane)) {
-                const int incl = warp_scan(count), total = __shfl_sync(0xffffffffu, incl, 31);
-                if (want < total) {
-                    const int l = __ffs(__ballot_sync(0xffffffffu, incl > want)) - 1;
-                    want -= __shfl_sync(0xffffffffu, incl - count, l);
-                    sq = s0 + l;
-                    break;
+            if (a.seqs > 1 && a.seqs <= 32) {
+                // the tile's level, the key tile that its last token is in: more than tile_id tiles are at level lo or behind, not so at hi
+                int lo = 0, hi = levels + 1, at_lo = tiles_here, at_hi = 0, before = 0;
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1, token = (mid - 1) * BN - (seq_here.len - seq_here.tokens);   // of this lane's sequence, first of the level
+                    int there = token < 0 ? tiles_here : token >= seq_here.tokens ? 0 : tiles_here;
+                    if (there > 1 && token > 0) there -= token / (C::NQ * a.tokens);
+                    const int total = warp_sum_int(there);
+                    if (total > tile_id) { lo = mid; at_lo = there; }
+                    else { hi = mid; at_hi = there; before = total; }
                 }
-                want -= total;
-                if (s0 + 32 >= a.seqs) return false;         // only if q_start changed under the call
+                const int incl = warp_scan(at_lo - at_hi), rank = tile_id - before;
+                sq = __ffs(__ballot_sync(0xffffffffu, incl > rank)) - 1;
+                want = __shfl_sync(0xffffffffu, tiles_here - 1 - at_hi + incl - (at_lo - at_hi), sq) - rank;
+            } else {
+                for (int s0 = 0;; s0 += 32, count = tiles_of(s0 + lane)) {
+                    const int incl = warp_scan(count), total = __shfl_sync(0xffffffffu, incl, 31);
+                    if (want < total) {
+                        const int l = __ffs(__ballot_sync(0xffffffffu, incl > want)) - 1;
+                        want -= __shfl_sync(0xffffffffu, incl - count, l);
+                        sq = s0 + l;
+                        break;
+                    }
+                    want -= total;
+                    if (s0 + 32 >= a.seqs) return false;     // only if q_start changed under the call
+                }
             }
             PfSeq of;
             if (sq < 32) {
@@ -638,7 +662,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             }
             x = prefill_tile<C::NQ, BN>(a, of, sq, want);
             x.head = id % a.c.kv_heads;
-            const int per = max(a.chunk_tiles, (x.kt.n + a.chunks - 1) / a.chunks);   // also where max_ctx was too small
+            const int per = max(chunk_tiles, (x.kt.n + a.chunks - 1) / a.chunks);     // also where max_ctx was too small
             const int used = a.chunks > 1 ? max(1, (x.kt.n + per - 1) / per) : 1;
             if (a.chunks > 1 && chunk == 0 && x.head == 0 && lane == 0) a.desc[tile_id] = make_int4(sq, want, used, 0);
             if (chunk >= used) return false;
@@ -683,12 +707,28 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         if (finder) {
             tiles_here = tiles_in(seq_here.tokens);
             for (int s0 = 0; s0 < a.seqs; s0 += 32) tiles += warp_sum_int(s0 ? tiles_of(s0 + lane) : tiles_here);
+            levels = (int)__reduce_max_sync(0xffffffffu, (unsigned)((seq_here.len + BN - 1) / BN));
+            if (a.chunks > 1 && a.seqs <= 32 && tiles * a.c.kv_heads <= a.sms && (a.seqs > 1 || levels * 8 < a.levels * 7)) {
+                // lengths other than max_ctx say better how to cut: the shortest chunks, 256 keys at least, with which all run at once
+                const int n1 = tiles_here ? prefill_tile<C::NQ, BN>(a, seq_here, lane, tiles_here - 1).kt.n : 0;
+                const int n0 = tiles_here > 1 ? prefill_tile<C::NQ, BN>(a, seq_here, lane, 0).kt.n : n1;
+                int hi = (int)__reduce_max_sync(0xffffffffu, (unsigned)max(n0, n1)), lo = max(256 / BN, (hi + a.chunks - 1) / a.chunks);
+                const float mean = 0.5f * (n0 + n1);
+                while (lo < hi) {
+                    const int mid = (lo + hi) >> 1;
+                    const float each = mean * (1.0f / mid);  // chunks of a tile; of those of several tiles the last is half full on average
+                    const int mine = (int)ceilf(tiles_here > 1 ? tiles_here * (each + 0.5f) : each);
+                    if (warp_sum_int(mine) * a.c.kv_heads <= a.sms) hi = mid;
+                    else lo = mid + 1;
+                }
+                chunk_tiles = lo;
+            }
             PfItem x;
             if (look_up(blockIdx.x, x)) publish(x);
             else find_next();
         }
         while (ok && next_item()) {
-            const int n = t.n, i0 = t.i0, len = t.len, prefix = t.prefix, qhi = t.qhi;
+            const int n = t.n, len = t.len, prefix = t.prefix, qhi = t.qhi;
             if (n == 0) {
                 if (finder) find_next();
                 continue;
@@ -699,7 +739,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             const int lo = a.o.window > 0 ? max(0, t.qlo - a.o.window + 1) : 0;
             auto row_of = [&](int x) { return (x >> 2) * 12 + lw * 4 + (x & 3); };
             auto key_of = [&](int j, int x) {                    // -1: a row nobody sees
-                const int rr = row_of(x), key = t.kt.tile(i0 + j) * BN + rr;
+                const int rr = row_of(x), key = tile_at(j) * BN + rr;
                 return x < NX && rr < BN && key < len && (key < prefix || (key >= lo && key <= qhi)) ? key : -1;
             };
             auto free_slot = [&](int slot) {
@@ -749,7 +789,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             // ---- by pages: lane i looks after box i of a tile ----
             int box_page = 0;
             auto box_key = [&](int j) {                          // -1: nobody sees a row of the box
-                const int key = t.kt.tile(i0 + j) * BN + lane * a.box;
+                const int key = tile_at(j) * BN + lane * a.box;
                 return j < n && lane < boxes && key < len && (key < prefix || (key + a.box > lo && key <= qhi)) ? key : -1;
             };
             auto fetch_box_page = [&](int j) {
@@ -854,7 +894,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                 if (!free_slot(slot)) return;
                 if (a.box) {
                     const int pages_of_tile = t.two || j == n - 1 ? v_page : v_page2;
-                    const int k0 = t.kt.tile(i0 + j) * BN;
+                    const int k0 = tile_at(j) * BN;
                     const bool whole = k0 + BN <= len && (k0 + BN <= prefix || (k0 >= lo && k0 + BN - 1 <= qhi));
                     if (whole && __all_sync(0xffffffffu, box_key(j) < 0 || (unsigned)pages_of_tile < (unsigned)a.c.pages)) {
                         copy_boxes(slot, &v_map, j, pages_of_tile);
@@ -904,7 +944,8 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
 
 // Joins the chunks of a row tile. A lane is a row, a warp 8 columns of 32 rows and every CG-th chunk; with CG > 1 the warps of a column group
 // meet in shared memory. CG = 1 for up to 8 chunks: no barrier, few CTAs (4 chunks of 68 tiles: 3 us, 17 with CG = 8). CG = 8
-// above: one thread's chain of loads over the chunks would take longer than the CTAs it saves (18 chunks: 3 us less).
+// above, where its CTAs run in two waves at most: one thread's chain of loads over the chunks would take longer than the CTAs it saves
+// (18 chunks of 16 tiles: 3 us less).
 template <int D, int CG>
 __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const PrefillArgs a) {
     constexpr int ROWS = PfCfg<D>::ROWS, GROUPS = 8 / CG;        // column groups of a CTA
@@ -965,17 +1006,19 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const PrefillAr
     if (a.lse && col == 0) a.lse[tok * a.Hq + head] = (m + log2f(l)) * 0.6931471805599453f;
 }
 
-struct PrefillPlan { int tiles, chunks, chunk_tiles; size_t part, ml, desc, total; };
-// Cutting the keys of a tile. With `work` key tiles in all an SM has work / SMs of them to do: a tile whose keys are a good deal more than half
-// of that is cut, so that its longest piece does not decide the time (prompts: the last rows see twice the average; chunks
-// behind contexts of different lengths: 4 drafts on contexts up to 40000 take 62 us at half of an SM's work, 65 at a third, 70 at a quarter).
-// Where that is less than 512 keys, a tile is cut as far as all pieces still run at once, into 256 keys at least, or else into 512:
-// below, the partial outputs and the join cost what they save (1024 tokens of 8 heads of 256, 64 tiles: 26.9 us in 96 pieces of up to 512
-// keys, 24.8 in 120 of up to 384, 28.9 in 160 of up to 256, which do not all run at once).
+struct PrefillPlan { int tiles, levels, chunks, chunk_tiles; size_t part, ml, desc, total; };
+// Cutting the keys of a tile. With no more (row tile, kv head) pairs than SMs they are cut as far as all chunks still run at once, into 256
+// keys at least: below, the partial outputs and the join cost what they save (1024 tokens of 8 heads of 256, 64 pairs: 26.9 us in 96 chunks of
+// up to 512 keys, 24.8 in 120 of up to 384, 28.9 in 160 of up to 256, which do not all run at once). `chunk_tiles` is what that comes to for
+// sequences of max_ctx; a call whose lengths are others finds its own from them, for which there is room for twice the chunks
+// (8 tokens behind 4096 keys, max_ctx 131072: 27.6 us with chunks made for max_ctx, 14.4 with its own). With more pairs than SMs a
+// tile is cut whose keys are a good deal more than half of an SM's share of the work, so that the longest does not decide the time, but not
+// below 512 keys.
 static PrefillPlan prefill_plan(int D, int kv_heads, int seqs, int total_q, int q_heads, int max_ctx, int window, bool has_prefix) {
     PrefillPlan p;
     const int rows = D == 256 ? 128 : 256, bn = D == 256 ? 64 : 128, tokens = rows / 128 * (128 / (q_heads / kv_heads)), sms = paged_sm_count();
     p.tiles = (int)std::min<int64_t>((int64_t)total_q / tokens + std::min(seqs, total_q), total_q);   // each sequence may end in one of its own
+    p.levels = (max_ctx + bn - 1) / bn;
     const int64_t pairs = (int64_t)p.tiles * kv_heads;
     // key tiles of the longest row tile, and of an average one: the mean over a sequence's new rows is half of them less
     double keys = max_ctx, mean = std::max(0.5 * max_ctx, max_ctx - 0.5 * total_q / std::max(1, seqs));
@@ -983,12 +1026,10 @@ static PrefillPlan prefill_plan(int D, int kv_heads, int seqs, int total_q, int 
         keys = std::min(keys, (double)window + tokens + bn);
         mean = std::min(mean, keys);
     }
-    const double longest = keys / bn, work = std::max(1.0, mean / bn) * pairs;
-    const double mean_pieces = (double)sms / pairs - 0.5;        // of a tile, when all run at once; the last piece of a tile is half full
-    const double fit = mean_pieces > 0 ? std::max(256.0 / bn, mean / bn / mean_pieces) : 512.0 / bn;
-    const double piece = std::max(std::min(fit, 512.0 / bn), work / (2.0 * sms));
-    p.chunks = (int)std::max(1.0, std::min(longest / piece, 1024.0));
+    const double longest = keys / bn, each = std::max(1.0, mean / bn), half = 0.5 * each * pairs / sms;
+    p.chunks = (int)std::max(1.0, std::min(longest / std::max((pairs <= sms ? 256.0 : 512.0) / bn, half), 1024.0));
     p.chunk_tiles = std::max(1, (int)((longest + p.chunks - 1) / p.chunks));
+    if (pairs <= sms) p.chunk_tiles = std::max(p.chunk_tiles, (int)std::ceil(each / ((double)sms / pairs - 0.5)));   // a tile's last chunk is half full
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
     const size_t parts = p.chunks > 1 ? (size_t)pairs * p.chunks : 0;
     p.part = up(parts * rows * D * 4);
@@ -1058,7 +1099,8 @@ static int32_t launch_prefill(cudaStream_t s, PrefillArgs a) {
     paged_prefill_kernel<D, FEAT><<<a.tiles * a.c.kv_heads * a.chunks, C::THREADS, C::TOTAL, s>>>(qm, km, vm, a);
     LTHN_CUDA_TRY(cudaGetLastError());
     if (a.chunks > 1) {
-        const bool few = a.chunks <= 8;
+        const int64_t ctas = (int64_t)a.tiles * a.c.kv_heads * (C::ROWS / 32 * (D / 8));    // of CG = 8; an SM runs 8
+        const bool few = a.chunks <= 8 || ctas > 16 * a.sms;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(a.tiles, a.c.kv_heads, C::ROWS / 32 * (few ? D / 64 : D / 8)); cfg.blockDim = dim3(256); cfg.stream = s;
         cudaLaunchAttribute at[1];
@@ -1130,7 +1172,7 @@ int32_t lthn_paged_prefill_attention(void* stream, const lthn_paged_kv* cache, c
     a.q = q; a.out = out; a.q_start = q_start; a.lens = kv_lens; a.lse = lse;
     a.seqs = seqs; a.total_q = total_q; a.Hq = q_heads; a.G = q_heads / cache->kv_heads;
     a.tokens = 128 / a.G;
-    a.tiles = p.tiles; a.chunks = p.chunks; a.chunk_tiles = p.chunk_tiles;
+    a.tiles = p.tiles; a.chunks = p.chunks; a.chunk_tiles = p.chunk_tiles; a.levels = p.levels; a.sms = paged_sm_count();
     a.part = (float4*)workspace;
     a.ml = (float2*)((char*)workspace + p.part);
     a.desc = (int4*)((char*)workspace + p.part + p.ml);
