@@ -419,6 +419,21 @@ def test_prefill_few_rows_long_axis(lthn, D, kv, G, new, past, ctx):
     check_prefill(lthn, c, rng.standard_normal((sum(new), kv * G, D)), new, ctx=ctx)
 
 
+@pytest.mark.parametrize("mask", [{}, dict(slopes=True), dict(slopes=True, window=333, prefix=40)], ids=str)
+@pytest.mark.parametrize("D,kv,G,seqs", [(128, 1, 4, 2), (64, 2, 1, 5), (256, 1, 2, 3), (64, 1, 2, 32), (128, 1, 2, 33)])
+@pytest.mark.parametrize("ctx", [0, 20000])
+def test_prefill_chunks_of_unlike_lengths(lthn, mask, D, kv, G, seqs, ctx):
+    """Sequences of one to several row tiles on contexts of none to thousands of keys: where their keys are cut depends on the lengths and on
+    their number."""
+    rng = np.random.default_rng(27 + seqs)
+    new = [int(n) for n in rng.integers(1, 12 if seqs > 5 else 300, seqs)]
+    past = [int(n) for n in 2.0 ** rng.uniform(0, 9 if seqs > 5 else 12, seqs)]
+    lens = [a + b for a, b in zip(new, past)]
+    c = HostCache(rng, lens, 16, kv, D)
+    o, kws = options(lthn, rng, kv * G, lens, **mask)
+    check_prefill(lthn, c, rng.standard_normal((sum(new), kv * G, D)), new, o, kws, ctx=ctx)
+
+
 def test_prefill_rows_nobody_owns_and_rows_before_the_first_position(lthn):
     rng = np.random.default_rng(23)
     new, lens = [10, 6, 4], [4, 6, 0]          # sequence 0 has more queries than positions, sequence 2 has none at all
