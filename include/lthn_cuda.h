@@ -319,7 +319,7 @@ typedef struct {
  *   base^(-2i/head_dim) the frequencies of lthn_rmsnorm_rope; scaled frequencies serve long contexts):
  *   pairs (i, i + head_dim/2), or neighbours (2i, 2i+1) with interleaved = 1.
  * Angles are formed in f64, everything else in f32, each result is rounded once. row_seq[r] < 0 marks a padding row: nothing of
- * it is read or written. Rows must name different positions: which of two equal ones stays is not defined.
+ * it is written (q, k and v have its place all the same). Rows must name different positions: which of two equal ones stays is not defined.
  * dtype (LTHN_DTYPE_*) is the type of q, k and v, q_dtype that of q_out; strides are elements between
  * rows (0 -> dense), multiples of 8, so that the three may be slices of one projection's output; all pointers
  * 16-byte aligned. q_out may be q itself (same type and stride). rows == 0 is a successful no-op.
@@ -377,7 +377,9 @@ int32_t lthn_paged_sdpa_decode(void* stream, const lthn_paged_kv* cache, const l
  * different sequences do not see each other. Rows that q_start leaves out are not touched, neither is their
  * lse; a sequence with more query rows than positions has empty rows in front. Scores and sums are f32, the weights
  * are rounded to bf16 for the second product, as in lthn_prefill_attention. max_ctx (0: the table's rows) bounds
- * kv_lens for the choice of how the work is cut; longer sequences are still computed right. A NaN or infinity in a
+ * kv_lens: it decides how finely a long context can be cut, and with it the workspace; longer sequences are still computed
+ * right. Lengths are read on the device and few rows are cut by the lengths themselves, so a captured call replays with new
+ * ones and a generous max_ctx costs workspace, not time. A NaN or infinity in a
  * value row that some query of a tile sees may reach the other queries of that tile (up to 256 rows of tokens times
  * query heads of a kv head). At most 128 query heads per kv head. Workspace and strides as above. */
 int32_t lthn_paged_prefill_attention_workspace(const lthn_paged_kv* cache, int32_t seqs, int32_t total_q, int32_t q_heads, int32_t max_ctx,
