@@ -599,6 +599,60 @@ def test_captured_steps_replay_with_new_lengths(lthn):
     assert lthn.device_status() == 0
 
 
+@pytest.mark.parametrize("D,G,extra", [(128, 4, 0), (64, 3, 64), (256, 2, 8)])
+def test_captured_prompt_chunks_in_strided_rows(lthn, D, G, extra):
+    """Queries and outputs inside wider rows, two graphs on two streams at once, replayed with other chunks and lengths: from drafts behind long
+    contexts, which are cut and joined, to prompts."""
+    rng = np.random.default_rng(33 + D)
+    kv, page, cap, total = 2, 16, [2000, 700, 40], 310
+    Hq = kv * G
+    qs, os = Hq * D + extra + (D if extra % D == 0 else 0), Hq * D + 24
+    c = HostCache(rng, cap, page, kv, D)
+    dev = c.device(lthn)
+    lanes = []
+    for _ in range(2):
+        st = lthn.Stream()
+        w = dict(q=lthn.Buf(total * qs * 2), out=lthn.Buf(total * os * 2), start=lthn.Buf(16), lens=lthn.Buf(12),
+                 ws=lthn.Buf(lthn.paged_prefill_attention_workspace(dev, 3, total, Hq)))
+        for b in w.values():
+            b.zero()
+        lthn.sync()
+
+        def step():
+            lthn.paged_prefill_attention(dev, w["q"], w["start"], w["lens"], 3, total, Hq, w["out"], w["ws"], q_stride=qs, out_stride=os, stream=st)
+        step()
+        st.sync()
+        w["graph"] = lthn.Graph(st)
+        with w["graph"]:
+            step()
+        lanes.append(w)
+    plans = [([4, 1, 9], [2000, 650, 40]), ([0, 270, 30], [1999, 270, 31]), ([150, 0, 2], [170, 700, 2]), ([1, 1, 1], [1, 700, 0])]
+    for t in range(0, len(plans), 2):
+        data = []
+        for w, (new, lens) in zip(lanes, plans[t:t + 2]):
+            q = np.full((total, qs), 9.0)
+            q[:, :Hq * D] = rng.standard_normal((total, Hq * D))
+            q = to_bf16(q)
+            w["q"].upload(q)
+            w["out"].upload(to_bf16(np.full((total, os), 5.0)))
+            start = 3 + np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+            w["start"].upload(start)
+            w["lens"].upload(np.array(lens, dtype=np.int32))
+            data.append((from_bf16(q)[:, :Hq * D].reshape(total, Hq, D), start, new, lens))
+        lthn.sync()
+        for w in lanes:
+            w["graph"].launch()
+        lthn.sync()
+        assert lthn.device_status() == 0
+        for w, (q, start, new, lens) in zip(lanes, data):
+            got = from_bf16(w["out"].download(np.uint16, (total, os)))
+            assert np.all(got[:, Hq * D:] == 5.0) and np.all(got[:start[0]] == 5.0) and np.all(got[start[-1]:] == 5.0)
+            for s in range(3):
+                rows = slice(start[s], start[s + 1])
+                want, _, mag = attention(c, s, q[rows], lens[s] - new[s], lens[s])
+                close(got[rows, :Hq * D].reshape(-1, Hq, D), want, 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + W) * mag)
+
+
 def test_offsets_past_32_bits(lthn):
     """Pages far apart, K and V side by side in one allocation: element offsets beyond 2^32 bytes and 2^31 elements."""
     rng = np.random.default_rng(33)
