@@ -12,7 +12,8 @@
 // lengths are, and no host knowledge of them is needed. (Without the start's unit the CTAs with many short
 // triples came last: 32 rows of 257 to 4608 keys, first CTA done after 66 us, last after 99.) A triple that lies within one CTA
 // is finished there; otherwise each CTA that holds part of it leaves (max, sum, unnormalised output) in its slot of the workspace
-// - a CTA has at most two such parts, its first and its last - and a second kernel joins them.
+// - a CTA has at most two such parts, its first and its last - and a second kernel joins them. A few short triples would wait for the
+// second launch longer than for their keys; each of those goes to a cluster of 8 CTAs, whose parts meet in distributed shared memory.
 //
 // A warp owns 16 keys of each piece and runs on its own: its own ring of shared-memory stages filled by its own cp.async (16 bytes,
 // rows padded by 16 bytes so that ldmatrix is free of bank conflicts), its own running maximum, sum and output; the
@@ -54,6 +55,7 @@ constexpr int DEC_WARPS = 4;
 constexpr int DEC_THREADS = DEC_WARPS * 32;
 constexpr int DEC_WK = 16;                       // keys of a warp's tile
 constexpr int DEC_TILE = DEC_WARPS * DEC_WK;
+constexpr int DEC_CLUSTER = 8;                   // CTAs of a cluster
 
 template <int D, int MODE>
 struct DecCfg {
@@ -100,7 +102,28 @@ struct DecSeg {
     int i0, i1;           // pieces
 };
 
-template <int D, int MODE>
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// address of a CTA's copy of a shared-memory variable
+__device__ __forceinline__ uint32_t cluster_map(uint32_t addr, int cta) {
+    uint32_t d;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(addr), "r"(cta));
+    return d;
+}
+__device__ __forceinline__ float4 cluster_ld4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 cluster_ld2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+
+// CLUSTER: a triple belongs to the DEC_CLUSTER CTAs of a cluster, an even share of its pieces each, and their parts meet in shared memory.
+template <int D, int MODE, bool CLUSTER>
 __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) paged_decode_kernel(const DecodeArgs a) {
     using C = DecCfg<D, MODE>;
     constexpr int HB = C::HB, NST = C::NST, PITCH = C::PITCH;
@@ -112,6 +135,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
     __shared__ float s_m[DEC_WARPS][16], s_l[DEC_WARPS][16];
     __shared__ int s_scan[DEC_WARPS];
     __shared__ int s_row, s_base;
+    __shared__ __align__(8) float2 s_part[HB];    // CLUSTER: maximum and sum of this CTA's part
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
@@ -120,57 +144,51 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
     const uint32_t ring = smem_u32(dec_smem) + warp * NST * C::STAGE;
     const int triples = a.c.kv_heads * a.nb;      // per row
 
-    pdl_trigger();
+    if (!CLUSTER) pdl_trigger();
     // ---- this CTA's units ------------------------------------------------------------------------------
-    auto units_of = [&](int r) { return r < a.rows ? decode_units(decode_tiles(a, r).n) : 0; };
-    int incl, mine = units_of(tid);
-    int total = paged_block_scan<DEC_WARPS>(mine, incl, s_scan);
-    int64_t U = total;                            // per triple of a row first
-    const bool note = a.rows > DEC_THREADS && blockIdx.x == 0;   // the join looks them up
-    if (note) a.base[tid] = incl - mine;
-    for (int r0 = DEC_THREADS; r0 < a.rows; r0 += DEC_THREADS) {
-        int x;
-        const int n = units_of(r0 + tid), more = paged_block_scan<DEC_WARPS>(n, x, s_scan);
-        if (note && r0 + tid < a.rows) a.base[r0 + tid] = U + x - n;
-        U += more;
-    }
-    if (note && tid == 0) a.base[a.rows] = U;
-    U *= triples;
-    const int ctas = (int)min((int64_t)a.ctas, U);   // none of them without a unit
-    if ((int)blockIdx.x >= ctas) return;
-    const int64_t u0 = decode_div(U * blockIdx.x, ctas), u1 = decode_div(U * (blockIdx.x + 1), ctas);
-    // the row that holds unit u0
-    int64_t base = 0;
+    int64_t u = 0, u1 = 0, base = 0;
     int row = 0;
-    for (int r0 = 0;;) {
-        if ((base + total) * triples > u0) {
-            if (mine > 0 && (base + incl) * triples > u0 && (base + incl - mine) * triples <= u0) { s_row = r0 + tid; s_base = incl - mine; }
-            __syncthreads();
-            row = s_row;
-            base = (base + s_base) * triples;     // first unit of the row
-            break;
+    if (!CLUSTER) {
+        auto units_of = [&](int r) { return r < a.rows ? decode_units(decode_tiles(a, r).n) : 0; };
+        int incl, mine = units_of(tid);
+        int total = paged_block_scan<DEC_WARPS>(mine, incl, s_scan);
+        int64_t U = total;                            // per triple of a row first
+        const bool note = a.rows > DEC_THREADS && blockIdx.x == 0;   // the join looks them up
+        if (note) a.base[tid] = incl - mine;
+        for (int r0 = DEC_THREADS; r0 < a.rows; r0 += DEC_THREADS) {
+            int x;
+            const int n = units_of(r0 + tid), more = paged_block_scan<DEC_WARPS>(n, x, s_scan);
+            if (note && r0 + tid < a.rows) a.base[r0 + tid] = U + x - n;
+            U += more;
         }
-        base += total;
-        r0 += DEC_THREADS;
-        mine = units_of(r0 + tid);
-        total = paged_block_scan<DEC_WARPS>(mine, incl, s_scan);
+        if (note && tid == 0) a.base[a.rows] = U;
+        U *= triples;
+        const int ctas = (int)min((int64_t)a.ctas, U);   // none of them without a unit
+        if ((int)blockIdx.x >= ctas) return;
+        const int64_t u0 = decode_div(U * blockIdx.x, ctas);
+        u = u0;
+        u1 = decode_div(U * (blockIdx.x + 1), ctas);
+        // the row that holds unit u0
+        for (int r0 = 0;;) {
+            if ((base + total) * triples > u0) {
+                if (mine > 0 && (base + incl) * triples > u0 && (base + incl - mine) * triples <= u0) { s_row = r0 + tid; s_base = incl - mine; }
+                __syncthreads();
+                row = s_row;
+                base = (base + s_base) * triples;     // first unit of the row
+                break;
+            }
+            base += total;
+            r0 += DEC_THREADS;
+            mine = units_of(r0 + tid);
+            total = paged_block_scan<DEC_WARPS>(mine, incl, s_scan);
+        }
     }
     const float s_in = a.o.softcap > 0.f ? a.o.scale / a.o.softcap : a.o.scale * LOG2E, s_cap = a.o.softcap * LOG2E;
 
-    int64_t u = u0;
+    const int rank = blockIdx.x % DEC_CLUSTER, my_triple = blockIdx.x / DEC_CLUSTER;   // of a cluster
+    bool begun = false;
     auto next_seg = [&](DecSeg& d) {              // the next part of a triple; false: there is none
-        while (u < u1 && row < a.rows) {
-            const KeyTiles kt = decode_tiles(a, row);
-            const int w = decode_units(kt.n);
-            if (w == 0) { row++; continue; }
-            const int64_t in_row = u - base;
-            const int triple = (int)decode_div(in_row, w), v = (int)(in_row - (int64_t)triple * w), take = (int)min((int64_t)(w - v), u1 - u);
-            u += take;
-            const int at = row;
-            if (u - base >= (int64_t)w * triples) { base += (int64_t)w * triples; row++; }
-            d.i0 = max(v - DEC_START, 0);
-            d.i1 = max(v + take - DEC_START, 0);
-            if (d.i0 >= d.i1) continue;           // its start alone: the next CTA begins it
+        auto fill = [&](int at, int triple, const KeyTiles& kt) {
             d.row = at;
             d.kvh = triple / a.nb;
             d.bundle = triple - d.kvh * a.nb;
@@ -178,9 +196,33 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
             d.prefix = a.o.prefix ? min(max(a.o.prefix[at], 0), d.len) : 0;
             d.lo = a.o.window > 0 ? max(0, d.len - a.o.window) : 0;
             d.kt = kt;
-            return true;
+        };
+        if constexpr (CLUSTER) {
+            if (begun) return false;
+            begun = true;
+            const int at = my_triple / triples;
+            fill(at, my_triple - at * triples, decode_tiles(a, at));
+            d.i0 = d.kt.n * rank / DEC_CLUSTER;   // (at most 2^20 pieces)
+            d.i1 = d.kt.n * (rank + 1) / DEC_CLUSTER;
+            return true;                          // also where its share is empty: it then adds nothing
+        } else {
+            while (u < u1 && row < a.rows) {
+                const KeyTiles kt = decode_tiles(a, row);
+                const int w = decode_units(kt.n);
+                if (w == 0) { row++; continue; }
+                const int64_t in_row = u - base;
+                const int triple = (int)decode_div(in_row, w), v = (int)(in_row - (int64_t)triple * w), take = (int)min((int64_t)(w - v), u1 - u);
+                u += take;
+                const int at = row;
+                if (u - base >= (int64_t)w * triples) { base += (int64_t)w * triples; row++; }
+                d.i0 = max(v - DEC_START, 0);
+                d.i1 = max(v + take - DEC_START, 0);
+                if (d.i0 >= d.i1) continue;           // its start alone: the next CTA begins it
+                fill(at, triple, kt);
+                return true;
+            }
+            return false;
         }
-        return false;
     };
 
     // ---- loads: piece i of a part goes to stage (sb + i - i0) % NST of this warp's ring, where sb counts the pieces before ------
@@ -271,6 +313,15 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
         }
     };
 
+    // four columns from d of a finished query head
+    auto store_out = [&](int at_row, int head, int d, float m, float l, const float (&x)[4]) {
+        const float inv = l > 0.f ? 1.0f / l : 0.f;
+        const int64_t at = at_row * a.out_stride + (int64_t)head * D + d;
+        if (MODE == DEC_F32_8) *(float4*)((float*)a.out + at) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        else *(uint2*)((uint16_t*)a.out + at) = make_uint2(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv));
+        if (a.lse && d == 0) a.lse[(int64_t)at_row * a.Hq + head] = (m + log2f(l)) * 0.6931471805599453f;
+    };
+
     // One round: the next part's first keys set out, the last part's warps meet in the stage they leave free and store it, then the next part
     // is worked through. (One copy of this code: it is long, and a short call waits for its instructions too.)
     float acc[ND][4], mrun[2], lrun[2];
@@ -278,7 +329,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
     for (int sn = 0;; sn = (sb + S.i1 - S.i0) % NST, have = true) {
         const bool more = next_seg(N);
         if (more) begin(N, sn);
-        const int red_at = ((sn + NST - 1) % NST) * C::STAGE;
+        const int red_at = (CLUSTER ? NST - 1 : (sn + NST - 1) % NST) * C::STAGE;   // (nothing comes after a cluster's part)
         if (have) {
             float* red = (float*)(dec_smem + warp * NST * C::STAGE + red_at);   // [HB][D]
 #pragma unroll
@@ -303,7 +354,8 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
         if (more) load_queries(N, qx);
         if (have) {
             const int h0 = S.kvh * a.G + S.bundle * HB, nh = min(HB, a.G - S.bundle * HB);   // first query head, heads
-            const bool whole = S.i1 - S.i0 == S.kt.n;
+            const bool whole = !CLUSTER && S.i1 - S.i0 == S.kt.n;
+            float* mine = (float*)dec_smem;                   // CLUSTER: this CTA's part, in a stage nobody uses any more
             const int slot = 2 * blockIdx.x + (S.i0 > 0 ? 0 : 1);
             for (int idx = tid; idx < nh * (D / 4); idx += DEC_THREADS) {
                 const int h = idx / (D / 4), d = (idx - h * (D / 4)) * 4;
@@ -318,16 +370,43 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
                     x[0] = fmaf(y.x, e, x[0]); x[1] = fmaf(y.y, e, x[1]); x[2] = fmaf(y.z, e, x[2]); x[3] = fmaf(y.w, e, x[3]);
                 }
                 if (whole) {
-                    const float inv = l > 0.f ? 1.0f / l : 0.f;
-                    const int64_t at = S.row * a.out_stride + (int64_t)(h0 + h) * D + d;
-                    if (MODE == DEC_F32_8) *(float4*)((float*)a.out + at) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-                    else *(uint2*)((uint16_t*)a.out + at) = make_uint2(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv));
-                    if (a.lse && d == 0) a.lse[(int64_t)S.row * a.Hq + h0 + h] = (m + log2f(l)) * 0.6931471805599453f;
+                    store_out(S.row, h0 + h, d, m, l, x);
+                } else if (CLUSTER) {
+                    *(float4*)(mine + h * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+                    if (d == 0) s_part[h] = make_float2(m, l);
                 } else {
                     *(float4*)(a.part + ((int64_t)slot * HB + h) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
                     if (d == 0) a.ml[slot * HB + h] = make_float2(m, l);
                 }
             }
+        }
+        if (CLUSTER && have) {
+            cluster_sync();                                   // all parts of the triple are there
+            const int h0 = S.kvh * a.G + S.bundle * HB, nh = min(HB, a.G - S.bundle * HB);
+            const uint32_t x_at = smem_u32(dec_smem), ml_at = smem_u32(s_part);
+            for (int idx = rank * DEC_THREADS + tid; idx < nh * (D / 4); idx += DEC_CLUSTER * DEC_THREADS) {
+                const int h = idx / (D / 4), d = (idx - h * (D / 4)) * 4;
+                float2 ml[DEC_CLUSTER];
+                float4 y[DEC_CLUSTER];
+                float m = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < DEC_CLUSTER; c++) {
+                    ml[c] = cluster_ld2(cluster_map(ml_at + h * 8, c));
+                    y[c] = cluster_ld4(cluster_map(x_at + (h * D + d) * 4, c));
+                }
+#pragma unroll
+                for (int c = 0; c < DEC_CLUSTER; c++) m = fmaxf(m, ml[c].x);
+                const float ref = m == -INFINITY ? 0.f : m;
+                float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < DEC_CLUSTER; c++) {
+                    const float e = ex2(ml[c].x - ref);
+                    l = fmaf(ml[c].y, e, l);
+                    x[0] = fmaf(y[c].x, e, x[0]); x[1] = fmaf(y[c].y, e, x[1]); x[2] = fmaf(y[c].z, e, x[2]); x[3] = fmaf(y[c].w, e, x[3]);
+                }
+                store_out(S.row, h0 + h, d, m, l, x);
+            }
+            cluster_sync();                                   // nobody reads this CTA's memory any more
         }
         if (!more) break;
         store_queries(qx);                                    // (all warps are through with the last part's)
@@ -570,7 +649,7 @@ static DecodePlan decode_plan(int D, int kv_heads, int rows, int q_heads, int dt
     return p;
 }
 
-template <int D, int MODE>
+template <int D, int MODE, bool CLUSTER>
 static int32_t launch_decode_kernel(cudaStream_t s, const DecodeArgs& a) {
     using C = DecCfg<D, MODE>;
     static uint32_t attr_devs = 0;
@@ -580,26 +659,49 @@ static int32_t launch_decode_kernel(cudaStream_t s, const DecodeArgs& a) {
     {
         std::lock_guard<std::mutex> lk(mu);
         if (!(attr_devs >> (dev & 31) & 1)) {
-            LTHN_CUDA_TRY(cudaFuncSetAttribute(paged_decode_kernel<D, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+            LTHN_CUDA_TRY(cudaFuncSetAttribute(paged_decode_kernel<D, MODE, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
             attr_devs |= 1u << (dev & 31);
         }
     }
-    paged_decode_kernel<D, MODE><<<a.ctas, DEC_THREADS, C::SMEM, s>>>(a);
-    LTHN_CUDA_TRY(cudaGetLastError());
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.Hq, a.rows); cfg.blockDim = dim3(128); cfg.stream = s;
     cudaLaunchAttribute at[1];
+    cfg.attrs = at; cfg.numAttrs = 1; cfg.stream = s;
+    if (CLUSTER) {
+        cfg.gridDim = dim3(a.rows * a.c.kv_heads * a.nb * DEC_CLUSTER); cfg.blockDim = dim3(DEC_THREADS); cfg.dynamicSmemBytes = C::SMEM;
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim = {DEC_CLUSTER, 1, 1};
+        LTHN_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_decode_kernel<D, MODE, CLUSTER>, a));
+        return LTHN_OK;
+    }
+    paged_decode_kernel<D, MODE, CLUSTER><<<a.ctas, DEC_THREADS, C::SMEM, s>>>(a);
+    LTHN_CUDA_TRY(cudaGetLastError());
+    cfg.gridDim = dim3(a.Hq, a.rows); cfg.blockDim = dim3(128);
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at; cfg.numAttrs = 1;
     LTHN_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_decode_join_kernel<D>, a, C::HB, MODE == DEC_F32_8 ? 1 : 0));
     return LTHN_OK;
 }
+// A cluster per triple, in one launch, where all clusters run at once and the longest row that a call can have gives a CTA no more than
+// 512 / D pieces more than an even share over the whole GPU would: that many take as long as the join (8 triples, head_dim 128, bf16: 512 keys
+// 7.0 us in even shares, 4.7 in clusters; 2048 keys 8.8, 7.9; 4096 keys 10.7, 11.6. 4 triples, head_dim 256, f32: 512 keys 8.9, 6.5; 1280
+// keys 10.5, 10.4; 2048 keys 11.0, 12.4). 16 clusters need two CTAs per SM: 16 triples of head_dim 256, 1 key: 6.8, 10.3.
+template <int D>
+static bool decode_clusters(const DecodeArgs& a) {
+    const int64_t triples = (int64_t)a.rows * a.c.kv_heads * a.nb;
+    if (triples * DEC_CLUSTER > (D == 256 ? 64 : 128)) return false;
+    int64_t pieces = ((int64_t)a.c.capacity + DEC_TILE - 1) / DEC_TILE;
+    if (a.o.window > 0 && !a.o.prefix) pieces = std::min<int64_t>(pieces, a.o.window / DEC_TILE + 2);
+    return pieces * (1.0 / DEC_CLUSTER - (double)triples / a.ctas) * D <= 512.0;
+}
+template <int D, int MODE>
+static int32_t launch_decode_form(cudaStream_t s, const DecodeArgs& a) {
+    return decode_clusters<D>(a) ? launch_decode_kernel<D, MODE, true>(s, a) : launch_decode_kernel<D, MODE, false>(s, a);
+}
 template <int D>
 static int32_t launch_decode_mode(cudaStream_t s, const DecodeArgs& a, int mode) {
-    if (mode == DEC_BF16_16) return launch_decode_kernel<D, DEC_BF16_16>(s, a);
-    if (mode == DEC_BF16_8) return launch_decode_kernel<D, DEC_BF16_8>(s, a);
-    return launch_decode_kernel<D, DEC_F32_8>(s, a);
+    if (mode == DEC_BF16_16) return launch_decode_form<D, DEC_BF16_16>(s, a);
+    if (mode == DEC_BF16_8) return launch_decode_form<D, DEC_BF16_8>(s, a);
+    return launch_decode_form<D, DEC_F32_8>(s, a);
 }
 
 }  // namespace lthn

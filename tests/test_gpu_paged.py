@@ -236,6 +236,31 @@ def test_decode_masks(lthn, mask, D, kv, G, f32):
     check_decode(lthn, c, rng.standard_normal((len(lens), kv * G, D)), f32, o, kws)
 
 
+def widen(c, rows):
+    """The same cache under a table with room for `rows` more rows a sequence: how a call is dealt out depends on the longest row it can have."""
+    more = (rows + c.ps - 1) // c.ps
+    c.table = np.ascontiguousarray(np.hstack([c.table, np.full((len(c.lens), more), -7, dtype=np.int32)]))
+    c.table_stride += more
+    return c
+
+
+@pytest.mark.parametrize("D,kv,G,page,f32,major,lens", DECODE)
+def test_decode_under_a_wide_table(lthn, D, kv, G, page, f32, major, lens):
+    rng = np.random.default_rng(len(lens) + D + G)
+    c = widen(HostCache(rng, lens, page, kv, D, major), 1 << 17)
+    check_decode(lthn, c, rng.standard_normal((len(lens), kv * G, D)), f32)
+
+
+@pytest.mark.parametrize("mask", MASKS, ids=str)
+@pytest.mark.parametrize("D,kv,G,f32,rows", [(128, 1, 3, True, 1 << 17), (64, 1, 9, False, 1 << 17), (256, 1, 4, False, 0)])
+def test_decode_masks_few_rows(lthn, mask, D, kv, G, f32, rows):
+    rng = np.random.default_rng(34)
+    lens = [400, 1, 0, 99, 64, 163, 1023]
+    c = widen(HostCache(rng, lens, 24, kv, D), rows)
+    o, kws = options(lthn, rng, kv * G, lens, **mask)
+    check_decode(lthn, c, rng.standard_normal((len(lens), kv * G, D)), f32, o, kws)
+
+
 def test_decode_many_rows_and_one_long(lthn):
     """More rows than a block scans at once; one row far longer than the others is cut over many blocks."""
     rng = np.random.default_rng(11)
