@@ -13,7 +13,7 @@
 // triples came last: 32 rows of 257 to 4608 keys, first CTA done after 66 us, last after 99.) A triple that lies within one CTA
 // is finished there; otherwise each CTA that holds part of it leaves (max, sum, unnormalised output) in its slot of the workspace
 // - a CTA has at most two such parts, its first and its last - and a second kernel joins them. A few short triples would wait for the
-// second launch longer than for their keys; each of those goes to a cluster of 8 CTAs, whose parts meet in distributed shared memory.
+// second launch longer than for their keys; each of those goes to a cluster of 8 or 16 CTAs, whose parts meet in distributed shared memory.
 //
 // A warp owns 16 keys of each piece and runs on its own: its own ring of shared-memory stages filled by its own cp.async (16 bytes,
 // rows padded by 16 bytes so that ldmatrix is free of bank conflicts), its own running maximum, sum and output; the
@@ -55,7 +55,6 @@ constexpr int DEC_WARPS = 4;
 constexpr int DEC_THREADS = DEC_WARPS * 32;
 constexpr int DEC_WK = 16;                       // keys of a warp's tile
 constexpr int DEC_TILE = DEC_WARPS * DEC_WK;
-constexpr int DEC_CLUSTER = 8;                   // CTAs of a cluster
 
 template <int D, int MODE>
 struct DecCfg {
@@ -122,8 +121,8 @@ __device__ __forceinline__ float2 cluster_ld2(uint32_t addr) {
     return v;
 }
 
-// CLUSTER: a triple belongs to the DEC_CLUSTER CTAs of a cluster, an even share of its pieces each, and their parts meet in shared memory.
-template <int D, int MODE, bool CLUSTER>
+// CLUSTER > 0: a triple belongs to a cluster of that many CTAs, an even share of its pieces each, and their parts meet in shared memory.
+template <int D, int MODE, int CLUSTER>
 __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) paged_decode_kernel(const DecodeArgs a) {
     using C = DecCfg<D, MODE>;
     constexpr int HB = C::HB, NST = C::NST, PITCH = C::PITCH;
@@ -185,7 +184,8 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
     }
     const float s_in = a.o.softcap > 0.f ? a.o.scale / a.o.softcap : a.o.scale * LOG2E, s_cap = a.o.softcap * LOG2E;
 
-    const int rank = blockIdx.x % DEC_CLUSTER, my_triple = blockIdx.x / DEC_CLUSTER;   // of a cluster
+    constexpr int CC = CLUSTER > 0 ? CLUSTER : 1;
+    const int rank = blockIdx.x % CC, my_triple = blockIdx.x / CC;   // of a cluster
     bool begun = false;
     auto next_seg = [&](DecSeg& d) {              // the next part of a triple; false: there is none
         auto fill = [&](int at, int triple, const KeyTiles& kt) {
@@ -197,13 +197,13 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
             d.lo = a.o.window > 0 ? max(0, d.len - a.o.window) : 0;
             d.kt = kt;
         };
-        if constexpr (CLUSTER) {
+        if constexpr (CLUSTER > 0) {
             if (begun) return false;
             begun = true;
             const int at = my_triple / triples;
             fill(at, my_triple - at * triples, decode_tiles(a, at));
-            d.i0 = d.kt.n * rank / DEC_CLUSTER;   // (at most 2^20 pieces)
-            d.i1 = d.kt.n * (rank + 1) / DEC_CLUSTER;
+            d.i0 = d.kt.n * rank / CC;            // (at most 2^20 pieces)
+            d.i1 = d.kt.n * (rank + 1) / CC;
             return true;                          // also where its share is empty: it then adds nothing
         } else {
             while (u < u1 && row < a.rows) {
@@ -380,26 +380,26 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
                 }
             }
         }
-        if (CLUSTER && have) {
+        if constexpr (CLUSTER > 0) if (have) {
             cluster_sync();                                   // all parts of the triple are there
             const int h0 = S.kvh * a.G + S.bundle * HB, nh = min(HB, a.G - S.bundle * HB);
             const uint32_t x_at = smem_u32(dec_smem), ml_at = smem_u32(s_part);
-            for (int idx = rank * DEC_THREADS + tid; idx < nh * (D / 4); idx += DEC_CLUSTER * DEC_THREADS) {
+            for (int idx = rank * DEC_THREADS + tid; idx < nh * (D / 4); idx += CC * DEC_THREADS) {
                 const int h = idx / (D / 4), d = (idx - h * (D / 4)) * 4;
-                float2 ml[DEC_CLUSTER];
-                float4 y[DEC_CLUSTER];
+                float2 ml[CC];
+                float4 y[CC];
                 float m = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < DEC_CLUSTER; c++) {
+                for (int c = 0; c < CC; c++) {
                     ml[c] = cluster_ld2(cluster_map(ml_at + h * 8, c));
                     y[c] = cluster_ld4(cluster_map(x_at + (h * D + d) * 4, c));
                 }
 #pragma unroll
-                for (int c = 0; c < DEC_CLUSTER; c++) m = fmaxf(m, ml[c].x);
+                for (int c = 0; c < CC; c++) m = fmaxf(m, ml[c].x);
                 const float ref = m == -INFINITY ? 0.f : m;
                 float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int c = 0; c < DEC_CLUSTER; c++) {
+                for (int c = 0; c < CC; c++) {
                     const float e = ex2(ml[c].x - ref);
                     l = fmaf(ml[c].y, e, l);
                     x[0] = fmaf(y[c].x, e, x[0]); x[1] = fmaf(y[c].y, e, x[1]); x[2] = fmaf(y[c].z, e, x[2]); x[3] = fmaf(y[c].w, e, x[3]);
@@ -649,27 +649,47 @@ static DecodePlan decode_plan(int D, int kv_heads, int rows, int q_heads, int dt
     return p;
 }
 
-template <int D, int MODE, bool CLUSTER>
-static int32_t launch_decode_kernel(cudaStream_t s, const DecodeArgs& a) {
+// How many clusters of such CTAs (CLUSTER = 0: unknown) a device runs at once; the kernel is made ready on the way.
+template <int D, int MODE, int CLUSTER>
+static int32_t decode_ready(int* at_once) {
     using C = DecCfg<D, MODE>;
-    static uint32_t attr_devs = 0;
+    static uint32_t known_devs = 0;
+    static int known[32];
     static std::mutex mu;
     int dev = 0;
     LTHN_CUDA_TRY(cudaGetDevice(&dev));
-    {
-        std::lock_guard<std::mutex> lk(mu);
-        if (!(attr_devs >> (dev & 31) & 1)) {
-            LTHN_CUDA_TRY(cudaFuncSetAttribute(paged_decode_kernel<D, MODE, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
-            attr_devs |= 1u << (dev & 31);
-        }
+    dev &= 31;
+    std::lock_guard<std::mutex> lk(mu);
+    if (known_devs >> dev & 1) {
+        *at_once = known[dev];
+        return LTHN_OK;
     }
+    LTHN_CUDA_TRY(cudaFuncSetAttribute(paged_decode_kernel<D, MODE, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+    int n = 0;
+    if (CLUSTER > 0) {
+        if (CLUSTER > 8) LTHN_CUDA_TRY(cudaFuncSetAttribute(paged_decode_kernel<D, MODE, CLUSTER>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim = {CLUSTER, 1, 1};
+        cfg.gridDim = dim3(CLUSTER); cfg.blockDim = dim3(DEC_THREADS); cfg.dynamicSmemBytes = C::SMEM; cfg.attrs = at; cfg.numAttrs = 1;
+        LTHN_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, paged_decode_kernel<D, MODE, CLUSTER>, &cfg));
+    }
+    known_devs |= 1u << dev;
+    *at_once = known[dev] = n;
+    return LTHN_OK;
+}
+
+template <int D, int MODE, int CLUSTER>
+static int32_t launch_decode_kernel(cudaStream_t s, const DecodeArgs& a) {
+    using C = DecCfg<D, MODE>;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute at[1];
     cfg.attrs = at; cfg.numAttrs = 1; cfg.stream = s;
-    if (CLUSTER) {
-        cfg.gridDim = dim3(a.rows * a.c.kv_heads * a.nb * DEC_CLUSTER); cfg.blockDim = dim3(DEC_THREADS); cfg.dynamicSmemBytes = C::SMEM;
+    if (CLUSTER > 0) {
+        cfg.gridDim = dim3(a.rows * a.c.kv_heads * a.nb * CLUSTER); cfg.blockDim = dim3(DEC_THREADS); cfg.dynamicSmemBytes = C::SMEM;
         at[0].id = cudaLaunchAttributeClusterDimension;
-        at[0].val.clusterDim = {DEC_CLUSTER, 1, 1};
+        at[0].val.clusterDim = {CLUSTER, 1, 1};
         LTHN_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_decode_kernel<D, MODE, CLUSTER>, a));
         return LTHN_OK;
     }
@@ -681,21 +701,34 @@ static int32_t launch_decode_kernel(cudaStream_t s, const DecodeArgs& a) {
     LTHN_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_decode_join_kernel<D>, a, C::HB, MODE == DEC_F32_8 ? 1 : 0));
     return LTHN_OK;
 }
-// A cluster per triple, in one launch, where all clusters run at once and the longest row that a call can have gives a CTA no more than
-// 512 / D pieces more than an even share over the whole GPU would: that many take as long as the join (8 triples, head_dim 128, bf16: 512 keys
-// 7.0 us in even shares, 4.7 in clusters; 2048 keys 8.8, 7.9; 4096 keys 10.7, 11.6. 4 triples, head_dim 256, f32: 512 keys 8.9, 6.5; 1280
-// keys 10.5, 10.4; 2048 keys 11.0, 12.4). 16 clusters need two CTAs per SM: 16 triples of head_dim 256, 1 key: 6.8, 10.3.
+// The size of the clusters that a call's triples go to, 0: the list. A cluster per triple, in one launch, where all clusters run at once and
+// the longest row that a call can have gives a CTA no more than 512 / D pieces more than an even share over the whole GPU would: that
+// many take as long as the join (8 triples, head_dim 128, bf16: 512 keys 7.0 us in even shares, 4.6 in clusters of 8; 2048 keys 8.6, 7.9; 4096
+// keys 10.9, 11.5). For up to 4 triples with more than a piece for each of 8 CTAs the clusters have 16 (4 triples, head_dim 256, f32: 512
+// keys 8.9 us, of 8 6.5, of 16 7.1; 1280 keys 10.8, 10.3, 8.9; 2048 keys 10.7, 12.3, 8.8; 8 triples, head_dim 128, 1280 keys: 8.7, 6.7, 7.4).
 template <int D>
-static bool decode_clusters(const DecodeArgs& a) {
+static int decode_cluster(const DecodeArgs& a) {
     const int64_t triples = (int64_t)a.rows * a.c.kv_heads * a.nb;
-    if (triples * DEC_CLUSTER > (D == 256 ? 64 : 128)) return false;
+    if (triples > 16) return 0;
     int64_t pieces = ((int64_t)a.c.capacity + DEC_TILE - 1) / DEC_TILE;
     if (a.o.window > 0 && !a.o.prefix) pieces = std::min<int64_t>(pieces, a.o.window / DEC_TILE + 2);
-    return pieces * (1.0 / DEC_CLUSTER - (double)triples / a.ctas) * D <= 512.0;
+    const int size = triples <= 4 && pieces > 8 ? 16 : 8;
+    return pieces * (1.0 / size - (double)triples / a.ctas) * D <= 512.0 ? size : 0;
 }
 template <int D, int MODE>
 static int32_t launch_decode_form(cudaStream_t s, const DecodeArgs& a) {
-    return decode_clusters<D>(a) ? launch_decode_kernel<D, MODE, true>(s, a) : launch_decode_kernel<D, MODE, false>(s, a);
+    const int triples = (int)std::min<int64_t>((int64_t)a.rows * a.c.kv_heads * a.nb, 1 << 30), size = decode_cluster<D>(a);
+    int32_t rc;
+    int at_once = 0;
+    if (size == 16) {
+        if ((rc = decode_ready<D, MODE, 16>(&at_once))) return rc;
+        if (at_once >= triples) return launch_decode_kernel<D, MODE, 16>(s, a);
+    } else if (size == 8) {
+        if ((rc = decode_ready<D, MODE, 8>(&at_once))) return rc;
+        if (at_once >= triples) return launch_decode_kernel<D, MODE, 8>(s, a);
+    }
+    if ((rc = decode_ready<D, MODE, 0>(&at_once))) return rc;
+    return launch_decode_kernel<D, MODE, 0>(s, a);
 }
 template <int D>
 static int32_t launch_decode_mode(cudaStream_t s, const DecodeArgs& a, int mode) {

@@ -362,7 +362,8 @@ typedef struct {
  * are exact in bf16 and the products of q and of the weights with them are not rounded), bf16 rounds the weights and the result.
  * Lengths are read on the device, so a captured call replays with new ones. All work of the call is one list of
  * 64-key pieces of all rows, dealt out evenly over the GPU: no bound on the lengths is needed and a long
- * row does not wait for its own block. workspace: device memory of
+ * row does not wait for its own block. (A few rows that the table or the window keep short take one launch
+ * instead, a cluster of blocks per row and kv head.) workspace: device memory of
  * lthn_paged_sdpa_decode_workspace bytes, 16-byte aligned, uninitialised; nothing is kept in it between
  * calls, but calls that can overlap (two streams, two captured graphs) need one each. Strides are
  * elements between rows (0 -> dense), multiples of 8; q and out 16-byte aligned. At most 65535 rows. */
