@@ -163,6 +163,7 @@ __device__ __forceinline__ void pf_tma_4d(uint32_t dst, const CUtensorMap* map, 
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ void pf_prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void pf_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -301,6 +302,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     pdl_trigger();                                           // of the join, which waits for the end of this grid
     PfSeq seq_here = {0, 0, 0, 0};                           // the last warp, which finds the items: sequence `lane`
+    if (warp == C::SM_WARPS + 1 && lane < 3 && (lane < 2 ? a.box : a.q_box)) pf_prefetch_map(lane == 0 ? &k_map : lane == 1 ? &v_map : &q_map);
     if (warp == C::WARPS - 1) seq_here = prefill_seq(a, lane);
     if (tid == 0) {
         for (int s = 0; s < ST; s++) { mbar_init(&full[s], 96); mbar_init(&empty[s], 1); }
