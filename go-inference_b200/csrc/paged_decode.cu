@@ -8,8 +8,8 @@
 // as the M rows, where up to 16 heads cost what one costs.
 //
 // Work. The pieces (64 keys) of all (row, kv head, bundle of query heads) triples form one list, row by row, in which a triple begins with
-// a unit for its start; CTA c of C takes units [U c / C, U (c+1) / C) of the U, so every CTA has the same work whatever the
-// lengths are, and no host knowledge of them is needed. (Without the start's unit the CTAs with many short
+// two units for its start; CTA c of C takes units [U c / C, U (c+1) / C) of the U, so every CTA has the same work whatever the
+// lengths are, and no host knowledge of them is needed. (Without the units of the start the CTAs with many short
 // triples came last: 32 rows of 257 to 4608 keys, first CTA done after 66 us, last after 99.) A triple that lies within one CTA
 // is finished there; otherwise each CTA that holds part of it leaves (max, sum, unnormalised output) in its slot of the workspace
 // - a CTA has at most two such parts, its first and its last - and a second kernel joins them. A few short triples would wait for the
@@ -23,8 +23,8 @@
 //
 // Types. K and V are exact in bf16. Bundles of up to 8 heads leave half of the 16 MMA rows free, and the free rows carry
 // what rounding to bf16 cuts off:
-//   bf16, <= 8 heads   rows 0-7 the weights rounded to bf16, rows 8-15 the remainders: the weights are good to 2^-17
-//   bf16, > 8 heads    16 heads, weights rounded to bf16 (2^-9 each, no more than the rounding of the output)
+//   bf16, <= 8 heads   rows 0-7 the weights rounded to bf16, rows 8-15 the remainders: the weights are good to 2^-16
+//   bf16, > 8 heads    16 heads, weights rounded to bf16 (2^-8 each, no more than the rounding of the output)
 //   f32                q and the weights as three bf16 parts (24 bits), two MMAs: rows 0-7 high, 8-15 middle; rows 0-7 low
 #include "paged.cuh"
 

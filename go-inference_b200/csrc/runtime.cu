@@ -42,7 +42,7 @@ uint32_t* device_status_word() {
 }
 
 // The word next to it collects LTHN_STATUS_PAGED, so that a caller's bad page table is not taken for a
-// failed wait by the engine objects, which judge the first word after every forward.
+// failed wait by the engine objects, which look at the first word after every forward.
 uint32_t* device_paged_status_word() {
     uint32_t* w = device_status_word();
     return w ? w + 1 : nullptr;

@@ -117,6 +117,15 @@ def test_append(lthn, D, kv, G, page, fin, fq, norms, inter, rotary, major, rows
         assert np.all(got[~keep] == 3.0)
 
 
+@pytest.mark.parametrize("D,kv,G,page,fin,fq,norms,inter,rotary,major,rows,far", [
+    (128, 16, 2, 32, False, False, "qk", False, 128, False, 400, 50),     # more rows than are shared between blocks
+    (256, 8, 8, 16, True, True, "q", True, 192, True, 150, 4000),
+    (64, 12, 8, 24, False, True, "k", False, 64, False, 310, 9),
+])
+def test_append_blocks_of_several_passes(lthn, D, kv, G, page, fin, fq, norms, inter, rotary, major, rows, far):
+    test_append(lthn, D, kv, G, page, fin, fq, norms, inter, rotary, major, rows, far)
+
+
 def test_append_in_place_queries(lthn):
     rng = np.random.default_rng(1)
     rows, kv, Hq, D = 9, 2, 4, 128
