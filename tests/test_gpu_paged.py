@@ -315,6 +315,36 @@ def test_decode_bad_pages_are_reported(lthn):
     assert lthn.device_status() == 0            # the bad page is behind the length: nobody needs it
 
 
+def test_decode_bad_pages_and_strided_rows_under_a_wide_table(lthn):
+    """The refusals and the layout of the two tests beside this one where a call is dealt out over the whole GPU."""
+    rng = np.random.default_rng(35)
+    kv, G, D, rows = 2, 2, 64, 3
+    Hq = kv * G
+    c = widen(HostCache(rng, [100, 0, 470], 16, kv, D), 1 << 17)
+    q = np.full((rows, Hq * D + 16), np.nan)
+    q[:, :Hq * D] = rng.standard_normal((rows, Hq * D))
+    x, qb = upload(lthn, q, False)
+    dev = c.device(lthn)
+    out = lthn.Buf.from_array(to_bf16(np.full((rows + 1, Hq * D + 24), 7.0)))
+    ws = lthn.Buf(lthn.paged_sdpa_decode_workspace(dev, rows, Hq, lthn.BF16))
+
+    def run(lens):
+        lthn.paged_sdpa_decode(dev, qb, lthn.BF16, lthn.Buf.from_array(np.array(lens, dtype=np.int32)), rows, Hq, out, ws, q_stride=Hq * D + 16,
+                               out_stride=Hq * D + 24)
+    for lens in ([116, 0, 470], [100, 10 ** 6, 470]):        # an entry that is no page; a length behind the table
+        run(lens)
+        with pytest.raises(lthn.LthnError) as e:
+            lthn.device_status()
+        assert e.value.code == 1
+    run(c.lens)
+    assert lthn.device_status() == 0
+    got = from_bf16(out.download(np.uint16, (rows + 1, Hq * D + 24)))
+    assert np.all(got[:, Hq * D:] == 7.0) and np.all(got[rows] == 7.0)
+    for r, n in enumerate(c.lens):
+        want, _, mag = attention(c, r, x[r:r + 1, :Hq * D].reshape(1, Hq, D), n - 1, n)
+        close(got[r, :Hq * D].reshape(1, Hq, D), want, 2.0 ** -8 * np.abs(want) + W * mag)
+
+
 def test_decode_strided_rows_leave_the_rest(lthn):
     rng = np.random.default_rng(15)
     rows, kv, G, D = 3, 2, 2, 64
