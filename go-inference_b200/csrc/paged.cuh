@@ -22,7 +22,7 @@ struct PagedCache {
 // Score options with the defaults filled in. Scores are kept in units of log2, so that a weight is one ex2.
 struct AttnOpts {
     float scale;         // softmax scale
-    float softcap;       // 0: none
+    float softcap;       // 0: none; at most 2^126, also in units of the raw product
     const float* slopes;
     int window;          // 0: none
     const int32_t* prefix;
@@ -36,6 +36,8 @@ int32_t paged_check_device(const char* name, const char* what, const void* p);
 int paged_sm_count();
 
 #ifdef __CUDACC__
+// what a raw product is multiplied with to be in units of the cap; finite, so that a product of zero stays zero under the smallest caps
+__device__ __forceinline__ float paged_cap_in(const AttnOpts& o) { return fminf(o.scale / o.softcap, 3.402823466e38f); }
 __device__ __forceinline__ int paged_entry(const PagedCache& c, int pos) { return (int)(((uint64_t)(uint32_t)pos * c.div_mul) >> c.div_shift); }
 __device__ __forceinline__ int paged_row(const PagedCache& c, int pos) { return pos - paged_entry(c, pos) * c.page_size; }
 

@@ -80,6 +80,8 @@ int32_t paged_check_options(const char* name, const lthn_attn_options* o, int he
         a.scale = o->scale; a.softcap = o->softcap; a.slopes = o->slopes; a.window = std::min(o->window, 1 << 30); a.prefix = o->prefix_lens;
     }
     if (a.scale <= 0.f) a.scale = 1.0f / sqrtf((float)head_dim);
+    // Larger caps leave f32 in the units of the kernels; they differ from this one in scores next to the largest f32 alone.
+    a.softcap = std::min(a.softcap, 0x1p126f * std::min(a.scale, 1.0f));
     *out = a;
     return LTHN_OK;
 }

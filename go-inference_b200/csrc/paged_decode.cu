@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DecCfg<D, MODE>::CTAS_PER_SM) pag
             total = paged_block_scan<DEC_WARPS>(mine, incl, s_scan);
         }
     }
-    const float s_in = a.o.softcap > 0.f ? a.o.scale / a.o.softcap : a.o.scale * LOG2E, s_cap = a.o.softcap * LOG2E;
+    const float s_in = a.o.softcap > 0.f ? paged_cap_in(a.o) : a.o.scale * LOG2E, s_cap = a.o.softcap * LOG2E;
 
     constexpr int CC = CLUSTER > 0 ? CLUSTER : 1;
     const int rank = blockIdx.x % CC, my_triple = blockIdx.x / CC;   // of a cluster

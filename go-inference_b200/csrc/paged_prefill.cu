@@ -241,6 +241,11 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ float rcp_approx(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -269,6 +274,8 @@ struct PfCfg {
     static_assert(LAG <= ST - 3, "a slot is handed over before the one that frees its successor is waited for");
     static_assert(TOTAL <= 232448, "shared memory of a CTA");
 };
+
+constexpr float CAP_NEAR = 0.3f;   // up to this part of the cap, a score's tanh is taken from a polynomial
 
 // FEAT bit 0: tanh cap, bit 1: distance bias
 template <int D, int FEAT>
@@ -355,9 +362,9 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         const int r_token = r / a.G, r_head = r - r_token * a.G;
         const uint32_t lanes = tmem + ((uint32_t)wr << 16);
         const uint32_t s_addr = lanes + wg * C::S_COLS;
-        // plain scores stay as the product left them, the others are brought to log2 units first
-        const float c1 = FEAT ? 1.0f : a.o.scale * LOG2E;
-        const float cap2 = a.o.softcap * LOG2E, cin = FEAT & 1 ? 2.0f * LOG2E * a.o.scale / a.o.softcap : a.o.scale * LOG2E;
+        // scores stay in the units of the product, those with a distance bias are brought to log2 units first
+        const float c1 = FEAT & 2 ? 1.0f : a.o.scale * LOG2E, c_in = a.o.scale * LOG2E;
+        const float cap = a.o.softcap / a.o.scale, u_in = paged_cap_in(a.o);   // the cap in the product's units, its inverse
         float* row_max = (float*)(pf_smem + C::ROW_MAX);     // one row tile only
         int uses = 0;                                        // of this warpgroup's score buffer
         int turns = 0, done0 = 0, done1 = 0, last0 = 0, last1 = 0, meets = 0;  // phases the barriers have gone through
@@ -390,14 +397,42 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                 pf_ld_wait();
                 const int k0 = tile_at(j) * BN;
                 if (FEAT & 1) {
-                    // cap tanh(x scale / cap) = cap (1 - 2 / (1 + e^(2 x scale / cap)))
+                    // cap tanh(u), u = x / cap. Where |u| < CAP_NEAR: x + x u^2 P(u^2), with P the fit of (tanh(u) / u - 1) / u^2 of least
+                    // error over the range (2^-24.5 of tanh u, 2^-23.4 with the f32 roundings): an error relative to the score, however large the cap.
+                    // Beyond: cap (1 - 2 / (1 + e^2u)), which is off by 1.6 * 2^-23 of the cap, there 2^-20.5 of the score.
+                    float top[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int x = 0; x < BN; x++) s[x] = fmaf(-2.0f * cap2, rcp_approx(1.0f + ex2(s[x] * cin)), cap2);
+                    for (int x = 0; x < BN; x += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) top[e] = max3(top[e], fabsf(s[x + e]), fabsf(s[x + 4 + e]));
+                    const bool near = fmaxf(max3(top[0], top[1], top[2]), top[3]) * u_in < CAP_NEAR;
+                    const uint64_t in2 = pack2(u_in, u_in);
+                    const uint64_t p1 = pack2(-0.33333287f, -0.33333287f), p2 = pack2(0.13323873f, 0.13323873f), p3 = pack2(-0.051132675f, -0.051132675f);
+                    auto small = [&](float x0, float x1, float& y0, float& y1) {
+                        const uint64_t x = pack2(x0, x1), u = mul2(x, in2), w = mul2(u, u);
+                        unpack2(fma2(x, mul2(w, fma2(w, fma2(w, p3, p2), p1)), x), y0, y1);
+                    };
+                    if (__all_sync(0xffffffffu, near)) {
+#pragma unroll
+                        for (int x = 0; x < BN; x += 2) small(s[x], s[x + 1], s[x], s[x + 1]);
+                    } else {
+                        const float e_in = 2.0f * LOG2E * u_in;
+#pragma unroll
+                        for (int x = 0; x < BN; x += 2) {
+                            float y[2];
+                            small(s[x], s[x + 1], y[0], y[1]);
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                const float far = fmaf(-2.0f * cap, rcp_approx(1.0f + ex2(s[x + e] * e_in)), cap);
+                                s[x + e] = fabsf(s[x + e]) * u_in < CAP_NEAR ? y[e] : far;
+                            }
+                        }
+                    }
                 }
                 if (FEAT & 2) {
                     const float gap = (float)(qpos - k0);
 #pragma unroll
-                    for (int x = 0; x < BN; x++) s[x] = fmaf(-slope, fabsf(gap - (float)x), FEAT & 1 ? s[x] : s[x] * cin);
+                    for (int x = 0; x < BN; x++) s[x] = fmaf(-slope, fabsf(gap - (float)x), s[x] * c_in);
                 }
                 const bool all = !live || k0 + BN <= pre || (k0 >= klo && k0 + BN <= khi);
                 if (!__all_sync(0xffffffffu, all)) {
