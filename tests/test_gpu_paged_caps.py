@@ -88,3 +88,24 @@ def test_prefill_caps_far_from_and_near_the_scores_in_one_tile(lthn):
     want, wl, mag = attention(c, 0, x, 60, 260, **kws[0])
     close(got, want, 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 24 * W) * mag)      # |q| up to 4 and |k| up to 6 times larger
     same_lse(lse, wl, 24)
+
+
+@pytest.mark.parametrize("cap", [63.0, 64.0, 65.0, 100.0, 1000.0])
+@pytest.mark.parametrize("D,slopes", [(64, False), (128, True), (256, False)])
+def test_prefill_scores_around_a_large_cap(lthn, cap, D, slopes):
+    """The same around the caps where the form changes: scores from hundredths to several times of 30."""
+    rng = np.random.default_rng(45)
+    c = HostCache(rng, [260, 70], 16, 1, D)
+    for s, n in enumerate(c.lens):
+        k, v = c.get(s, n)
+        k[::9] *= 6.0
+        c.put(s, np.arange(n), k, v)
+    o, kws = options(lthn, rng, 2, c.lens, softcap=cap, slopes=slopes)
+    new = [200, 70]
+    q = rng.standard_normal((270, 2, D)) * 2.0 ** rng.uniform(-6, 3, (270, 1, 1))
+    x, got, lse, start = run_prefill(lthn, c, q, new, o)
+    for s, n in enumerate(c.lens):
+        rows = slice(start[s], start[s + 1])
+        want, wl, mag = attention(c, s, x[rows], n - new[s], n, **kws[s])
+        close(got[rows], want, 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 48 * W) * mag)      # |q| up to 8 and |k| up to 6 times larger
+        same_lse(lse[rows], wl, 48)
