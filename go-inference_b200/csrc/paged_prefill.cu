@@ -38,8 +38,9 @@
 // Where there are few items the keys of a tile are cut into chunks, which leave (maximum, sum, unnormalised output)
 // in the workspace for a second kernel to join.
 //
-// Every wait is bounded: on a time-out the roles record it in the device status word, drain what they have in flight, free
-// the tensor memory and return.
+// Every wait is bounded: on a time-out the roles record it in the device status word and leave; when all have, the loaders wait for the
+// boxes and the answer that are still on their way to this CTA's shared memory and the issuer for its products, then the tensor memory is
+// freed and the CTA returns.
 #include "paged.cuh"
 
 #include <cuda.h>
@@ -70,6 +71,7 @@ struct PrefillArgs {
     int chunks;          // chunks per row tile and kv head
     int chunk_tiles;     // key tiles per chunk, unless the lengths call for others
     int levels, sms;     // key tiles of max_ctx
+    int give_up;         // tests: a role that never starts (1 softmax, 2 issuer, 3 one of the loaders), so that the others' waits run out
     float4* part;        // [tiles*kv_heads*chunks][D/4][rows] unnormalised outputs, four columns each
     float2* ml;          // [tiles*kv_heads*chunks][rows] maximum (log2 units) and sum
     int4* desc;          // [tiles] sequence, tile of the sequence, chunks in use
@@ -304,7 +306,9 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
     uint32_t* tmem_slot = (uint32_t*)(answered + 1);
     unsigned char* answer = pf_smem + C::BARS + 320;         // 16 bytes
     PfItem* items = (PfItem*)(answer + 16);                  // [2]
-    static_assert((2 * ST + 23) * 8 + 8 <= 320 && 336 + 2 * sizeof(PfItem) <= 512, "barriers and items");
+    int* gave_up = (int*)(items + 2);                        // [8] whether a role has; then, of each loader warp that has left, the ring slots and
+                                                             //     the queries it had arrived for; the question without an answer, -1: none
+    static_assert((2 * ST + 23) * 8 + 8 <= 320 && 336 + 2 * sizeof(PfItem) + 32 <= 512, "barriers, items and what is left behind");
 
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     pdl_trigger();                                           // of the join, which waits for the end of this grid
@@ -324,6 +328,8 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         mbar_init(meet, C::SM_WARPS * 32);
         mbar_init(drain, 1);
         mbar_init(answered, 1);
+        gave_up[0] = 0;
+        for (int x = 1; x < 8; x++) gave_up[x] = -1;
         mbar_fence_init();
     }
     if (warp == C::SM_WARPS) pf_tmem_alloc(tmem_slot, 512);
@@ -369,6 +375,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         float* row_max = (float*)(pf_smem + C::ROW_MAX);     // one row tile only
         int uses = 0;                                        // of this warpgroup's score buffer
         int turns = 0, done0 = 0, done1 = 0, last0 = 0, last1 = 0, meets = 0;  // phases the barriers have gone through
+        if (a.give_up == 1) ok = false;
         auto pair_sync = [&] {
             pf_arrive(meet);
             const bool met = __all_sync(0xffffffffu, paged_wait(meet, meets++ & 1));
@@ -588,7 +595,10 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             }
             if (!two && n > 0) pair_sync();                      // both have read O before the next item's first weights let it be replaced
         }
-        if (!ok && lane == 0) atomicOr(a.wait_status, 1u << 26);
+        if (!ok && lane == 0) {
+            gave_up[0] = 1;
+            atomicOr(a.wait_status, 1u << 26);
+        }
     } else if (warp == C::SM_WARPS) {
         // ================================ issuer ================================
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
@@ -597,6 +607,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
         const uint32_t idesc_s = idesc | ((uint32_t)(BN >> 3) << 17), idesc_o = idesc | (1u << 16) | ((uint32_t)(D >> 3) << 17);
         int slot0 = 0, seen = 0;                             // ring slots and items with keys so far
         uint32_t uses = 0;                                   // bit b: parity of the uses of score buffer b
+        if (a.give_up == 2) ok = false;
         while (ok && next_item()) {
             const bool two = t.two;
             const int n = t.n, units = two ? 2 * n : n;
@@ -638,10 +649,9 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             slot0 += 2 * n;
             seen++;
         }
-        if (!ok) {
-            if (lane == 0) atomicOr(a.wait_status, 1u << 25);
-            pf_commit(drain);                                // nothing of this CTA may still run when its memory is given back
-            paged_wait(drain, 0);
+        if (!ok && lane == 0) {
+            gave_up[0] = 1;
+            atomicOr(a.wait_status, 1u << 25);
         }
         __syncwarp();
     } else {
@@ -745,7 +755,10 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                 }
                 __syncwarp();
                 ok = ok && __all_sync(0xffffffffu, paged_wait(answered, asked & 1));
-                if (!ok) return;
+                if (!ok) {
+                    if (lane == 0) gave_up[7] = asked;
+                    return;
+                }
                 asked++;
                 const int id = paged_cancelled(answer);
                 __syncwarp();
@@ -780,6 +793,7 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             if (look_up(blockIdx.x, x)) publish(x);
             else find_next();
         }
+        if (a.give_up == 3 && lw == 1) ok = false;
         while (ok && next_item()) {
             const int n = t.n, len = t.len, prefix = t.prefix, qhi = t.qhi;
             if (n == 0) {
@@ -795,8 +809,12 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                 const int rr = row_of(x), key = tile_at(j) * BN + rr;
                 return x < NX && rr < BN && key < len && (key < prefix || (key >= lo && key <= qhi)) ? key : -1;
             };
+            auto left_at = [&](int slot, int queries) {
+                if (lane == 0) { gave_up[1 + lw] = slot; gave_up[4 + lw] = queries; }
+            };
             auto free_slot = [&](int slot) {
                 ok = __all_sync(0xffffffffu, paged_wait(&empty[slot % ST], ((slot / ST) & 1) ^ 1));
+                if (!ok) left_at(slot, slot > slot0 ? seen + 1 : seen);   // (slots are filled in their order, the queries come behind the first)
                 return ok;
             };
             // ---- row by row ----
@@ -885,7 +903,10 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
                     while (handed < slot0 + k_slot(0) + 1) pf_arrive(&full[handed++ % ST]);
                 }
                 ok = __all_sync(0xffffffffu, paged_wait(q_empty, (seen & 1) ^ 1));
-                if (!ok) return;
+                if (!ok) {
+                    left_at(slot0 + 1, seen);
+                    return;
+                }
                 const int row_tiles = t.two ? 2 : 1;
                 if (a.q_box) {                                   // tokens behind the sequence's last are somebody else's, or zeros: never stored
                     if (lw == 0 && lane < row_tiles * (D / 64)) {
@@ -986,12 +1007,37 @@ __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(con
             pf_fence_async();
             while (handed < slot0) pf_arrive(&full[handed++ % ST]);
         } else if (!ok && lane == 0) {
+            gave_up[0] = 1;
             atomicOr(a.wait_status, 1u << 24);
         }
+        if (lane == 0 && gave_up[1 + lw] < 0) { gave_up[1 + lw] = slot0; gave_up[4 + lw] = seen; }   // it left between two items
         __syncwarp();
     }
     pf_fence_before();
     __syncthreads();
+    if (gave_up[0]) {
+        // Nothing of this CTA may still run or be written when its memory is given back. A phase of `full` takes the arrivals of all
+        // three warps: those that left earlier make up for what the others have arrived for since. That is at most ST slots, one of each
+        // stage, and one item's queries: a stage is filled again, as are the queries, only after all three had arrived for it.
+        if (warp == C::SM_WARPS) {
+            pf_commit(drain);                                // all products
+            paged_wait(drain, 0);
+        } else if (warp > C::SM_WARPS) {
+            const int lw = warp - C::SM_WARPS - 1, *slots = gave_up + 1, *queries = gave_up + 4;
+            if (a.box) {                                     // (rows copied one by one have been waited for)
+                const int last = max(slots[0], max(slots[1], slots[2]));
+                for (int s = slots[lw]; s < last; s++) pf_arrive(&full[s % ST]);
+                for (int s = max(last - ST, 0); s < last; s++) paged_wait(&full[s % ST], (s / ST) & 1);
+            }
+            if (a.q_box) {
+                const int last = max(queries[0], max(queries[1], queries[2]));
+                if (queries[lw] < last) pf_arrive(q_full);
+                if (last > 0) paged_wait(q_full, (last - 1) & 1);
+            }
+            if (lw == 2 && gave_up[7] >= 0) paged_wait(answered, gave_up[7] & 1);
+        }
+        __syncthreads();
+    }
     if (warp == C::SM_WARPS) pf_tmem_dealloc(tmem, 512);
 }
 
@@ -1132,6 +1178,8 @@ static bool prefill_q_map(const PrefillArgs& a, int D, CUtensorMap* qm) {
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+LTHN_HIDDEN int g_paged_give_up = 0;  // PrefillArgs::give_up: zero in the product library (setter: test_hooks.cu)
+
 template <int D, int FEAT>
 static int32_t launch_prefill(cudaStream_t s, PrefillArgs a) {
     using C = PfCfg<D>;
@@ -1235,6 +1283,7 @@ int32_t lthn_paged_prefill_attention(void* stream, const lthn_paged_kv* cache, c
     a.seqs = seqs; a.total_q = total_q; a.Hq = q_heads; a.G = q_heads / cache->kv_heads;
     a.tokens = 128 / a.G;
     a.tiles = p.tiles; a.chunks = p.chunks; a.chunk_tiles = p.chunk_tiles; a.levels = p.levels; a.sms = paged_sm_count();
+    a.give_up = g_paged_give_up;
     a.part = (float4*)workspace;
     a.ml = (float2*)((char*)workspace + p.part);
     a.desc = (int4*)((char*)workspace + p.part + p.ml);

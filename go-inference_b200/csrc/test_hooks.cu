@@ -10,6 +10,7 @@
 namespace lthn {
 extern LTHN_HIDDEN int g_force_rt, g_force_warps, g_force_kernel;  // qmv.cu
 extern LTHN_HIDDEN int g_force_nt;                                 // qmm.cu
+extern LTHN_HIDDEN int g_paged_give_up;                            // paged_prefill.cu
 }  // namespace lthn
 
 using namespace lthn;
@@ -29,6 +30,9 @@ void lthn_debug_qmv_force_kernel(int32_t kernel) {
     g_i8_stg = (kernel >> 8) & 7;
 }
 void lthn_debug_qmm_force_tile(int32_t nt) { g_force_nt = nt; }
+// A role of lthn_paged_prefill_attention that does not start (1 softmax, 2 issuer, 3 one of the three loaders, 0 none): the waits of the
+// others run out, within a few tenths of a second per block.
+void lthn_debug_paged_prefill_give_up(int32_t role) { g_paged_give_up = role; }
 
 // The plan the integer tensor-core matvec would run for a call (host logic only, no CUDA call): returns 1 and
 // out = {J, W, stg, RS, nblocks, threads, bs_off, stage_off, ks, Gs, fuse, smem bytes}, or 0 when the kernel
