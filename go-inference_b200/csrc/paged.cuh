@@ -3,6 +3,8 @@
 #pragma once
 #include "common.cuh"
 
+#include <initializer_list>
+
 namespace lthn {
 
 // lthn_paged_kv with its default strides filled in.
@@ -31,8 +33,15 @@ struct AttnOpts {
 // Host: checks of the arguments every call has, and the fill-in. `name` is the entry point, for messages.
 int32_t paged_check_cache(const char* name, const lthn_paged_kv* c, PagedCache* out);
 int32_t paged_check_options(const char* name, const lthn_attn_options* o, int head_dim, AttnOpts* out);
-// the pointer is device memory of the current device (a host pointer or another GPU's would fault in the kernel)
-int32_t paged_check_device(const char* name, const char* what, const void* p);
+// An argument that the kernels read or write through. NULL ones are skipped: the optional arguments.
+struct PagedPtr {
+    const char* what;
+    const void* p;
+    int align;           // bytes
+    bool pinned;         // page-locked host memory serves too (not where TMA or wide copies go through it)
+};
+// Every pointer is aligned and memory that the current device can reach: a host pointer or another GPU's would fault in the kernel.
+int32_t paged_check_pointers(const char* name, std::initializer_list<PagedPtr> list);
 int paged_sm_count();
 
 #ifdef __CUDACC__

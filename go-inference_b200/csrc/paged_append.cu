@@ -19,6 +19,8 @@
 // there to [-1/2, 1/2], and handed to sincospif.
 #include "paged.cuh"
 
+#include <cuda.h>
+
 #include <algorithm>
 
 namespace lthn {
@@ -31,16 +33,47 @@ int paged_sm_count() {
     return sms;
 }
 
-int32_t paged_check_device(const char* name, const char* what, const void* p) {
-    cudaPointerAttributes at;
+typedef CUresult (*PointerAttributes)(unsigned, CUpointer_attribute*, void**, CUdeviceptr);
+static PointerAttributes pointer_attributes() {
+    static PointerAttributes fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        return cudaGetDriverEntryPoint("cuPointerGetAttributes", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess
+                   ? (PointerAttributes)p : nullptr;
+    }();
+    return fn;
+}
+
+int32_t paged_check_pointers(const char* name, std::initializer_list<PagedPtr> list) {
+    for (const PagedPtr& x : list)
+        if ((uintptr_t)x.p & (x.align - 1)) return fail(LTHN_ERR_INVALID, named(name, x.what) + " must be " + std::to_string(x.align) + "-byte aligned");
     int dev = 0;
     LTHN_CUDA_TRY(cudaGetDevice(&dev));
-    if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
-        cudaGetLastError();
-        return fail(LTHN_ERR_INVALID, named(name, what) + " is not a pointer CUDA knows");
+    if (!pointer_attributes()) return fail(LTHN_ERR_CUDA, named(name, "the driver has no pointer queries"));
+    // A query takes about 45 ns of the host; arguments within an allocation that has been looked up are not asked for again.
+    uintptr_t begin[4] = {}, end[4] = {};
+    int known = 0;
+    for (const PagedPtr& x : list) {
+        const uintptr_t p = (uintptr_t)x.p;
+        bool done = !p;
+        for (int i = 0; i < std::min(known, 4); i++) done |= p >= begin[i] && p < end[i];
+        if (done) continue;
+        unsigned type = 0, managed = 0;
+        int at = -1;
+        CUdeviceptr device_ptr = 0, start = 0;
+        size_t bytes = 0;
+        CUpointer_attribute what[6] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_IS_MANAGED, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL,
+                                       CU_POINTER_ATTRIBUTE_DEVICE_POINTER, CU_POINTER_ATTRIBUTE_RANGE_START_ADDR, CU_POINTER_ATTRIBUTE_RANGE_SIZE};
+        void* into[6] = {&type, &managed, &at, &device_ptr, &start, &bytes};
+        if (pointer_attributes()(6, what, into, (CUdeviceptr)p) != CUDA_SUCCESS) type = managed = 0;
+        const bool here = managed || (type == CU_MEMORYTYPE_DEVICE && at == dev);
+        if (!here && !(x.pinned && type == CU_MEMORYTYPE_HOST && (uintptr_t)device_ptr == p))
+            return fail(LTHN_ERR_INVALID, named(name, x.what) + " is not memory of the current device");
+        if (here && bytes) {
+            begin[known % 4] = (uintptr_t)start;
+            end[known++ % 4] = (uintptr_t)start + bytes;
+        }
     }
-    if (at.type != cudaMemoryTypeManaged && (at.type != cudaMemoryTypeDevice || at.device != dev))
-        return fail(LTHN_ERR_INVALID, named(name, what) + " is not memory of the current device");
     return LTHN_OK;
 }
 
@@ -287,8 +320,12 @@ extern "C" int32_t lthn_paged_kv_append(void* stream, const lthn_paged_kv* cache
                  "paged_kv_append: q, k, v and q_out must be 16-byte aligned");
     LTHN_REQUIRE(!q_heads || q_out != q || (q_dtype == dtype && a.q_out_stride == a.q_stride),
                  "paged_kv_append: q_out may be q itself only with the same type and stride");
-    if ((rc = paged_check_device(me, "the cache", cache->k))) return rc;
-    if ((rc = paged_check_device(me, "k", k))) return rc;
+    if ((rc = paged_check_pointers(me, {{"the cache's k", cache->k, 16, false}, {"the cache's v", cache->v, 16, false},
+                                        {"page_table", cache->page_table, 4, true}, {"k", k, 16, false}, {"v", v, 16, true}, {"q", q_heads ? q : nullptr, 16, true},
+                                        {"q_out", q_heads ? q_out : nullptr, 16, true}, {"row_seq", row_seq, 4, true}, {"row_pos", row_pos, 4, true},
+                                        {"inv_freq", a.half_rot ? a.inv_freq : nullptr, 8, true}, {"q_norm", q_heads ? a.q_norm : nullptr, 16, true},
+                                        {"k_norm", a.k_norm, 16, true}})))
+        return rc;
     a.q = q; a.k = k; a.v = v; a.q_out = q_out; a.Hq = q_heads;
     a.row_seq = row_seq; a.row_pos = row_pos;
     a.c.status = device_paged_status_word();

@@ -782,8 +782,11 @@ int32_t lthn_paged_sdpa_decode(void* stream, const lthn_paged_kv* cache, const l
     LTHN_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15) == 0, "paged_sdpa_decode: q, out and workspace must be 16-byte aligned");
     const DecodePlan p = decode_plan(D, cache->kv_heads, rows, q_heads, dtype, a.c.capacity);
     LTHN_REQUIRE(workspace_bytes >= p.total, "paged_sdpa_decode: workspace too small");
-    if ((rc = paged_check_device(me, "the cache", cache->k))) return rc;
-    if ((rc = paged_check_device(me, "workspace", workspace))) return rc;
+    if ((rc = paged_check_pointers(me, {{"the cache's k", cache->k, 16, false}, {"the cache's v", cache->v, 16, false},
+                                        {"page_table", cache->page_table, 4, true}, {"q", q, 16, true}, {"kv_lens", kv_lens, 4, true}, {"out", out, 16, true},
+                                        {"lse", lse, 4, true}, {"workspace", workspace, 16, false}, {"slopes", a.o.slopes, 4, true},
+                                        {"prefix_lens", a.o.prefix, 4, true}})))
+        return rc;
     a.q = q; a.out = out; a.lens = kv_lens; a.lse = lse; a.rows = rows; a.Hq = q_heads; a.G = q_heads / cache->kv_heads;
     a.nb = p.nb; a.ctas = p.ctas;
     a.part = (float*)workspace;

@@ -1276,8 +1276,11 @@ int32_t lthn_paged_prefill_attention(void* stream, const lthn_paged_kv* cache, c
                                        a.o.prefix != nullptr);
     LTHN_REQUIRE((int64_t)p.tiles * cache->kv_heads * p.chunks < (int64_t)1 << 31, "paged_prefill_attention: too many query rows");
     LTHN_REQUIRE(workspace_bytes >= p.total, "paged_prefill_attention: workspace too small");
-    if ((rc = paged_check_device(me, "the cache", cache->k))) return rc;
-    if ((rc = paged_check_device(me, "q", q))) return rc;
+    if ((rc = paged_check_pointers(me, {{"the cache's k", cache->k, 16, false}, {"the cache's v", cache->v, 16, false},
+                                        {"page_table", cache->page_table, 4, true}, {"q", q, 16, false}, {"q_start", q_start, 4, true},
+                                        {"kv_lens", kv_lens, 4, true}, {"out", out, 16, true}, {"lse", lse, 4, true}, {"workspace", workspace, 16, false},
+                                        {"slopes", a.o.slopes, 4, true}, {"prefix_lens", a.o.prefix, 4, true}})))
+        return rc;
     a.out_sectors = (((uintptr_t)out | (uintptr_t)(a.out_stride * 2)) & 31) == 0;
     a.q = q; a.out = out; a.q_start = q_start; a.lens = kv_lens; a.lse = lse;
     a.seqs = seqs; a.total_q = total_q; a.Hq = q_heads; a.G = q_heads / cache->kv_heads;

@@ -280,8 +280,10 @@ int32_t lthn_prefill_attention(void* stream, const float* q, const uint16_t* kca
  * engine object; the reference keeps its paged forms inside its engines (engine/metal/kernels/
  * attention/lthn_sdpa_paged*.metal) and has no public counterpart.
  *
- * The struct and the option structs are read by the host during the call; the pointers in them are
- * device pointers of the current device. Row of position p of sequence s, kv head h:
+ * The struct and the option structs are read by the host during the call; the pointers in them and of the
+ * calls are device pointers of the current device (index arrays, norm weights, slopes, lse, v, q_out, out and but for the prompt
+ * call q may be page-locked host memory) on a multiple of their element's size; others are refused.
+ * Row of position p of sequence s, kv head h:
  *   page = page_table[s*table_stride + p / page_size],
  *   first element at k + page*page_stride + (p % page_size)*row_stride + h*head_stride (v alike).
  * So both [page][row][head][dim] (strides left 0) and [page][head][row][dim] (row_stride = head_dim,
