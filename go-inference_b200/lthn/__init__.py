@@ -567,6 +567,15 @@ def rope_inv_freq(base: float, head_dim: int, rotary_dim: int = 0) -> np.ndarray
 
 
 def rope_params(inv_freq=None, rotary_dim=0, interleaved=False, q_norm=None, k_norm=None, eps=1e-6) -> RopeParams:
+    """rotary_dim 0: a pair for every frequency inv_freq (f64) holds. No rotation: inv_freq None."""
+    if inv_freq is not None:
+        held = getattr(inv_freq, "nbytes", None)
+        if not rotary_dim:
+            if held is None:
+                raise LthnError(1, "rope_params: rotary_dim is needed for frequencies of unknown number")
+            rotary_dim = 2 * (held // 8)
+        elif held is not None and 8 * (rotary_dim // 2) > held:
+            raise LthnError(1, f"rope_params: {held // 8} frequencies for a rotary_dim of {rotary_dim}")
     p = RopeParams(_p(inv_freq), rotary_dim, int(interleaved), _p(q_norm), _p(k_norm), eps)
     p._keep = (inv_freq, q_norm, k_norm)
     return p

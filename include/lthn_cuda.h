@@ -329,7 +329,7 @@ typedef struct {
  * lthn_qknorm_rope_bf16.metal, engine/hip/kernels/norms/rms_norm.hipinc:306-377). */
 typedef struct {
     const double* inv_freq;     /* NULL: no rotation */
-    int32_t rotary_dim;         /* even, <= head_dim */
+    int32_t rotary_dim;         /* even, <= head_dim; 0: no rotation */
     int32_t interleaved;
     const float* q_norm;
     const float* k_norm;
