@@ -1128,6 +1128,9 @@ static PrefillPlan prefill_plan(int D, int kv_heads, int seqs, int total_q, int 
     const double longest = keys / bn, each = std::max(1.0, mean / bn), half = 0.5 * each * pairs / sms;
     p.chunks = (int)std::max(1.0, std::min(longest / std::max((pairs <= sms ? 256.0 : 512.0) / bn, half), 1024.0));
     p.chunk_tiles = std::max(1, (int)((longest + p.chunks - 1) / p.chunks));
+    // The other roles wait 0.2 s for the next item at the most. A look-up reads the sequences before the item's, 12 ns each, and of the up to
+    // 4 * 148 chunks one CTA may come upon all that are not there, one after another; without chunks each look-up finds an item.
+    if (seqs > 1 << 15) p.chunks = 1;
     if (pairs <= sms) p.chunk_tiles = std::max(p.chunk_tiles, (int)std::ceil(each / ((double)sms / pairs - 0.5)));   // a tile's last chunk is half full
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
     const size_t parts = p.chunks > 1 ? (size_t)pairs * p.chunks : 0;
@@ -1235,6 +1238,7 @@ static int32_t prefill_check(const lthn_paged_kv* cache, int32_t seqs, int32_t t
     if ((rc = paged_check_cache("paged_prefill_attention", cache, c))) return rc;
     LTHN_REQUIRE(seqs >= 0 && total_q >= 0 && max_ctx >= 0, "paged_prefill_attention: negative size");
     LTHN_REQUIRE(seqs <= cache->seqs, "paged_prefill_attention: more sequences than the page table has");
+    LTHN_REQUIRE(seqs <= 1 << 20, "paged_prefill_attention: at most 2^20 sequences");   // 12 ms a look-up
     LTHN_REQUIRE(q_heads > 0 && q_heads <= 65535 && q_heads % cache->kv_heads == 0, "paged_prefill_attention: q_heads must be a positive multiple of kv_heads");
     LTHN_REQUIRE(q_heads / cache->kv_heads <= 128, "paged_prefill_attention: at most 128 query heads per kv head");
     LTHN_REQUIRE(total_q <= 1 << 30, "paged_prefill_attention: too many query rows");
@@ -1274,7 +1278,8 @@ int32_t lthn_paged_prefill_attention(void* stream, const lthn_paged_kv* cache, c
     LTHN_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15) == 0, "paged_prefill_attention: q, out and workspace must be 16-byte aligned");
     const PrefillPlan p = prefill_plan(D, cache->kv_heads, seqs, total_q, q_heads, max_ctx ? std::min(max_ctx, a.c.capacity) : a.c.capacity, a.o.window,
                                        a.o.prefix != nullptr);
-    LTHN_REQUIRE((int64_t)p.tiles * cache->kv_heads * p.chunks < (int64_t)1 << 31, "paged_prefill_attention: too many query rows");
+    // more than the queries of a whole device's memory come to; items that are not there take a CTA 1 us each, 0.1 s in all
+    LTHN_REQUIRE((int64_t)p.tiles * cache->kv_heads * p.chunks < 1 << 24, "paged_prefill_attention: too many query rows or sequences");
     LTHN_REQUIRE(workspace_bytes >= p.total, "paged_prefill_attention: workspace too small");
     if ((rc = paged_check_pointers(me, {{"the cache's k", cache->k, 16, false}, {"the cache's v", cache->v, 16, false},
                                         {"page_table", cache->page_table, 4, true}, {"q", q, 16, false}, {"q_start", q_start, 4, true},

@@ -384,7 +384,8 @@ int32_t lthn_paged_sdpa_decode(void* stream, const lthn_paged_kv* cache, const l
  * right. Lengths are read on the device and few rows are cut by the lengths themselves, so a captured call replays with new
  * ones and a generous max_ctx costs workspace, not time. A NaN or infinity in a
  * value row that some query of a tile sees may reach the other queries of that tile (up to 256 rows of tokens times
- * query heads of a kv head). At most 128 query heads per kv head. Workspace and strides as above. */
+ * query heads of a kv head). At most 128 query heads per kv head, 2^20 sequences (more than 2^15 are not cut) and 2^24 pairs of
+ * a kv head and a tile of up to 256 rows, of which every sequence may begin one. Workspace and strides as above. */
 int32_t lthn_paged_prefill_attention_workspace(const lthn_paged_kv* cache, int32_t seqs, int32_t total_q, int32_t q_heads, int32_t max_ctx,
                                                size_t* bytes);
 int32_t lthn_paged_prefill_attention(void* stream, const lthn_paged_kv* cache, const lthn_attn_options* options, const uint16_t* q,
