@@ -11,7 +11,7 @@
 // one token row: its D/2 angles are formed once, by one thread each, and read by all of the row's heads. Position, page,
 // angles and norm are a chain of latencies, so what counts is how many rows an SM has at work: the first heads are loaded before
 // position and page are known, and CTAs are small (8190 rows of 64 heads of 128, bf16, 268 MB: 64 us with 4 CTAs of 256 threads per SM,
-// 53.5 us = 5.0 TB/s with 10 of 128; fetching the next row under this one instead: 67 us; 8 elements a
+// 53.5 us = 5.0 TB/s with 10 of 128, which leaves 48 registers and spills 8 bytes, 24 to 32 with f32 queries out; fetching the next row under this one instead: 67 us; 8 elements a
 // thread and half the threads: 60 us). For a few rows the chain is all
 // there is, and a row's heads are shared between CTAs (1 row of 16 heads of 256, f32: 3.9 us, shared 3.4; 64 rows of 48 heads
 // of 128, bf16: 3.3, 2.6). The angle is the only place

@@ -706,6 +706,8 @@ static int32_t launch_decode_kernel(cudaStream_t s, const DecodeArgs& a) {
 // many take as long as the join (8 triples, head_dim 128, bf16: 512 keys 7.0 us in even shares, 4.6 in clusters of 8; 2048 keys 8.6, 7.9; 4096
 // keys 10.9, 11.5). For up to 4 triples with more than a piece for each of 8 CTAs the clusters have 16 (4 triples, head_dim 256, f32: 512
 // keys 8.9 us, of 8 6.5, of 16 7.1; 1280 keys 10.8, 10.3, 8.9; 2048 keys 10.7, 12.3, 8.8; 8 triples, head_dim 128, 1280 keys: 8.7, 6.7, 7.4).
+// "Can have" is by the table and the window, not by the lengths, which the host does not know: 4 triples of head_dim 256 take the list under tables of
+// more than about 3600 rows, 8 of head_dim 128 from about 2600 on, however short their sequences are.
 template <int D>
 static int decode_cluster(const DecodeArgs& a) {
     const int64_t triples = (int64_t)a.rows * a.c.kv_heads * a.nb;

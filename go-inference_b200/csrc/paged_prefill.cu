@@ -23,7 +23,12 @@
 //                   dimensions and gcd(page size, BN) rows. V rows that nobody sees must be zeros (they may hold NaN,
 //                   which a weight of zero would not silence), so a V tile with such rows - the last of a sequence, the
 //                   first of a window - and pools of other page sizes come row by row with cp.async of 16 bytes,
-//                   zero-filled; unseen K rows may hold anything, their scores are replaced. 8192 tokens of 32 heads: 1007 us with cp.async throughout, 541 us with TMA.
+//                   zero-filled; unseen K rows may hold anything, their scores are replaced. 8192 tokens of 32 heads: 1007 us with cp.async throughout, 541 us with TMA
+//                   as it was then; pages of other sizes still cost about twice.
+//
+// Weights are rounded to bf16 (2^-8 each, the size of the rounding of the output) because the second product takes one type for both operands
+// and V is bf16; a second product with the remainders, as in the one-token kernel, would cost half as much again of what bounds long prompts.
+// The sums take the weights before that rounding.
 //
 // The running maximum is only moved when a row's grew by more than 2^8: until then weights are up to 2^8, which neither
 // their bf16 rounding (relative) nor the f32 sums mind, and O in tensor memory needs no correction. A move multiplies
@@ -280,6 +285,7 @@ struct PfCfg {
 constexpr float CAP_SMALL = 64.0f, CAP_NEAR = 0.3f;
 
 // FEAT bit 0: tanh cap of at most CAP_SMALL, bit 1: distance bias, bit 2: a larger cap
+// 168 registers a thread at launch, and spills of 48 to 260 bytes; head_dim 64 under a large cap has the most.
 template <int D, int FEAT>
 __global__ void __launch_bounds__(PfCfg<D>::THREADS, 1) paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                                                                        const __grid_constant__ CUtensorMap v_map, const PrefillArgs a) {

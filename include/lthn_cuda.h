@@ -289,8 +289,10 @@ int32_t lthn_prefill_attention(void* stream, const float* q, const uint16_t* kca
  * So both [page][row][head][dim] (strides left 0) and [page][head][row][dim] (row_stride = head_dim,
  * head_stride = page_size*head_dim) pools are served, as are pools that hold K and V side by side.
  * k and v are 16-byte aligned and the strides multiples of 8 elements. Offsets are 64 bits wide.
- * No call reads a row at or behind a sequence's length, nor a page it does not need: what lies there
- * (NaN, stale rows, table entries of any value) does not matter.
+ * Rows at or behind a sequence's length and pages that a call does not need have no influence on it (NaN, stale rows, table
+ * entries of any value): value rows there are not read, key rows of a page that holds others of the sequence may be, their
+ * scores are replaced. A page size that is a multiple of 8 rows is the one to take: prompts read the pages of others row by row, at
+ * about half the speed.
  *
  * Errors the host cannot see: a page table entry outside [0, pages), a position or length beyond the
  * table's table_stride*page_size rows, a sequence number >= seqs or a decreasing q_start sets bit
@@ -361,11 +363,14 @@ typedef struct {
  * position kv_lens[r]-1 of sequence r of the page table and attends to its kv_lens[r] rows (its own
  * included: append first); kv_lens[r] <= 0 is an empty row. q_heads is a multiple of kv_heads, head
  * map as lthn_sdpa_decode. dtype is the type of q and out: f32 computes at f32 grade (the keys and values
- * are exact in bf16 and the products of q and of the weights with them are not rounded), bf16 rounds the weights and the result.
+ * are exact in bf16 and the products of q and of the weights with them are not rounded), bf16 rounds the weights (with more than 8 query
+ * heads per kv head to bf16, else to 2^-16) and the result. Queries and weights are split into bf16 parts for that, of which some are zero: an
+ * infinity in a visible value, and with f32 in a visible key, gives NaN.
  * Lengths are read on the device, so a captured call replays with new ones. All work of the call is one list of
  * 64-key pieces of all rows, dealt out evenly over the GPU: no bound on the lengths is needed and a long
  * row does not wait for its own block. (A few rows that the table or the window keep short take one launch
- * instead, a cluster of blocks per row and kv head.) workspace: device memory of
+ * instead, a cluster of blocks per row and kv head: up to 16 of them, by table_stride * page_size and the window, whatever the
+ * lengths are.) workspace: device memory of
  * lthn_paged_sdpa_decode_workspace bytes, 16-byte aligned, uninitialised; nothing is kept in it between
  * calls, but calls that can overlap (two streams, two captured graphs) need one each. Strides are
  * elements between rows (0 -> dense), multiples of 8; q and out 16-byte aligned. At most 65535 rows. */
@@ -381,8 +386,8 @@ int32_t lthn_paged_sdpa_decode(void* stream, const lthn_paged_kv* cache, const l
  * lse; a sequence with more query rows than positions has empty rows in front. Scores and sums are f32, the weights
  * are rounded to bf16 for the second product, as in lthn_prefill_attention. max_ctx (0: the table's rows) bounds
  * kv_lens: it decides how finely a long context can be cut, and with it the workspace; longer sequences are still computed
- * right. Lengths are read on the device and few rows are cut by the lengths themselves, so a captured call replays with new
- * ones and a generous max_ctx costs workspace, not time. A NaN or infinity in a
+ * right. Lengths are read on the device, so a captured call replays with new ones. With up to 32 sequences few rows are cut by the lengths
+ * themselves, and a generous max_ctx costs workspace, not time; with more the cut follows max_ctx. A NaN or infinity in a
  * value row that some query of a tile sees may reach the other queries of that tile (up to 256 rows of tokens times
  * query heads of a kv head). At most 128 query heads per kv head, 2^20 sequences (more than 2^15 are not cut) and 2^24 pairs of
  * a kv head and a tile of up to 256 rows, of which every sequence may begin one. Workspace and strides as above. */
